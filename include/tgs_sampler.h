@@ -71,7 +71,7 @@ typedef enum {
   TGS_ETOOBIG = -5     /* size beyond what the handle was created for     */
 } tgs_status;
 
-typedef enum { TGS_F32 = 0, TGS_BF16 = 1 } tgs_dtype;
+typedef enum { TGS_F32 = 0, TGS_BF16 = 1, TGS_F16 = 2 /* key/value caches only */ } tgs_dtype;
 
 #define TGS_FLAG_GREEDY 1 /* decode this row by argmax regardless of T */
 
@@ -253,6 +253,135 @@ int tgs_mask_rows_from_dfa(tgs_handle h, const uint8_t* d_byte_class, const int3
  * bounded by the handle's limits (no per-row workspace beyond a few bytes). */
 int tgs_token_logprobs(tgs_handle h, const void* d_logits, tgs_dtype dt, int B, int V, int64_t row_stride,
                        const int32_t* d_tokens, float* d_out_logprob, float* d_out_lse, tgs_stream stream);
+
+/* ------------------------------------------------------------------------
+ * Beam search and tree speculation over a paged key/value cache: what runs
+ * around the sampler in a decode step.  The reference keeps one contiguous
+ * cache per conversation (KVCache, native-mac/Sources/TinyGPTModel) and has
+ * no counterpart of these calls.
+ *
+ * They check what the host can see, allocate nothing, use the handle's
+ * workspace (order calls on one handle on one stream) and can be captured
+ * into a graph.  Lengths, page tables and parents are device data; an entry
+ * that points outside what the arguments describe is never followed, and is
+ * reported in the outputs as each call says. */
+
+/* A cache of `layers` layers over one pool of pages (all strides in
+ * elements, multiples of 8; k and v 16-byte aligned):
+ *   k [layers][n_pages][kv_heads][page][head_dim]
+ *   v [layers][n_pages][kv_heads][page / 8][head_dim][8]
+ * the eight tokens of a block of values lie next to each other for each
+ * element of the head, as the attention's second product takes them.
+ * k_layer, k_page, v_layer, v_page are the distances between layers and
+ * between pages; a page is contiguous.  Token t of a sequence is slot
+ * t % page of page tables[sequence][t / page]. */
+typedef struct {
+  void* k;
+  void* v;
+  int64_t k_layer, k_page, v_layer, v_page;
+  int32_t layers, n_pages;
+  int32_t page;     /* tokens of a page: a power of two, 8 to 1024 */
+  int32_t kv_heads;
+  int32_t head_dim; /* a multiple of 8; kv_heads * head_dim < 65536 */
+  int32_t dtype;    /* TGS_BF16 or TGS_F16 */
+} tgs_kv_cache;
+
+/* New keys and values, [layers][B][T][kv_heads][head_dim] with any strides
+ * (in elements); head_dim is contiguous.  No alignment is asked for. */
+typedef struct {
+  const void* k;
+  const void* v;
+  int64_t k_layer, k_seq, k_tok, k_head;
+  int64_t v_layer, v_seq, v_tok, v_head;
+} tgs_kv_rows;
+
+/* The sequences of a call: page tables [B][width] and lengths [B] (tokens in
+ * the cache). */
+typedef struct {
+  const int32_t* tables;
+  const int32_t* lens;
+  int32_t B, width;
+} tgs_kv_seqs;
+
+/* Selects from each of G requests with W beams the n_out best continuations
+ *   scores[g W + w] + x[g W + w][v] - logsumexp(x[g W + w])
+ * over beams w and ids v, in descending order, equal ones by the lower beam,
+ * then the lower id.  Logits as in tgs_sample (NaN and -inf logits are not
+ * selected).  Totals are compared in 64 bits.  A beam whose score is not
+ * finite (-inf: it has ended) or whose row holds +inf or nothing gives no
+ * candidates; outputs past the last candidate are -inf, -1, -1 and an empty
+ * history.
+ *   d_scores     [G W]
+ *   d_hist       [G W][hist_cap] with d_hist_len [G W], nullable with
+ *                hist_cap 0: ids so far, oldest first
+ *   d_out_scores, d_out_parents (row g W + w), d_out_tokens  [G n_out]
+ *   d_out_hist   [G n_out][hist_cap], d_out_hist_len: the parent's history and
+ *                the new id, the oldest dropped when it is full, -1 padded
+ * W and n_out at most 64, n_out <= W V; outputs must not overlap inputs. */
+int tgs_beam_select(tgs_handle h, const void* d_logits, tgs_dtype dt, int G, int W, int V, int64_t row_stride,
+                    const float* d_scores, int n_out, const int32_t* d_hist, const int32_t* d_hist_len, int hist_cap,
+                    float* d_out_scores, int32_t* d_out_parents, int32_t* d_out_tokens, int32_t* d_out_hist,
+                    int32_t* d_out_hist_len, tgs_stream stream);
+
+/* Queries of T drafted nodes per sequence (T = 1: a decode step). */
+typedef struct {
+  const void* q; /* [B][T][q_heads][head_dim], strides in elements, head_dim contiguous */
+  int64_t q_seq, q_tok, q_head;
+  const int32_t* parents; /* [B][T] node each one follows: an earlier one, or -1 (a root); nullable: a chain */
+  void* out;              /* [B][T][q_heads][head_dim] in the cache's type, 16-byte aligned */
+  float* lse;             /* [B][T][q_heads] natural logsumexp of the scaled scores; nullable */
+  int32_t T, q_heads;     /* 1 <= T <= 64; q_heads a multiple of kv_heads */
+  int32_t max_len;        /* a bound of lens that the host knows (sizes the launch; longer ones stay right) */
+  float scale;            /* > 0 */
+} tgs_attn;
+
+/* Attention of each drafted node over its sequence's cache (every token), its
+ * ancestors and itself, q_heads / kv_heads query heads to a key head.  cache:
+ * one layer (layers 1); head_dim 64, 96, 128 or 256; rows: the nodes' own
+ * keys and values (layer strides unused), read beside the cache, not written
+ * to it.  A sequence of which a page lies outside the pool gives NaN; lengths are taken
+ * within [0, width page].  What the cache's pages hold past a sequence's end
+ * is never used.  Products and sums are 32-bit; softmax weights are rounded
+ * to the cache's type before they multiply values. */
+int tgs_tree_attention(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs,
+                       const tgs_attn* attn, tgs_stream stream);
+
+/* Writes rows i < counts[b] of sequence b (T for all when d_counts is NULL)
+ * to positions lens[b] + i in every layer, and d_lens_out[b] = lens[b] +
+ * counts[b].  A sequence whose rows do not fit (a count outside [0, T], a
+ * position past its table, a page outside the pool) keeps its cache and gets
+ * -1.  Tables of different sequences must not name one page where rows are written. */
+int tgs_kv_append(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs, int T,
+                  const int32_t* d_counts, int32_t* d_lens_out, tgs_stream stream);
+
+/* Accepts and commits a drafted tree per sequence: from node 0 (the root,
+ * whose token is already decided) the path goes on to the lowest child whose
+ * drafted token d_draft[b][child] is d_sampled[b][node], the id that the
+ * target model samples after the node; the path's keys and values are written
+ * as tgs_kv_append writes rows.
+ *   d_parents, d_draft, d_sampled [B][T], 1 <= T <= 64 (a parent is an earlier node)
+ *   d_n_acc  [B] nodes accepted, the root not counted
+ *   d_tokens [B][T] accepted tokens, then the id sampled at the last, -1 padded
+ *   d_path   [B][T] the root and the accepted nodes, -1 padded
+ *   d_lens_out [B] lens + 1 + n_acc; -1: the rows did not fit */
+int tgs_tree_commit(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs, int T,
+                    const int32_t* d_parents, const int32_t* d_draft, const int32_t* d_sampled, int32_t* d_n_acc,
+                    int32_t* d_tokens, int32_t* d_path, int32_t* d_lens_out, tgs_stream stream);
+
+/* Reorders the rows of a cache after a beam step: row r goes on from row
+ * d_parents[r] (seqs: the rows as they are).  Full pages are shared.  Of the
+ * pages from there on, which hold the last tokens and have room for `room`
+ * new ones, each has one writer: it stays with the first row (in row, then
+ * slot order) that names it, unless a row shares it; the other rows get free
+ * pages, in ascending order, and copies of the tokens in every layer (whole
+ * blocks of eight).  Free are the pages of the pool that no row names any
+ * more, so the pool must belong to these rows alone.
+ *   d_tables_out [B][width]: -1 past the slots in use; d_lens_out [B]
+ * A parent outside [0, B) gives an empty row (its pages become free); a row
+ * that finds no free page, or whose table has no slots for its room, gets the length -1.
+ * Outputs must not overlap inputs. */
+int tgs_kv_fork(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_seqs* seqs, const int32_t* d_parents, int room,
+                int32_t* d_tables_out, int32_t* d_lens_out, tgs_stream stream);
 
 #ifdef __cplusplus
 }

@@ -24,6 +24,7 @@ TGS_ETOOBIG = -5
 
 TGS_F32 = 0
 TGS_BF16 = 1
+TGS_F16 = 2  # key/value caches only
 TGS_FLAG_GREEDY = 1
 
 # Exported entry points of include/tgs_sampler.h.
@@ -43,6 +44,11 @@ EXPORTS = (
     "tgs_spec_verify",
     "tgs_token_logprobs",
     "tgs_mask_rows_from_dfa",
+    "tgs_beam_select",
+    "tgs_tree_attention",
+    "tgs_kv_append",
+    "tgs_tree_commit",
+    "tgs_kv_fork",
 )
 
 ROW_PARAMS_DTYPE = np.dtype(
@@ -132,6 +138,17 @@ def load() -> C.CDLL:
     L.tgs_token_logprobs.argtypes = [P, P, I, I, I, C.c_int64, P, P, P, P]
     L.tgs_mask_rows_from_dfa.restype = I
     L.tgs_mask_rows_from_dfa.argtypes = [P, P, P, I, P, I, P, P, C.c_int64, I, I, P, P, I, P]
+    # argument blocks (tgs_kv_cache, tgs_kv_rows, tgs_kv_seqs, tgs_attn) come as packed bytes
+    L.tgs_beam_select.restype = I
+    L.tgs_beam_select.argtypes = [P, P, I, I, I, I, C.c_int64, P, I, P, P, I, P, P, P, P, P, P]
+    L.tgs_tree_attention.restype = I
+    L.tgs_tree_attention.argtypes = [P, P, P, P, P, P]
+    L.tgs_kv_append.restype = I
+    L.tgs_kv_append.argtypes = [P, P, P, P, I, P, P, P]
+    L.tgs_tree_commit.restype = I
+    L.tgs_tree_commit.argtypes = [P, P, P, P, I, P, P, P, P, P, P, P, P]
+    L.tgs_kv_fork.restype = I
+    L.tgs_kv_fork.argtypes = [P, P, P, P, I, P, P, P]
     _lib = L
     return L
 

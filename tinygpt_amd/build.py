@@ -20,7 +20,7 @@ OUT = os.path.join(HERE, "libtgs_sampler.so")
 FLOOR_SRC = "tgs_floor.hip"
 FLOOR_OUT = os.path.join(HERE, "libtgs_floor.so")
 SOURCES = ["tgs_kernels.hip", "tgs_k64.hip", "tgs_spec.hip", "tgs_topp.hip", "tgs_topp_split.hip", "tgs_topk.hip", "tgs_logprob.hip",
-           "tgs_mask.hip", "tgs_api.hip"]
+           "tgs_mask.hip", "tgs_kv.hip", "tgs_beam.hip", "tgs_attn_narrow.hip", "tgs_attn_wide.hip", "tgs_kv_api.hip", "tgs_api.hip"]
 ARCH = os.environ.get("TGS_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

@@ -19,61 +19,19 @@
 #include <unordered_map>
 #include <vector>
 
+#include "tgs_ctx.h"
 #include "tgs_device.h"
 #include "tgs_kernels.h"
 
-struct tgs_ctx {
-  int device = 0;
-  int max_batch = 0, max_vocab = 0, max_hist = 0;
-  int num_cu = 256;
-  size_t lds_limit = 65536;
-  unsigned long long* ws = nullptr;
-  int* ws_cnt = nullptr;
-  int ws_rows = 0;  // chunk lists of KMAX entries the workspace holds
-  size_t ws_words = 0;  // its 8-byte words
-  // one allocation, zeroed once, from k64_lists on
-  unsigned long long* k64_lists = nullptr;  // fused kernel chunk lists, [max_batch * kMaxSplit][64]
-  unsigned long long* k64_keys = nullptr;   // fused kernel bound-exchange keys, [max_batch][K64_KEYS]
-  unsigned long long* tp_lines = nullptr;   // split-kernel exchange lines, [max_batch][TOPPS_LINE]
-  unsigned* k64_cnt = nullptr;  // fused kernel exchange lines (arrival counter, epoch, count words), one per row
-  uint32_t* mask_table = nullptr;
-  int n_states = 0, mask_vocab = 0, mask_words = 0;
-  void* mask_stage = nullptr;  // tgs_mask_table_update staging (grown on demand)
-  size_t mask_stage_bytes = 0;
-  float* spec_blk_m = nullptr;             // speculative workspace (tgs_reserve_spec)
-  unsigned long long* spec_blk_q = nullptr;
-  unsigned long long* spec_blk_w = nullptr;
-  void* spec_state = nullptr;
-  int spec_b = 0, spec_k = -1, spec_nbs = 0;
-  std::string err;
-};
-
 namespace {
+
+using tgs::DeviceGuard;
+using tgs::fail;
+using tgs::hip_fail;
 
 constexpr int kMaxVocab = 262144;  // 256 speculative blocks of 1024 ids
 constexpr int kMaxHist = 4096;
 constexpr int kMaxSplit = 16;
-
-struct DeviceGuard {
-  int prev = -1;
-  bool ok = false;
-  explicit DeviceGuard(int dev) {
-    if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-    ok = hipSetDevice(dev) == hipSuccess;
-  }
-  ~DeviceGuard() {
-    if (prev >= 0) (void)hipSetDevice(prev);
-  }
-};
-
-int fail(tgs_ctx* h, int code, const std::string& msg) {
-  if (h) h->err = msg;
-  return code;
-}
-
-int hip_fail(tgs_ctx* h, hipError_t e, const char* what) {
-  return fail(h, TGS_EHIP, std::string(what) + ": " + hipGetErrorString(e));
-}
 
 int next_pow2(int x) {
   int p = 1;

@@ -1,0 +1,349 @@
+// tgs_attn_narrow.hip -- tree attention where a key head has at most 32 query
+// rows: the cache is read once and the reading bounds it.
+//
+// Each wave owns whole tiles of 32 tokens and loads their keys and values from
+// the cache straight into the matrix units' operand registers; nothing is
+// shared while tiles are read, so no wave waits for another.  The next tile's
+// keys are requested as soon as this tile's are used, and so the values: with
+// eight waves a CU has about 100 KB on the way.  The waves' states join
+// through LDS at the end of a (sequence, key head).
+#include "tgs_attn.h"
+
+namespace tgs {
+namespace attn {
+
+
+
+template <int D, int QT>
+constexpr int narrow_waves() { return D * QT >= 512 || D == 256 ? 4 : 8; }
+
+template <typename DT, int D, int QT, int NW>
+struct Narrow {
+  static constexpr int KK = D / 32, DT16 = D / 16;
+  static constexpr int ROWS = 16 * QT;
+  struct Shared {
+    f32x4 o[NW][DT16 * QT][64];
+    float ml[NW][ROWS][2];
+    float tot[ROWS][2];
+  };
+
+  const AttnArgs& a;
+  const int lane, wave, col, grp;
+  // the tiles in progress
+  int b, h, len, nc;
+  const int* table;
+  bool bad;
+
+  __device__ __forceinline__ Narrow(const AttnArgs& a_)
+      : a(a_), lane(lane_id()), wave((int)threadIdx.x >> 6), col(lane & 15), grp(lane >> 4), b(0), h(0), len(0), nc(0),
+        table(nullptr), bad(false) {}
+
+  // Page entries of tile i for the lane's key block and value block.
+  __device__ __forceinline__ int2 entries(int i) const {
+    if (i >= nc) return make_int2(0, 0);
+    const int kb = i * NTILE + (col >> 2) * 8, vb = i * NTILE + grp * 8;
+    const int last = len - 1;
+    return make_int2(table[(kb < last ? kb : last) >> a.page_shift], table[(vb < last ? vb : last) >> a.page_shift]);
+  }
+  __device__ __forceinline__ long long page_of(int e) {
+    if ((unsigned)e >= (unsigned)a.n_pages) {
+      bad = true;  // (its sequence's rows become NaN)
+      return 0;
+    }
+    return e;
+  }
+
+  // Keys of tile i: product row r = 4 g + j of half t is token 8 g + 4 t + j.
+  __device__ __forceinline__ void load_keys(int i, int entry, uint4 (&k)[2][KK]) {
+    const int tok = (col >> 2) * 8 + (col & 3);
+    if (i < nc) {
+      const uint16_t* base = (const uint16_t*)a.k + page_of(entry) * a.k_page + (((long long)h * D) << a.page_shift) + grp * 8;
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        int p = i * NTILE + tok + 4 * t;
+        p = (p < len ? p : len - 1) & ((1 << a.page_shift) - 1);
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) k[t][kk] = *(const uint4*)(base + p * D + kk * 32);
+      }
+    } else {
+      const uint16_t* base = (const uint16_t*)a.k_new + b * a.kn_b + h * a.kn_h + grp * 8;
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        int p = (i - nc) * NTILE + tok + 4 * t;
+        p = p < a.T ? p : a.T - 1;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) k[t][kk] = load_row16<false>(base + p * a.kn_t + kk * 32);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load_values(int i, int entry, uint4 (&v)[DT16]) {
+    if (i < nc) {
+      const int blk = i * NTILE + grp * 8, last = (len - 1) & ~7;
+      const int p = (blk < last ? blk : last) & ((1 << a.page_shift) - 1);
+      const uint16_t* base = (const uint16_t*)a.v + page_of(entry) * a.v_page + (((long long)h * D) << a.page_shift) +
+                             (long long)p * D + col * 8;
+#pragma unroll
+      for (int d = 0; d < DT16; d++) v[d] = *(const uint4*)(base + d * 128);
+    } else {
+      const uint16_t* base = (const uint16_t*)a.v_new + b * a.vn_b + h * a.vn_h + col;
+#pragma unroll
+      for (int d = 0; d < DT16; d++) {
+        v[d] = tree_values(base + d * 16, a.vn_t, (i - nc) * NTILE + grp * 8, a.T);
+        sched_fence();  // (all of them at once would take 8 D / 16 registers)
+      }
+    }
+  }
+
+  // Tiles [t0, t1) of (b, h); full: they are all of it.  part: the workspace's rows otherwise.
+  __device__ __forceinline__ void segment(Shared& s, int t0, int t1, bool full, long long part) {
+    len = seq_len(a, b);
+    nc = (len + NTILE - 1) / NTILE;
+    table = a.tables + (long long)b * a.P;
+    bad = false;
+    const u64 anc = t1 > nc ? ancestors(a, b) : 0ull;  // of node `lane`
+    uint4 q[QT][KK];
+    u64 sees[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      const int i = t * 16 + col;
+      const int node = i < a.M ? i / a.G : 0, hg = i < a.M ? i - node * a.G : 0;
+      const uint16_t* p = (const uint16_t*)a.q + b * a.q_b + node * a.q_t + (long long)(h * a.G + hg) * a.q_h + grp * 8;
+#pragma unroll
+      for (int kk = 0; kk < KK; kk++) q[t][kk] = load_row16<false>(p + kk * 32);
+      sees[t] = ((u64)(uint32_t)__shfl((int)(anc >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)anc, node, 64);
+    }
+    f32x4 o[QT][DT16];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      m[t] = NEG;
+      l[t] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT16; d++) o[t][d] = f32x4{0, 0, 0, 0};
+    }
+    uint4 k[2][KK], v[DT16];
+    int i = t0 + wave;
+    if (i < t1) {
+      int2 e = entries(i);
+      load_keys(i, e.x, k);
+      load_values(i, e.y, v);
+      e = i + NW < t1 ? entries(i + NW) : e;
+      for (; i < t1; i += NW) {
+        f32x4 sc[QT][2];
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            sc[t][x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) sc[t][x] = mfma16<DT>(k[x][kk], q[t][kk], sc[t][x]);
+          }
+        const bool more = i + NW < t1;
+        if (more) load_keys(i + NW, e.x, k);
+        const int first = i * NTILE + grp * 8;  // the lane's eight tokens
+        if (i >= nc) {
+#pragma unroll
+          for (int t = 0; t < QT; t++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              const int tok = (i - nc) * NTILE + grp * 8 + j;
+              if (!((sees[t] >> tok) & 1)) sc[t][j >> 2][j & 3] = NEG;
+            }
+        } else if ((i + 1) * NTILE > len) {
+#pragma unroll
+          for (int t = 0; t < QT; t++)
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+              if (first + j >= len) sc[t][j >> 2][j & 3] = NEG;
+          // what lies past the end is not 0 (it may be anything, NaN too)
+#pragma unroll
+          for (int d = 0; d < DT16; d++) v[d] = keep_first(v[d], len - first);
+        }
+        uint4 p[QT];
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          float top = sc[t][0][0];
+#pragma unroll
+          for (int j = 1; j < 8; j++) top = fmaxf(top, sc[t][j >> 2][j & 3]);
+          top *= a.scale_log2;
+          if (__ballot(top > m[t] + SLACK)) {
+            top = fmaxf(top, xor_lane<16>(top));
+            top = fmaxf(top, xor_lane<32>(top));
+            const float now = fmaxf(m[t], top);
+            const float f = m[t] == NEG ? 0.0f : exp2_hw(m[t] - now);
+            m[t] = now;
+            l[t] *= f;
+#pragma unroll
+            for (int d = 0; d < DT16; d++) o[t][d] *= f;
+          }
+          const float base = m[t] == NEG ? 0.0f : m[t];
+          float w[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            w[j] = exp2_hw(__builtin_fmaf(sc[t][j >> 2][j & 3], a.scale_log2, -base));
+            l[t] += w[j];
+          }
+          p[t] = make_uint4(pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7]));
+        }
+#pragma unroll
+        for (int d = 0; d < DT16; d++)
+#pragma unroll
+          for (int t = 0; t < QT; t++) o[t][d] = mfma16<DT>(v[d], p[t], o[t][d]);
+        if (more) {
+          load_values(i + NW, e.y, v);
+          if (i + 2 * NW < t1) e = entries(i + 2 * NW);
+        }
+      }
+    }
+    // the waves' states
+    const bool any_bad = __ballot(bad) != 0;
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      l[t] += xor_lane<16>(l[t]);
+      l[t] += xor_lane<32>(l[t]);
+      if (any_bad) l[t] = __builtin_nanf("");
+      if (grp == 0) {
+        s.ml[wave][t * 16 + col][0] = m[t];
+        s.ml[wave][t * 16 + col][1] = l[t];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      float top = NEG, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; w++) top = fmaxf(top, s.ml[w][t * 16 + col][0]);
+#pragma unroll
+      for (int w = 0; w < NW; w++) {
+        const float mw = s.ml[w][t * 16 + col][0];
+        sum += s.ml[w][t * 16 + col][1] * (mw == NEG ? 1.0f : exp2_hw(mw - top));
+      }
+      const float f = m[t] == NEG ? 0.0f : exp2_hw(m[t] - top);
+#pragma unroll
+      for (int d = 0; d < DT16; d++) s.o[wave][d * QT + t][lane] = o[t][d] * f;
+      if (wave == 0 && grp == 0) {
+        s.tot[t * 16 + col][0] = top;
+        s.tot[t * 16 + col][1] = sum;
+      }
+    }
+    __syncthreads();
+    for (int e = wave; e < DT16 * QT; e += NW) {
+      f32x4 x = s.o[0][e][lane];
+#pragma unroll
+      for (int w = 1; w < NW; w++) x += s.o[w][e][lane];
+      const int t = e % QT, d = e / QT * 16 + grp * 4, i = t * 16 + col;
+      if (i >= a.M) continue;
+      if (full) {
+        const int node = i / a.G;
+        const long long row = ((long long)b * a.T + node) * a.Hq + h * a.G + (i - node * a.G);
+        const float r = 1.0f / s.tot[i][1];
+        store4<DT>((uint16_t*)a.out + row * D + d, x * r);
+        if (a.lse && e < QT && grp == 0) a.lse[row] = row_lse(s.tot[i][0], s.tot[i][1]);
+      } else {
+        *(f32x4*)(a.part_o + (part + i) * D + d) = x;
+        if (e < QT && grp == 0) {
+          a.part_ml[(part + i) * 2] = s.tot[i][0];
+          a.part_ml[(part + i) * 2 + 1] = s.tot[i][1];
+        }
+      }
+    }
+    __syncthreads();
+  }
+};
+
+template <typename DT, int D, int QT, int NW>
+__global__ __launch_bounds__(NW * 64, NW / 4) void narrow_kernel(AttnArgs a) {
+  typedef Narrow<DT, D, QT, NW> K;
+  TGS_DYN_SMEM(dyn);
+  typename K::Shared& s = *(typename K::Shared*)dyn;
+  K n(a);
+  const int tree = (a.T + NTILE - 1) / NTILE;
+  if (a.nwg == 0) {
+    n.b = blockIdx.x / a.Hkv;
+    n.h = blockIdx.x % a.Hkv;
+    n.segment(s, 0, cache_tiles<NTILE>(a, n.b) + tree, true, 0);
+    return;
+  }
+  int before, all, b;
+  tiles_before<NTILE>(a, 0, before, all);
+  const long long U = (long long)all * a.Hkv;
+  const long long u0 = share_start(U, a.nwg, blockIdx.x), u1 = share_start(U, a.nwg, blockIdx.x + 1);
+  if (u0 == u1) return;
+  long long skip;
+  find_tile<NTILE>(a, u0, a.Hkv, b, skip);
+  int nt = cache_tiles<NTILE>(a, b) + tree;
+  int h = (int)((u0 - skip) / nt), at = (int)((u0 - skip) - (long long)h * nt);
+  for (long long u = u0; u < u1;) {
+    const int end = nt - at < u1 - u ? nt : at + (int)(u1 - u);
+    n.b = b;
+    n.h = h;
+    n.segment(s, at, end, at == 0 && end == nt, ((long long)blockIdx.x * 2 + (u != u0)) * a.QB);
+    u += end - at;
+    at = 0;
+    if (++h == a.Hkv) {
+      h = 0;
+      if (++b < a.B) nt = cache_tiles<NTILE>(a, b) + tree;
+    }
+  }
+}
+
+template <typename DT, int D, int QT>
+hipError_t narrow_run(const AttnArgs& a, hipStream_t st) {
+  constexpr int NW = narrow_waves<D, QT>();
+  typedef Narrow<DT, D, QT, NW> K;
+  const int grid = a.nwg ? a.nwg : a.B * a.Hkv;
+  hipLaunchKernelGGL((narrow_kernel<DT, D, QT, NW>), dim3(grid), dim3(NW * 64), sizeof(typename K::Shared), st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.nwg == 0) return e;
+  const long long rows = (long long)a.B * a.Hkv * a.M;
+  hipLaunchKernelGGL((join_kernel<DT, NTILE>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+template <typename DT, int D, int QT>
+hipError_t narrow_lds() {
+  constexpr int NW = narrow_waves<D, QT>();
+  return hipFuncSetAttribute((const void*)narrow_kernel<DT, D, QT, NW>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)sizeof(typename Narrow<DT, D, QT, NW>::Shared));
+}
+
+template <typename DT>
+hipError_t narrow_type(const AttnArgs& a, int qt, hipStream_t st) {
+  switch (a.D * 2 + qt - 1) {
+    case 128: return narrow_run<DT, 64, 1>(a, st);
+    case 129: return narrow_run<DT, 64, 2>(a, st);
+    case 192: return narrow_run<DT, 96, 1>(a, st);
+    case 193: return narrow_run<DT, 96, 2>(a, st);
+    case 256: return narrow_run<DT, 128, 1>(a, st);
+    case 257: return narrow_run<DT, 128, 2>(a, st);
+    case 512: return narrow_run<DT, 256, 1>(a, st);
+    case 513: return narrow_run<DT, 256, 2>(a, st);
+  }
+  return hipErrorInvalidValue;
+}
+template <typename DT>
+hipError_t narrow_lds_type() {
+  hipError_t e = hipSuccess;
+  auto take = [&](hipError_t x) { e = x != hipSuccess ? x : e; };
+  take(narrow_lds<DT, 64, 1>());
+  take(narrow_lds<DT, 64, 2>());
+  take(narrow_lds<DT, 96, 1>());
+  take(narrow_lds<DT, 96, 2>());
+  take(narrow_lds<DT, 128, 1>());
+  take(narrow_lds<DT, 128, 2>());
+  take(narrow_lds<DT, 256, 1>());
+  take(narrow_lds<DT, 256, 2>());
+  return e;
+}
+
+}  // namespace attn
+
+hipError_t launch_attn_narrow(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st) {
+  return dtype == TGS_BF16 ? attn::narrow_type<attn::BF16>(a, p.qw, st) : attn::narrow_type<attn::F16>(a, p.qw, st);
+}
+hipError_t set_attn_narrow_lds(size_t) {
+  const hipError_t e = attn::narrow_lds_type<attn::BF16>(), f = attn::narrow_lds_type<attn::F16>();
+  return e != hipSuccess ? e : f;
+}
+
+}  // namespace tgs

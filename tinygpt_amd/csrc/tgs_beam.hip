@@ -1,0 +1,254 @@
+// tgs_beam.hip -- beam search's selection: of a request's W beams over V ids
+// each, the n largest of score[w] + x[w][v] - logsumexp(x[w]), and the
+// histories that go with them.
+//
+// One read of the logits bounds it.  chunk_kernel holds a chunk of a row in
+// registers: thread maxima give a bound that at most a few more than n ids
+// pass (the n-th largest of the maxima), these are collected and sorted, and
+// the chunk's maximum and sum of exponentials come from the same registers.
+// Inside a row the order is the logits' own, so it needs no arithmetic; join_kernel
+// then orders the candidates of different beams by totals held in 64 bits,
+// since those of different beams may lie closer than 32 bits tell apart.
+#include "tgs_device.h"
+#include "tgs_kv.h"
+#include "tgs_row.h"
+
+namespace tgs {
+namespace beam {
+
+// 2^x by the hardware instruction; results below 2^-126 are 0, next to a sum
+// of at least 1.
+__device__ __forceinline__ float exp2_hw(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_exp2f(x);
+#else
+  return exp2f(x);
+#endif
+}
+
+struct ChunkShared {
+  BlockScratch bs;
+  uint32_t top[BEAM_NT / 64][64];
+  u64 cand[BEAM_CAP];
+  double sum[BEAM_NT / 64];
+  unsigned n;
+};
+
+// Workgroup (row, chunk): ids [c L, min(V, (c + 1) L)), NVT vectors a thread.
+template <typename Tin, int NVT>
+__global__ __launch_bounds__(BEAM_NT) void chunk_kernel(BeamArgs a) {
+  constexpr int EPV = Elem<Tin>::EPV;
+  TGS_STATIC_SMEM(ChunkShared, s);
+  const int row = blockIdx.x / a.S, c = blockIdx.x % a.S, tid = threadIdx.x, w = tid >> 6;
+  const Tin* rowp = (const Tin*)a.logits + (long long)row * a.row_stride;
+  const int v0 = c * a.L, v1 = v0 + a.L < a.V ? v0 + a.L : a.V;
+  const int nvec = (v1 - v0) / EPV, tail0 = v0 + nvec * EPV;
+  constexpr uint32_t NB = Elem<Tin>::NAN_BITS;
+  uint4 raw[NVT];
+#pragma unroll
+  for (int j = 0; j < NVT; j++) {
+    const int i = j * BEAM_NT + tid;
+    raw[j] = make_uint4(NB, NB, NB, NB);
+    if (i < nvec) raw[j] = load_row16<true>(rowp + v0 + i * EPV);
+  }
+  // the last ids of a row that is not whole vectors, one a thread
+  const float xt = tid < v1 - tail0 ? Elem<Tin>::scalar(rowp, tail0 + tid) : -__builtin_inff();
+  if (tid == 0) s.n = 0;
+  float tm = fmaxf(xt, -__builtin_inff());  // (of a NaN and a number the number)
+#pragma unroll
+  for (int j = 0; j < NVT; j++)
+#pragma unroll
+    for (int e = 0; e < EPV; e++) tm = fmaxf(tm, Elem<Tin>::get(raw[j], e));
+  uint32_t top = wave_sort_desc(tg_key(tm));
+  s.top[w][lane_id()] = top;
+  __syncthreads();
+  top = s.top[0][lane_id()];
+#pragma unroll
+  for (int i = 1; i < BEAM_NT / 64; i++) top = wave_merge_top64(top, s.top[i][lane_id()]);
+  const float m = tg_unkey(readlane_u32(top, 0)), bound = tg_unkey(readlane_u32(top, a.n - 1));
+  // candidates and the sum; exp(x - m) as 2^(d log2 e) with the constant in two parts
+  constexpr float L2H = 0x1.715476p+0f, L2L = 0x1.4ae0cp-26f;
+  double sum = 0.0;
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < NVT; j++)
+#pragma unroll
+      for (int e = 0; e < EPV; e++)
+        f(Elem<Tin>::get(raw[j], e), v0 + (j * BEAM_NT + tid) * EPV + e);
+    f(xt, tail0 + tid);
+  };
+  each([&](float x, int v) {
+    if (x >= bound && x > -__builtin_inff()) {
+      const unsigned at = atomicAdd(&s.n, 1u);
+      if (at < (unsigned)BEAM_CAP) s.cand[at] = comp_key(tg_key(x), v);
+    }
+  });
+  auto term = [&](float x) {
+    const float d = x - m;
+    const float e = exp2_hw(__builtin_fmaf(d, L2H, d * L2L));
+    return x > -__builtin_inff() ? e : 0.0f;
+  };
+#pragma unroll
+  for (int j = 0; j < NVT; j++) {
+    float part = 0.0f;  // (of one vector's terms)
+#pragma unroll
+    for (int e = 0; e < EPV; e++) part += term(Elem<Tin>::get(raw[j], e));
+    sum += (double)part;
+  }
+  sum += (double)term(xt);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane_id() == 0) s.sum[w] = sum;
+  __syncthreads();
+  unsigned n = s.n;
+  if (n > (unsigned)BEAM_CAP) {  // many equal logits: the exact n-th by its composite
+    const u64 least = block_select_kth<u64, 64, BEAM_NT>(
+        [&](auto f) {
+          each([&](float x, int v) {
+            if (x > -__builtin_inff()) f(comp_key(tg_key(x), v));
+          });
+        },
+        (unsigned)a.n, s.bs);
+    __syncthreads();
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    each([&](float x, int v) {
+      if (x > -__builtin_inff() && comp_key(tg_key(x), v) >= least) {
+        const unsigned at = atomicAdd(&s.n, 1u);
+        if (at < (unsigned)BEAM_CAP) s.cand[at] = comp_key(tg_key(x), v);
+      }
+    });
+    __syncthreads();
+    n = s.n;
+  }
+  if (w == 0) {
+    const int lane = lane_id();
+    u64 best = wave_sort_desc((unsigned)lane < n ? s.cand[lane] : 0ull);
+    for (unsigned i = 64; i < n; i += 64)
+      best = wave_merge_top64(best, wave_sort_desc(i + lane < n ? s.cand[i + lane] : 0ull));
+    if (lane < a.n) a.lists[(long long)blockIdx.x * a.n + lane] = best;
+    if (lane == 0) {
+      double t = 0.0;
+#pragma unroll
+      for (int i = 0; i < BEAM_NT / 64; i++) t += s.sum[i];
+      a.sums[2 * (long long)blockIdx.x] = (double)m;
+      a.sums[2 * (long long)blockIdx.x + 1] = t;
+    }
+  }
+}
+
+struct JoinShared {
+  double total[BEAM_MAX][BEAM_MAX];  // -inf past a beam's candidates
+  int id[BEAM_MAX][BEAM_MAX];
+  double best[BEAM_MAX];
+  int parent[BEAM_MAX], token[BEAM_MAX];
+};
+
+// Workgroup per request.  A wave per beam joins its chunks; a candidate's
+// place among all is its place in its own sorted list plus, by bisection, the
+// number of candidates ahead of it in every other.
+__global__ __launch_bounds__(BEAM_NT) void join_kernel(BeamArgs a) {
+  TGS_STATIC_SMEM(JoinShared, s);
+  const int g = blockIdx.x, tid = threadIdx.x, lane = lane_id();
+  const int W = a.W, n = a.n;
+  const double NINF = -__builtin_inf();
+  for (int w = tid >> 6; w < W; w += BEAM_NT / 64) {
+    const long long row = (long long)g * W + w;
+    const u64* lists = a.lists + row * a.S * n;
+    const double* sums = a.sums + row * a.S * 2;
+    double m = lane < a.S ? sums[2 * lane] : NINF, t = lane < a.S ? sums[2 * lane + 1] : 0.0;
+    u64 best = lane < n ? lists[lane] : 0ull;
+    for (int i = 1; i < a.S; i++) best = wave_merge_top64(best, lane < n ? lists[i * n + lane] : 0ull);
+    double top = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const double y = __shfl_xor(top, o, 64);
+      top = y > top ? y : top;
+    }
+    t = m == top ? t : t * exp(m - top);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
+    const double lse = top + log(t);
+    const float score = a.scores[row];
+    // a beam that has ended (its score not a number above -inf), or whose row
+    // holds +inf or nothing, has no candidates
+    const bool live = __builtin_isfinite(score) && __builtin_isfinite(lse);
+    if (lane < n) {
+      const bool has = live && best != 0ull;
+      s.total[w][lane] = has ? (double)score + ((double)comp_y(best) - lse) : NINF;
+      s.id[w][lane] = has ? comp_id(best) : -1;
+    }
+  }
+  for (int i = tid; i < n; i += BEAM_NT) {
+    s.best[i] = NINF;
+    s.parent[i] = -1;
+    s.token[i] = -1;
+  }
+  __syncthreads();
+  for (int i = tid; i < W * n; i += BEAM_NT) {
+    const int w = i / n, j = i - w * n;
+    const double x = s.total[w][j];
+    if (x == NINF) continue;
+    int rank = j;
+    for (int o = 0; o < W && rank < n; o++) {
+      if (o == w) continue;
+      int lo = 0, hi = n;  // entries of o ahead of x; of equal ones the lower beam's
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        const double y = s.total[o][mid];
+        if (y > x || (y == x && o < w))
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      rank += lo;
+    }
+    if (rank < n) {
+      s.best[rank] = x;
+      s.parent[rank] = g * W + w;
+      s.token[rank] = s.id[w][j];
+    }
+  }
+  __syncthreads();
+  const long long out = (long long)g * n;
+  for (int i = tid; i < n; i += BEAM_NT) {
+    a.out_scores[out + i] = (float)s.best[i];
+    a.out_parents[out + i] = s.parent[i];
+    a.out_tokens[out + i] = s.token[i];
+  }
+  if (a.H == 0) return;
+  for (int r = tid >> 6; r < n; r += BEAM_NT / 64) {
+    const int p = s.parent[r], H = a.H;
+    int have = p < 0 ? 0 : a.hist_len[p];
+    have = have < 0 ? 0 : have > H ? H : have;
+    const int drop = have == H, kept = p < 0 ? -1 : have - drop;
+    const int* from = a.hist + (long long)(p < 0 ? 0 : p) * H + drop;
+    int* to = a.out_hist + (out + r) * H;
+    for (int j = lane; j < H; j += 64) to[j] = j < kept ? from[j] : j == kept ? s.token[r] : -1;
+    if (lane == 0) a.out_hist_len[out + r] = kept + 1;
+  }
+}
+
+template <typename Tin>
+hipError_t launch_t(const BeamArgs& a, hipStream_t st) {
+  const int per = BEAM_NT * Elem<Tin>::EPV;
+  const dim3 grid(a.G * a.W * a.S);
+  if (a.L <= 4 * per)
+    hipLaunchKernelGGL((chunk_kernel<Tin, 4>), grid, dim3(BEAM_NT), 0, st, a);
+  else
+    hipLaunchKernelGGL((chunk_kernel<Tin, BEAM_NVT>), grid, dim3(BEAM_NT), 0, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(join_kernel, dim3(a.G), dim3(BEAM_NT), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace beam
+
+int beam_chunk_ids(int dtype) { return BEAM_NT * BEAM_NVT * (dtype == TGS_BF16 ? 8 : 4); }
+
+hipError_t launch_beam(const BeamArgs& a, int dtype, hipStream_t st) {
+  return dtype == TGS_BF16 ? beam::launch_t<uint16_t>(a, st) : beam::launch_t<float>(a, st);
+}
+
+}  // namespace tgs

@@ -13,6 +13,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import ROW_PARAMS_DTYPE, TGS_BF16, TGS_F32, TgsDebug, TgsError, TgsHint
+from .cache import CacheOps
 
 
 _torch_module = None
@@ -228,7 +229,7 @@ def sample_noalloc(logits, params_dev, u, hist=None, hist_len=None, out=None, vo
     return out
 
 
-class Sampler:
+class Sampler(CacheOps):
     """One sampler handle on one GPU.
 
     max_batch / max_vocab / max_hist bound every call; the workspace is
