@@ -45,8 +45,8 @@ inline uint32_t hipcpu_pack2(float lo, float hi) {
 struct hipcpu_ops {
   uint16_t a[64][8], b[64][8];
 };
-template <int N, bool BF16, typename V>
-inline V hipcpu_mfma(const uint4& a, const uint4& b, V c) {
+template <int N, bool BF16, typename A, typename V>
+inline V hipcpu_mfma(const A& a, const A& b, V c) {
   static hipcpu_ops ops[16];
   hipcpu_ops& o = ops[hipcpu::t_thread.x / 64];
   const int l = hipcpu::lane();

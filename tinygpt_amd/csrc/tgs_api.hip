@@ -537,7 +537,7 @@ int tgs_create(tgs_handle* out, int device, int max_batch, int max_vocab, int ma
     pairs = std::max((size_t)std::min(h->num_cu, max_batch * tgs::TOPPS_MAX_SPLIT), (size_t)max_batch * smin);
     pairs = std::min(pairs, (size_t)kSplitSlabs);
   }
-  h->ws_words = std::max((size_t)h->ws_rows * tgs::KMAX, pairs * tgs::TOPPS_PAIR);
+  h->ws_words = std::max({(size_t)h->ws_rows * tgs::KMAX, pairs * tgs::TOPPS_PAIR, tgs::attn_ws_words(h->num_cu)});
   hipError_t e = hipMalloc(&h->ws, sizeof(unsigned long long) * h->ws_words);
   if (e == hipSuccess) e = hipMalloc(&h->ws_cnt, sizeof(int) * (size_t)h->ws_rows * (tgs::KMAX / 64));
   // everything that starts zeroed in one allocation: chunk lists ("not

@@ -31,6 +31,13 @@ namespace attn {
 
 typedef float f32x4 __attribute__((vector_size(16)));
 typedef float f32x16 __attribute__((vector_size(64)));
+typedef uint32_t Vec __attribute__((vector_size(16)));  // eight 16-bit values
+__device__ __forceinline__ Vec vec16(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return Vec{a, b, c, d}; }
+// At any alignment of the values.
+__device__ __forceinline__ Vec load16(const uint16_t* p) {
+  typedef Vec Vec2 __attribute__((aligned(2)));
+  return *(const Vec2*)p;
+}
 
 struct BF16 {};
 struct F16 {};
@@ -46,7 +53,7 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 // c + a b, 16 x 16 with 32 products each: lane l holds a's row (b's column)
 // l % 16, k = 8 (l / 16) .. + 7, and c's rows 4 (l / 16) .. + 3 of column l % 16.
 template <typename DT>
-__device__ __forceinline__ f32x4 mfma16(const uint4& a, const uint4& b, f32x4 c) {
+__device__ __forceinline__ f32x4 mfma16(Vec a, Vec b, f32x4 c) {
 #if defined(__HIP_DEVICE_COMPILE__)
   if constexpr (__is_same(DT, BF16))
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -63,7 +70,7 @@ __device__ __forceinline__ f32x4 mfma16(const uint4& a, const uint4& b, f32x4 c)
 // The same for 32 x 32 with 16 products: row or column l % 32, k = 8 (l / 32)
 // .. + 7; c's element i is row 8 (i / 4) + 4 (l / 32) + i % 4.
 template <typename DT>
-__device__ __forceinline__ f32x16 mfma32(const uint4& a, const uint4& b, f32x16 c) {
+__device__ __forceinline__ f32x16 mfma32(Vec a, Vec b, f32x16 c) {
 #if defined(__HIP_DEVICE_COMPILE__)
   if constexpr (__is_same(DT, BF16))
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -111,6 +118,18 @@ __device__ __forceinline__ void sched_fence() {
 #endif
 }
 
+// A workgroup barrier for LDS alone: requests to memory stay on their way
+// (__syncthreads may wait for them).
+__device__ __forceinline__ void lds_barrier() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+#elif defined(TGS_HOST_MFMA)
+  __syncthreads();
+#endif
+}
+
 constexpr int NTILE = 32, WTILE = 64;  // tokens of a tile of the narrow and of the wide kernel
 constexpr float NEG = -__builtin_inff();
 
@@ -122,21 +141,22 @@ constexpr float SLACK = 6.0f;
 
 // ------------------------------------------------------------------ shares
 
-struct Share {
-  long long U;   // tiles of all sequences and key heads
-  int b, h;      // the position of the next tile: sequence, key head,
-  int nc, nt;    // its tiles of the cache and in all,
-  int at;        // and the tile in it
-};
+// A value that every lane of the wave holds, for the scalar unit: what loops,
+// branches and addresses derive from it takes no vector registers.
+__device__ __forceinline__ int uniform(int x) { return (int)__builtin_amdgcn_readfirstlane((unsigned)x); }
 
-__device__ __forceinline__ int seq_len(const AttnArgs& a, int b) {
-  const int n = a.lens[b];
+__device__ __forceinline__ int clamp_len(const AttnArgs& a, int n) {
   const long long cap = (long long)a.P << a.page_shift;
   return n < 0 ? 0 : n > cap ? (int)cap : n;
 }
+__device__ __forceinline__ int seq_len(const AttnArgs& a, int b) { return uniform(clamp_len(a, a.lens[b])); }
 template <int TILE>
 __device__ __forceinline__ int cache_tiles(const AttnArgs& a, int b) {
   return (seq_len(a, b) + TILE - 1) / TILE;
+}
+template <int TILE>  // (a sequence per lane)
+__device__ __forceinline__ int lane_tiles(const AttnArgs& a, int b) {
+  return (clamp_len(a, a.lens[b]) + TILE - 1) / TILE;
 }
 
 // Tiles of sequences before b (of one key head), and of all: by one wave.
@@ -145,12 +165,12 @@ __device__ __forceinline__ void tiles_before(const AttnArgs& a, int b, int& befo
   const int tree = (a.T + TILE - 1) / TILE;
   int x = 0, y = 0;
   for (int i = lane_id(); i < a.B; i += 64) {
-    const int n = cache_tiles<TILE>(a, i) + tree;
+    const int n = lane_tiles<TILE>(a, i) + tree;
     y += n;
     if (i < b) x += n;
   }
-  before = wave_sum(x);
-  all = wave_sum(y);
+  before = uniform(wave_sum(x));
+  all = uniform(wave_sum(y));
 }
 
 // The sequence that holds tile t of one key head's tiles in order, and the tiles before it: by one wave.
@@ -159,7 +179,7 @@ __device__ __forceinline__ void find_tile(const AttnArgs& a, long long t, int he
   const int tree = (a.T + TILE - 1) / TILE, lane = lane_id();
   before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int n = b0 + lane < a.B ? cache_tiles<TILE>(a, b0 + lane) + tree : 0;
+    const int n = b0 + lane < a.B ? lane_tiles<TILE>(a, b0 + lane) + tree : 0;
     const int incl = wave_incl_scan(n);
     const u64 ends = __ballot(b0 + lane < a.B && before + (long long)incl * heads > t);
     if (ends) {
@@ -200,17 +220,33 @@ __device__ __forceinline__ u64 ancestors(const AttnArgs& a, int b) {
 }
 
 // Of the eight 16-bit values of x those with index < n stay (n <= 0: none), the others become 0.
-__device__ __forceinline__ uint4 keep_first(uint4 x, int n) {
+__device__ __forceinline__ Vec keep_first(Vec x, int n) {
   auto word = [&](uint32_t w, int i) { return n >= i + 2 ? w : n == i + 1 ? w & 0xFFFFu : 0u; };
-  return make_uint4(word(x.x, 0), word(x.y, 2), word(x.z, 4), word(x.w, 6));
+  return vec16(word(x[0], 0), word(x[1], 2), word(x[2], 4), word(x[3], 6));
+}
+
+// 8 x 8 16-bit values, rows x[j], turned: x[i] becomes the i-th of every row.
+__device__ __forceinline__ void transpose8(Vec (&x)[8]) {
+  uint32_t w[8][4];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    for (int i = 0; i < 4; i++) w[j][i] = x[j][i];
+  }
+  auto lo = [&](int i, int j) { return (w[j][i] & 0xFFFFu) | (w[j + 1][i] << 16); };
+  auto hi = [&](int i, int j) { return (w[j][i] >> 16) | (w[j + 1][i] & 0xFFFF0000u); };
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    x[2 * i] = vec16(lo(i, 0), lo(i, 2), lo(i, 4), lo(i, 6));
+    x[2 * i + 1] = vec16(hi(i, 0), hi(i, 2), hi(i, 4), hi(i, 6));
+  }
 }
 
 // Eight tokens' values of one d, tok .. tok + 7 of the drafted nodes; past the last 0.
-__device__ __forceinline__ uint4 tree_values(const uint16_t* v, long long stride, int tok, int T) {
+__device__ __forceinline__ Vec tree_values(const uint16_t* v, long long stride, int tok, int T) {
   uint32_t x[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) x[j] = tok + j < T ? v[(tok + j) * stride] : 0u;
-  return make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+  return vec16(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
 }
 
 // ------------------------------------------------------------------ results
@@ -228,6 +264,16 @@ __device__ __forceinline__ float row_lse(float m, float l) {
   return (float)(((double)m + (double)log2f(l)) * 0.69314718055994530942);
 }
 
+// Sum over the wave, the same in every lane.
+__device__ __forceinline__ float wave_sumf(float x) {
+  x += xor_lane<32>(x);
+  x += xor_lane<16>(x);
+  x += xor_lane<8>(x);
+  x += xor_lane<4>(x);
+  x += xor_lane<2>(x);
+  return x + xor_lane<1>(x);
+}
+
 // Joins the parts of (sequence, key head)s that several workers hold: a wave
 // per output row, in the workers' order.
 template <typename DT, int TILE>
@@ -243,29 +289,46 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
   const int N = a.nwg;
   const int w0 = (int)(((s0 + 1) * N - 1) / U), w1 = (int)((s1 * N - 1) / U);
   if (w0 == w1) return;
+  // A lane per part (64 at a time): its place, maximum and sum.  A worker's
+  // second part is the one that starts past its share's first tile.
   const int qb = i / a.QB, r = i - qb * a.QB;
-  auto part = [&](int w) {  // a worker's second part is the one that starts past its share's first tile
-    const int slot = share_start(U, N, w) < s0 ? 1 : 0;
-    return ((long long)(qb * N + w) * 2 + slot) * a.QB + r;
+  auto part_of = [&](int w) -> int {
+    if (w > w1) return -1;
+    const long long from = share_start(U, N, w);
+    if (from == share_start(U, N, w + 1)) return -1;
+    return ((qb * N + w) * 2 + (from < s0)) * a.QB + r;
   };
-  auto empty = [&](int w) { return share_start(U, N, w) == share_start(U, N, w + 1); };
   float m = NEG;
-  for (int w = w0 + lane; w <= w1; w += 64)
-    if (!empty(w)) m = fmaxf(m, a.part_ml[part(w) * 2]);
+  for (int w = w0; w <= w1; w += 64) {
+    const int p = part_of(w + lane);
+    m = fmaxf(m, p < 0 ? NEG : a.part_ml[2ll * p]);
+  }
   m = wave_maxf(m);
   float l = 0.0f;
-  float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int w = w0; w <= w1; w++) {
-    if (empty(w)) continue;
-    const long long p = part(w);
-    const float f = exp2_hw(a.part_ml[p * 2] - m);
-    l += f * a.part_ml[p * 2 + 1];
+  float o[4] = {0, 0, 0, 0};
+  for (int w = w0; w <= w1; w += 64) {
+    int p = part_of(w + lane);
+    const float f = p < 0 ? 0.0f : exp2_hw(a.part_ml[2ll * p] - m);
+    l += p < 0 ? 0.0f : f * a.part_ml[2ll * p + 1];
+    p = p < 0 ? 0 : p;  // (its factor is 0)
+    const int n = w1 - w + 1 < 64 ? w1 - w + 1 : 64;
+    for (int j = 0; j < n; j += 4) {
+      float x[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int d = j * 64 + lane;
-      if (d < a.D) o[j] += f * a.part_o[p * a.D + d];
+      for (int y = 0; y < 4; y++) {  // (past the last part: part 0's values, not used)
+        const long long at = (long long)(int)readlane_u32((uint32_t)p, j + y < n ? j + y : j) * a.D;
+#pragma unroll
+        for (int z = 0; z < 4; z++) x[y][z] = z * 64 + lane < a.D ? a.part_o[at + z * 64 + lane] : 0.0f;
+      }
+#pragma unroll
+      for (int y = 0; y < 4; y++) {
+        const float g = j + y < n ? readlane_f32(f, j + y < n ? j + y : j) : 0.0f;
+#pragma unroll
+        for (int z = 0; z < 4; z++) o[z] += g == 0.0f ? 0.0f : g * x[y][z];
+      }
     }
   }
+  l = wave_sumf(l);
   const int t = i / a.G, hq = h * a.G + i % a.G;
   const long long out = ((long long)b * a.T + t) * a.Hq + hq;
 #pragma unroll
@@ -281,6 +344,5 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 hipError_t launch_attn_narrow(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st);
 hipError_t launch_attn_wide(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st);
 hipError_t set_attn_narrow_lds(size_t bytes);
-hipError_t set_attn_wide_lds(size_t bytes);
 
 }  // namespace tgs

@@ -15,7 +15,7 @@ namespace attn {
 
 
 template <int D, int QT>
-constexpr int narrow_waves() { return D * QT >= 512 || D == 256 ? 4 : 8; }
+constexpr int narrow_waves() { return 4; }
 
 template <typename DT, int D, int QT, int NW>
 struct Narrow {
@@ -35,12 +35,16 @@ struct Narrow {
   bool bad;
 
   __device__ __forceinline__ Narrow(const AttnArgs& a_)
-      : a(a_), lane(lane_id()), wave((int)threadIdx.x >> 6), col(lane & 15), grp(lane >> 4), b(0), h(0), len(0), nc(0),
+      : a(a_), lane(lane_id()), wave((int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), col(lane & 15), grp(lane >> 4), b(0), h(0), len(0), nc(0),
         table(nullptr), bad(false) {}
 
-  // Page entries of tile i for the lane's key block and value block.
+  struct State {
+    f32x4 o[QT][DT16];
+    float m[QT], l[QT];  // (l: of the lane's tokens alone)
+  };
+
+  // Page entries of cache tile i for the lane's key block and value block.
   __device__ __forceinline__ int2 entries(int i) const {
-    if (i >= nc) return make_int2(0, 0);
     const int kb = i * NTILE + (col >> 2) * 8, vb = i * NTILE + grp * 8;
     const int last = len - 1;
     return make_int2(table[(kb < last ? kb : last) >> a.page_shift], table[(vb < last ? vb : last) >> a.page_shift]);
@@ -53,46 +57,101 @@ struct Narrow {
     return e;
   }
 
-  // Keys of tile i: product row r = 4 g + j of half t is token 8 g + 4 t + j.
-  __device__ __forceinline__ void load_keys(int i, int entry, uint4 (&k)[2][KK]) {
-    const int tok = (col >> 2) * 8 + (col & 3);
-    if (i < nc) {
-      const uint16_t* base = (const uint16_t*)a.k + page_of(entry) * a.k_page + (((long long)h * D) << a.page_shift) + grp * 8;
+  // Keys of cache tile i: product row r = 4 g + j of half t is token 8 g + 4 t + j.
+  __device__ __forceinline__ void load_keys(int i, int entry, Vec (&k)[2][KK]) {
+    const uint16_t* base = (const uint16_t*)a.k + page_of(entry) * a.k_page + (((long long)h * D) << a.page_shift) + grp * 8;
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        int p = i * NTILE + tok + 4 * t;
-        p = (p < len ? p : len - 1) & ((1 << a.page_shift) - 1);
+    for (int t = 0; t < 2; t++) {
+      int p = i * NTILE + (col >> 2) * 8 + (col & 3) + 4 * t;
+      p = (p < len ? p : len - 1) & ((1 << a.page_shift) - 1);
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) k[t][kk] = *(const uint4*)(base + p * D + kk * 32);
+      for (int kk = 0; kk < KK; kk++) k[t][kk] = *(const Vec*)(base + p * D + kk * 32);
+    }
+  }
+  __device__ __forceinline__ void load_values(int i, int entry, Vec (&v)[DT16]) {
+    const int blk = i * NTILE + grp * 8, last = (len - 1) & ~7;
+    const int p = (blk < last ? blk : last) & ((1 << a.page_shift) - 1);
+    const uint16_t* base = (const uint16_t*)a.v + page_of(entry) * a.v_page + (((long long)h * D) << a.page_shift) +
+                           (long long)p * D + col * 8;
+#pragma unroll
+    for (int d = 0; d < DT16; d++) v[d] = *(const Vec*)(base + d * 128);
+  }
+
+  // The same of the drafted nodes from node t0 on.  Their values come row by
+  // row and turn into blocks of eight tokens in registers and through `turn`,
+  // the wave's own 4 D vectors of LDS.
+  __device__ __forceinline__ void load_tree(int t0, Vec* turn, Vec (&k)[2][KK], Vec (&v)[DT16]) const {
+    const uint16_t* kb = (const uint16_t*)a.k_new + b * a.kn_b + h * a.kn_h + grp * 8;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      int p = t0 + (col >> 2) * 8 + (col & 3) + 4 * t;
+      p = p < a.T ? p : a.T - 1;
+#pragma unroll
+      for (int kk = 0; kk < KK; kk++) k[t][kk] = load16(kb + p * a.kn_t + kk * 32);
+    }
+    const uint16_t* vb = (const uint16_t*)a.v_new + b * a.vn_b + h * a.vn_h;
+#pragma unroll 1
+    for (int c = col; c < D / 8; c += 16) {
+      Vec x[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int p = t0 + grp * 8 + j;
+        x[j] = vec16(0, 0, 0, 0);
+        if (p < a.T) x[j] = load16(vb + p * a.vn_t + c * 8);
       }
-    } else {
-      const uint16_t* base = (const uint16_t*)a.k_new + b * a.kn_b + h * a.kn_h + grp * 8;
+      transpose8(x);
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        int p = (i - nc) * NTILE + tok + 4 * t;
-        p = p < a.T ? p : a.T - 1;
+      for (int j = 0; j < 8; j++) turn[grp * D + c * 8 + j] = x[j];
+    }
+    wave_lds_sync();
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) k[t][kk] = load_row16<false>(base + p * a.kn_t + kk * 32);
+    for (int d = 0; d < DT16; d++) v[d] = turn[grp * D + d * 16 + col];
+  }
+
+  __device__ __forceinline__ void scores(const Vec (&k)[2][KK], const Vec (&q)[QT][KK], f32x4 (&sc)[QT][2]) const {
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        sc[t][x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) sc[t][x] = mfma16<DT>(k[x][kk], q[t][kk], sc[t][x]);
       }
+  }
+
+  __device__ __forceinline__ void weights(const f32x4 (&sc)[QT][2], State& s, Vec (&p)[QT]) const {
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      float top = sc[t][0][0];
+#pragma unroll
+      for (int j = 1; j < 8; j++) top = fmaxf(top, sc[t][j >> 2][j & 3]);
+      top *= a.scale_log2;
+      if (__ballot(top > s.m[t] + SLACK)) {
+        top = fmaxf(top, xor_lane<16>(top));
+        top = fmaxf(top, xor_lane<32>(top));
+        const float now = fmaxf(s.m[t], top);
+        const float f = s.m[t] == NEG ? 0.0f : exp2_hw(s.m[t] - now);
+        s.m[t] = now;
+        s.l[t] *= f;
+#pragma unroll
+        for (int d = 0; d < DT16; d++) s.o[t][d] *= f;
+      }
+      const float base = s.m[t] == NEG ? 0.0f : s.m[t];
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        w[j] = exp2_hw(__builtin_fmaf(sc[t][j >> 2][j & 3], a.scale_log2, -base));
+        s.l[t] += w[j];
+      }
+      p[t] = vec16(pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7]));
     }
   }
 
-  __device__ __forceinline__ void load_values(int i, int entry, uint4 (&v)[DT16]) {
-    if (i < nc) {
-      const int blk = i * NTILE + grp * 8, last = (len - 1) & ~7;
-      const int p = (blk < last ? blk : last) & ((1 << a.page_shift) - 1);
-      const uint16_t* base = (const uint16_t*)a.v + page_of(entry) * a.v_page + (((long long)h * D) << a.page_shift) +
-                             (long long)p * D + col * 8;
+  __device__ __forceinline__ void add(const Vec (&v)[DT16], const Vec (&p)[QT], State& s) const {
 #pragma unroll
-      for (int d = 0; d < DT16; d++) v[d] = *(const uint4*)(base + d * 128);
-    } else {
-      const uint16_t* base = (const uint16_t*)a.v_new + b * a.vn_b + h * a.vn_h + col;
+    for (int d = 0; d < DT16; d++)
 #pragma unroll
-      for (int d = 0; d < DT16; d++) {
-        v[d] = tree_values(base + d * 16, a.vn_t, (i - nc) * NTILE + grp * 8, a.T);
-        sched_fence();  // (all of them at once would take 8 D / 16 registers)
-      }
-    }
+      for (int t = 0; t < QT; t++) s.o[t][d] = mfma16<DT>(v[d], p[t], s.o[t][d]);
   }
 
   // Tiles [t0, t1) of (b, h); full: they are all of it.  part: the workspace's rows otherwise.
@@ -101,111 +160,92 @@ struct Narrow {
     nc = (len + NTILE - 1) / NTILE;
     table = a.tables + (long long)b * a.P;
     bad = false;
-    const u64 anc = t1 > nc ? ancestors(a, b) : 0ull;  // of node `lane`
-    uint4 q[QT][KK];
-    u64 sees[QT];
+    Vec q[QT][KK];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
       const int i = t * 16 + col;
       const int node = i < a.M ? i / a.G : 0, hg = i < a.M ? i - node * a.G : 0;
       const uint16_t* p = (const uint16_t*)a.q + b * a.q_b + node * a.q_t + (long long)(h * a.G + hg) * a.q_h + grp * 8;
 #pragma unroll
-      for (int kk = 0; kk < KK; kk++) q[t][kk] = load_row16<false>(p + kk * 32);
-      sees[t] = ((u64)(uint32_t)__shfl((int)(anc >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)anc, node, 64);
+      for (int kk = 0; kk < KK; kk++) q[t][kk] = load16(p + kk * 32);
     }
-    f32x4 o[QT][DT16];
-    float m[QT], l[QT];
+    State st;
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-      m[t] = NEG;
-      l[t] = 0.0f;
+      st.m[t] = NEG;
+      st.l[t] = 0.0f;
 #pragma unroll
-      for (int d = 0; d < DT16; d++) o[t][d] = f32x4{0, 0, 0, 0};
+      for (int d = 0; d < DT16; d++) st.o[t][d] = f32x4{0, 0, 0, 0};
     }
-    uint4 k[2][KK], v[DT16];
+    Vec k[2][KK], v[DT16], p[QT];
+    f32x4 sc[QT][2];
     int i = t0 + wave;
-    if (i < t1) {
+    const int tc = t1 < nc ? t1 : nc;  // the end of the cache's tiles
+    if (i < tc) {
+      // Requests complete in order: a tile's keys, the entries of the tile
+      // after the next, then its values, each waited for with what follows it
+      // still on the way.  Only the last tile can end inside.
       int2 e = entries(i);
       load_keys(i, e.x, k);
+      sched_fence();
+      int2 next = entries(i + NW < tc ? i + NW : i);
+      sched_fence();
       load_values(i, e.y, v);
-      e = i + NW < t1 ? entries(i + NW) : e;
-      for (; i < t1; i += NW) {
-        f32x4 sc[QT][2];
+      sched_fence();
+      for (; i + NW < tc; i += NW) {
+        scores(k, q, sc);
+        e = next;
+        load_keys(i + NW, e.x, k);
+        sched_fence();
+        next = entries(i + 2 * NW < tc ? i + 2 * NW : i);
+        sched_fence();
+        weights(sc, st, p);
+        add(v, p, st);
+        load_values(i + NW, e.y, v);
+        sched_fence();
+      }
+      scores(k, q, sc);
+      const int left = len - i * NTILE - grp * 8;  // of the lane's eight tokens
+      if ((i + 1) * NTILE > len) {
 #pragma unroll
         for (int t = 0; t < QT; t++)
 #pragma unroll
-          for (int x = 0; x < 2; x++) {
-            sc[t][x] = f32x4{0, 0, 0, 0};
+          for (int j = 0; j < 8; j++)
+            if (j >= left) sc[t][j >> 2][j & 3] = NEG;
+        // what lies past the end is not 0 (it may be anything, NaN too)
 #pragma unroll
-            for (int kk = 0; kk < KK; kk++) sc[t][x] = mfma16<DT>(k[x][kk], q[t][kk], sc[t][x]);
-          }
-        const bool more = i + NW < t1;
-        if (more) load_keys(i + NW, e.x, k);
-        const int first = i * NTILE + grp * 8;  // the lane's eight tokens
-        if (i >= nc) {
-#pragma unroll
-          for (int t = 0; t < QT; t++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-              const int tok = (i - nc) * NTILE + grp * 8 + j;
-              if (!((sees[t] >> tok) & 1)) sc[t][j >> 2][j & 3] = NEG;
-            }
-        } else if ((i + 1) * NTILE > len) {
-#pragma unroll
-          for (int t = 0; t < QT; t++)
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-              if (first + j >= len) sc[t][j >> 2][j & 3] = NEG;
-          // what lies past the end is not 0 (it may be anything, NaN too)
-#pragma unroll
-          for (int d = 0; d < DT16; d++) v[d] = keep_first(v[d], len - first);
-        }
-        uint4 p[QT];
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-          float top = sc[t][0][0];
-#pragma unroll
-          for (int j = 1; j < 8; j++) top = fmaxf(top, sc[t][j >> 2][j & 3]);
-          top *= a.scale_log2;
-          if (__ballot(top > m[t] + SLACK)) {
-            top = fmaxf(top, xor_lane<16>(top));
-            top = fmaxf(top, xor_lane<32>(top));
-            const float now = fmaxf(m[t], top);
-            const float f = m[t] == NEG ? 0.0f : exp2_hw(m[t] - now);
-            m[t] = now;
-            l[t] *= f;
-#pragma unroll
-            for (int d = 0; d < DT16; d++) o[t][d] *= f;
-          }
-          const float base = m[t] == NEG ? 0.0f : m[t];
-          float w[8];
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            w[j] = exp2_hw(__builtin_fmaf(sc[t][j >> 2][j & 3], a.scale_log2, -base));
-            l[t] += w[j];
-          }
-          p[t] = make_uint4(pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7]));
-        }
-#pragma unroll
-        for (int d = 0; d < DT16; d++)
-#pragma unroll
-          for (int t = 0; t < QT; t++) o[t][d] = mfma16<DT>(v[d], p[t], o[t][d]);
-        if (more) {
-          load_values(i + NW, e.y, v);
-          if (i + 2 * NW < t1) e = entries(i + 2 * NW);
-        }
+        for (int d = 0; d < DT16; d++) v[d] = keep_first(v[d], left);
       }
+      weights(sc, st, p);
+      add(v, p, st);
+      i += NW;
+    }
+    for (; i < t1; i += NW) {
+      const u64 anc = ancestors(a, b);  // of node `lane`
+      load_tree((i - nc) * NTILE, (Vec*)s.o[wave], k, v);
+      scores(k, q, sc);
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        const int node = t * 16 + col < a.M ? (t * 16 + col) / a.G : 0;
+        const u64 sees = ((u64)(uint32_t)__shfl((int)(anc >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)anc, node, 64);
+        const uint32_t in = (uint32_t)(sees >> ((i - nc) * NTILE + grp * 8));
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (!((in >> j) & 1)) sc[t][j >> 2][j & 3] = NEG;
+      }
+      weights(sc, st, p);
+      add(v, p, st);
     }
     // the waves' states
     const bool any_bad = __ballot(bad) != 0;
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-      l[t] += xor_lane<16>(l[t]);
-      l[t] += xor_lane<32>(l[t]);
-      if (any_bad) l[t] = __builtin_nanf("");
+      st.l[t] += xor_lane<16>(st.l[t]);
+      st.l[t] += xor_lane<32>(st.l[t]);
+      if (any_bad) st.l[t] = __builtin_nanf("");
       if (grp == 0) {
-        s.ml[wave][t * 16 + col][0] = m[t];
-        s.ml[wave][t * 16 + col][1] = l[t];
+        s.ml[wave][t * 16 + col][0] = st.m[t];
+        s.ml[wave][t * 16 + col][1] = st.l[t];
       }
     }
     __syncthreads();
@@ -219,9 +259,9 @@ struct Narrow {
         const float mw = s.ml[w][t * 16 + col][0];
         sum += s.ml[w][t * 16 + col][1] * (mw == NEG ? 1.0f : exp2_hw(mw - top));
       }
-      const float f = m[t] == NEG ? 0.0f : exp2_hw(m[t] - top);
+      const float f = st.m[t] == NEG ? 0.0f : exp2_hw(st.m[t] - top);
 #pragma unroll
-      for (int d = 0; d < DT16; d++) s.o[wave][d * QT + t][lane] = o[t][d] * f;
+      for (int d = 0; d < DT16; d++) s.o[wave][d * QT + t][lane] = st.o[t][d] * f;
       if (wave == 0 && grp == 0) {
         s.tot[t * 16 + col][0] = top;
         s.tot[t * 16 + col][1] = sum;
@@ -253,7 +293,7 @@ struct Narrow {
 };
 
 template <typename DT, int D, int QT, int NW>
-__global__ __launch_bounds__(NW * 64, NW / 4) void narrow_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void narrow_kernel(AttnArgs a) {
   typedef Narrow<DT, D, QT, NW> K;
   TGS_DYN_SMEM(dyn);
   typename K::Shared& s = *(typename K::Shared*)dyn;

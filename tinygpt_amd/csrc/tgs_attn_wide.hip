@@ -2,8 +2,8 @@
 // rows: a tile's keys and values go through LDS, where every wave of the
 // workgroup, each with 32 rows of its own, reads them.
 //
-// Tiles of 64 tokens.  The next tile is on its way to registers while this
-// one is worked on.  Keys lie in LDS row by row with the 16-byte chunks of a
+// Tiles of 64 tokens, two in LDS and one or two more on their way to
+// registers, one barrier a tile.  Keys lie in LDS row by row with the 16-byte chunks of a
 // row permuted by the row's number, so that the 16 lanes served together take
 // 16 different chunks; values lie as in the cache, where a lane's operands
 // are neighbours already.
@@ -19,9 +19,10 @@ struct Wide {
   static constexpr int NTHR = QW * 64, KK = D / 16, DT32 = D / 32, C = D / 8;
   static constexpr int NCH = (WTILE * C + NTHR - 1) / NTHR;  // chunks a thread moves, of keys and of values
   static constexpr bool EVEN = WTILE * C % NTHR == 0;
+  static constexpr int AHEAD = NCH <= 4 ? 2 : 1;  // tiles on their way (a tile takes 8 NCH registers)
   struct Shared {
-    uint4 k[WTILE * C];
-    uint4 v[WTILE * C];
+    Vec k[2][WTILE * C];
+    Vec v[2][WTILE * C];
   };
 
   const AttnArgs& a;
@@ -31,7 +32,7 @@ struct Wide {
   bool bad;
 
   __device__ __forceinline__ Wide(const AttnArgs& a_)
-      : a(a_), tid((int)threadIdx.x), lane(lane_id()), wave(tid >> 6), col(lane & 31), half(lane >> 5), b(0), h(0), qb(0),
+      : a(a_), tid((int)threadIdx.x), lane(lane_id()), wave((int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), col(lane & 31), half(lane >> 5), b(0), h(0), qb(0),
         len(0), nc(0), table(nullptr), bad(false) {}
 
   // Where chunk ch of row tok lies.
@@ -44,55 +45,60 @@ struct Wide {
     }
   }
 
-  // Page of each of the tile's eight 8-token blocks, block lane % 8 in a lane.
+  // Page of each of cache tile i's eight 8-token blocks, block lane % 8 in a
+  // lane; of a block past the end, the last one's.
   __device__ __forceinline__ int entries(int i) const {
-    if (i >= nc) return 0;
     const int blk = i * WTILE + (lane & 7) * 8, last = len - 1;
     return table[(blk < last ? blk : last) >> a.page_shift];
   }
 
-  __device__ __forceinline__ void load(int i, int entry, uint4 (&k)[NCH], uint4 (&v)[NCH]) {
-    if (i < nc) {  // (the drafted nodes' tile goes to LDS directly)
-      if ((unsigned)entry >= (unsigned)a.n_pages) {
-        bad = true;  // (its sequence's rows become NaN)
-        entry = 0;
-      }
-      const long long head = ((long long)h * D) << a.page_shift;
-      const int mask = (1 << a.page_shift) - 1;
-      const bool tail = (i + 1) * WTILE > len;
-#pragma unroll
-      for (int n = 0; n < NCH; n++) {
-        const int c = EVEN || n * NTHR + tid < WTILE * C ? n * NTHR + tid : 0;
-        const int tok = c / C, ch = c - tok * C;
-        int p = i * WTILE + tok;
-        p = p < len ? p : len - 1;
-        const long long pg = __shfl(entry, tok >> 3, 64);
-        k[n] = *(const uint4*)((const uint16_t*)a.k + pg * a.k_page + head + (long long)(p & mask) * D + ch * 8);
-      }
-#pragma unroll
-      for (int n = 0; n < NCH; n++) {
-        const int c = EVEN || n * NTHR + tid < WTILE * C ? n * NTHR + tid : 0;
-        const int blk = c / D, d = c - blk * D;
-        int p = i * WTILE + blk * 8;
-        const int last = (len - 1) & ~7;
-        const int first = p;
-        p = p < last ? p : last;
-        const long long pg = __shfl(entry, blk, 64);
-        v[n] = *(const uint4*)((const uint16_t*)a.v + pg * a.v_page + head + (long long)(p & mask) * D + d * 8);
-        // what lies past the end is not 0 (it may be anything, NaN too)
-        if (tail) v[n] = keep_first(v[n], len - first);
-      }
-    }
+  // Where chunk c's 8-token block blk of tile i lies in its pool, in elements.
+  // The chunks of a wave belong to one block (but for rows of 12 chunks), so this is
+  // scalar arithmetic.
+  __device__ __forceinline__ long long block_at(int i, int blk, int entry, long long page) const {
+    const int last = (len - 1) >> 3, x = i * (WTILE / 8) + blk;
+    const int in_page = ((x < last ? x : last) << 3) & ((1 << a.page_shift) - 1);
+    long long pg;
+    if constexpr (C == 12)
+      pg = __shfl(entry, blk, 64);
+    else
+      pg = (int)readlane_u32((uint32_t)entry, blk);
+    return pg * page + (((long long)h * D) << a.page_shift) + (long long)in_page * D;
+  }
+  // A chunk's index, its wave's for the block's sake.
+  __device__ __forceinline__ int chunk(int n) const {
+    const int c = n * NTHR + tid;
+    return EVEN || c < WTILE * C ? c : 0;
+  }
+  template <int PER>  // chunks of a block of tokens
+  __device__ __forceinline__ int block_of(int n) const {
+    if constexpr (C == 12) return chunk(n) / PER;
+    return (n * NTHR + wave * 64) / PER;
   }
 
-  __device__ __forceinline__ void store(Shared& s, const uint4 (&k)[NCH], const uint4 (&v)[NCH]) {
+  __device__ __forceinline__ void load(int i, int entry, Vec (&k)[NCH], Vec (&v)[NCH]) {
+    if ((unsigned)entry >= (unsigned)a.n_pages) {
+      bad = true;  // (its sequence's rows become NaN)
+      entry = 0;
+    }
+#pragma unroll
+    for (int n = 0; n < NCH; n++)
+      k[n] = *(const Vec*)((const uint16_t*)a.k + block_at(i, block_of<8 * C>(n), entry, a.k_page) + chunk(n) % (8 * C) * 8);
+#pragma unroll
+    for (int n = 0; n < NCH; n++)
+      v[n] = *(const Vec*)((const uint16_t*)a.v + block_at(i, block_of<D>(n), entry, a.v_page) + chunk(n) % D * 8);
+  }
+
+  // To buffer f; what lies past the sequence's end is not 0 there (it may be
+  // anything, NaN too), and is 0 here.
+  __device__ __forceinline__ void store(Shared& s, int f, int i, const Vec (&k)[NCH], const Vec (&v)[NCH]) {
+    const bool tail = (i + 1) * WTILE > len;
 #pragma unroll
     for (int n = 0; n < NCH; n++) {
       const int c = n * NTHR + tid;
       if (EVEN || c < WTILE * C) {
-        const int tok = c / C;
-        s.k[at_key(tok, c - tok * C)] = k[n];
-        s.v[c] = v[n];
+        s.k[f][at_key(c / C, c % C)] = k[n];
+        s.v[f][c] = tail ? keep_first(v[n], len - i * WTILE - c / D * 8) : v[n];
       }
     }
   }
@@ -104,9 +110,59 @@ struct Wide {
 #pragma unroll 1
     for (int c = tid; c < WTILE * C; c += NTHR) {
       const int tok = c / C, ch = c - tok * C, p = t0 + tok < a.T ? t0 + tok : a.T - 1;
-      s.k[at_key(tok, ch)] = load_row16<false>(kb + p * a.kn_t + ch * 8);
+      s.k[0][at_key(tok, ch)] = load16(kb + p * a.kn_t + ch * 8);
       const int blk = c / D, d = c - blk * D;
-      s.v[c] = tree_values(vb + d, a.vn_t, t0 + blk * 8, a.T);
+      s.v[0][c] = tree_values(vb + d, a.vn_t, t0 + blk * 8, a.T);
+    }
+  }
+
+  struct State {
+    f32x16 o[DT32];
+    float m, l;
+  };
+
+  // S^T of the tile in buffer f: element j of half x is token 32 x + 16 (j / 8) + 8 half + j % 8.
+  __device__ __forceinline__ void scores(const Shared& s, int f, const Vec (&q)[KK], f32x16 (&sc)[2]) const {
+    // product row r = 8 x + 4 y + j (j < 4, y < 2) of a half tile is its token 16 (x / 2) + 8 y + 4 (x % 2) + j
+    const int tok = (col >> 4) * 16 + ((col >> 2) & 1) * 8 + ((col >> 3) & 1) * 4 + (col & 3);
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) sc[x][j] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+      for (int x = 0; x < 2; x++) sc[x] = mfma32<DT>(s.k[f][at_key(x * 32 + tok, kk * 2 + half)], q[kk], sc[x]);
+  }
+
+  __device__ __forceinline__ void add(const Shared& s, int f, const f32x16 (&sc)[2], State& st) const {
+    float top = sc[0][0];
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) top = fmaxf(top, sc[x][j]);
+    top *= a.scale_log2;
+    if (__ballot(top > st.m + SLACK)) {
+      top = fmaxf(top, xor_lane<32>(top));
+      const float now = fmaxf(st.m, top);
+      const float g = st.m == NEG ? 0.0f : exp2_hw(st.m - now);
+      st.m = now;
+      st.l *= g;
+#pragma unroll
+      for (int d = 0; d < DT32; d++) st.o[d] *= g;
+    }
+    const float base = st.m == NEG ? 0.0f : st.m;
+#pragma unroll
+    for (int y = 0; y < 4; y++) {  // the 16 tokens 16 y .. of the tile
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        w[j] = exp2_hw(__builtin_fmaf(sc[y >> 1][(y & 1) * 8 + j], a.scale_log2, -base));
+        st.l += w[j];
+      }
+      const Vec p = vec16(pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7]));
+#pragma unroll
+      for (int d = 0; d < DT32; d++) st.o[d] = mfma32<DT>(s.v[f][(y * 2 + half) * D + d * 32 + col], p, st.o[d]);
     }
   }
 
@@ -119,95 +175,94 @@ struct Wide {
     const bool work = row0 < a.M;
     const int i = row0 + col;
     const int node = i < a.M ? i / a.G : 0, hg = i < a.M ? i - node * a.G : 0;
-    u64 sees = t1 > nc ? ancestors(a, b) : 0ull;
-    sees = ((u64)(uint32_t)__shfl((int)(sees >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)sees, node, 64);
-    uint4 q[KK];
+    Vec q[KK];
     {
       const uint16_t* p = (const uint16_t*)a.q + b * a.q_b + node * a.q_t + (long long)(h * a.G + hg) * a.q_h + half * 8;
 #pragma unroll
-      for (int kk = 0; kk < KK; kk++) q[kk] = load_row16<false>(p + kk * 16);
+      for (int kk = 0; kk < KK; kk++) q[kk] = load16(p + kk * 16);
     }
-    // product row r = 8 x + 4 y + j (j < 4, y < 2) of a half tile is its token 16 (x / 2) + 8 y + 4 (x % 2) + j
-    const int tok = (col >> 4) * 16 + ((col >> 2) & 1) * 8 + ((col >> 3) & 1) * 4 + (col & 3);
-    f32x16 o[DT32];
-    float m = NEG, l = 0.0f;
+    State st;
+    st.m = NEG;
+    st.l = 0.0f;
 #pragma unroll
     for (int d = 0; d < DT32; d++)
 #pragma unroll
-      for (int x = 0; x < 16; x++) o[d][x] = 0.0f;
-    uint4 k[NCH], v[NCH];
-    int e = entries(t0);
-    load(t0, e, k, v);
-    e = t0 + 1 < t1 ? entries(t0 + 1) : e;
-    for (int t = t0; t < t1; t++) {
-      __syncthreads();
-      if (t < nc)
-        store(s, k, v);
-      else
-        store_tree(s, (t - nc) * WTILE);
-      __syncthreads();
-      if (t + 1 < t1) {
-        load(t + 1, e, k, v);
-        e = t + 2 < t1 ? entries(t + 2) : e;
+      for (int x = 0; x < 16; x++) st.o[d][x] = 0.0f;
+    f32x16 sc[2];
+    const int tc = t1 < nc ? t1 : nc;  // the end of the cache's tiles
+    lds_barrier();                     // (the buffers are free)
+    if (t0 < tc) {
+      // Tile t is worked on in one buffer while t + 1 goes to the other and
+      // the next AHEAD ones are on their way to registers; requests past the
+      // last tile ask for it again, so that the number in flight is known.
+      auto cut = [&](int t) { return t < tc ? t : tc - 1; };
+      Vec k0[NCH], v0[NCH], k1[NCH], v1[NCH];
+      int e = entries(t0), next = entries(cut(t0 + 1));
+      load(t0, e, k0, v0);
+      sched_fence();
+      store(s, 0, t0, k0, v0);
+      e = next;
+      next = entries(cut(t0 + 2));
+      sched_fence();
+      load(cut(t0 + 1), e, k0, v0);
+      sched_fence();
+      if constexpr (AHEAD == 2) {
+        e = next;
+        next = entries(cut(t0 + 3));
+        sched_fence();
+        load(cut(t0 + 2), e, k1, v1);
+        sched_fence();
       }
-      if (!work) continue;
-      f32x16 sc[2];
+      lds_barrier();
+      auto step = [&](int t, int f, Vec (&ks)[NCH], Vec (&vs)[NCH]) {
+        store(s, f ^ 1, cut(t + 1), ks, vs);
+        e = next;
+        next = entries(cut(t + 2 + AHEAD));
+        sched_fence();
+        load(cut(t + 1 + AHEAD), e, ks, vs);
+        sched_fence();
+        if (work) {
+          scores(s, f, q, sc);
+          if ((t + 1) * WTILE > len) {
+            const int left = len - t * WTILE - 8 * half;
 #pragma unroll
-      for (int x = 0; x < 2; x++) {
+            for (int x = 0; x < 2; x++)
 #pragma unroll
-        for (int j = 0; j < 16; j++) sc[x][j] = 0.0f;
-#pragma unroll
-        for (int kk = 0; kk < KK; kk++)
-          sc[x] = mfma32<DT>(s.k[at_key(x * 32 + tok, kk * 2 + half)], q[kk], sc[x]);
+              for (int j = 0; j < 16; j++)
+                if (32 * x + 16 * (j >> 3) + (j & 7) >= left) sc[x][j] = NEG;
+          }
+          add(s, f, sc, st);
+        }
+        lds_barrier();
+      };
+      for (int t = t0;;) {
+        step(t, 0, k0, v0);
+        if (++t == tc) break;
+        if constexpr (AHEAD == 2)
+          step(t, 1, k1, v1);
+        else
+          step(t, 1, k0, v0);
+        if (++t == tc) break;
       }
-      // element j of half tile x is token 32 x + 16 (j / 8) + 8 half + j % 8
-      if (t >= nc) {
+    }
+    if (t1 > nc) {
+      store_tree(s, 0);
+      u64 sees = ancestors(a, b);
+      sees = ((u64)(uint32_t)__shfl((int)(sees >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)sees, node, 64);
+      lds_barrier();
+      if (work) {
+        scores(s, 0, q, sc);
         const u64 in = sees >> (8 * half);
 #pragma unroll
         for (int x = 0; x < 2; x++)
 #pragma unroll
           for (int j = 0; j < 16; j++)
             if (!((in >> (32 * x + 16 * (j >> 3) + (j & 7))) & 1)) sc[x][j] = NEG;
-      } else if ((t + 1) * WTILE > len) {
-        const int left = len - t * WTILE - 8 * half;
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-          for (int j = 0; j < 16; j++)
-            if (32 * x + 16 * (j >> 3) + (j & 7) >= left) sc[x][j] = NEG;
+        add(s, 0, sc, st);
       }
-      float top = sc[0][0];
-#pragma unroll
-      for (int x = 0; x < 2; x++)
-#pragma unroll
-        for (int j = 0; j < 16; j++) top = fmaxf(top, sc[x][j]);
-      top *= a.scale_log2;
-      if (__ballot(top > m + SLACK)) {
-        top = fmaxf(top, xor_lane<32>(top));
-        const float now = fmaxf(m, top);
-        const float f = m == NEG ? 0.0f : exp2_hw(m - now);
-        m = now;
-        l *= f;
-#pragma unroll
-        for (int d = 0; d < DT32; d++) o[d] *= f;
-      }
-      const float base = m == NEG ? 0.0f : m;
-      uint4 p[4];
-#pragma unroll
-      for (int y = 0; y < 4; y++) {  // the 16 tokens 16 y .. of the tile
-        float w[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          w[j] = exp2_hw(__builtin_fmaf(sc[y >> 1][(y & 1) * 8 + j], a.scale_log2, -base));
-          l += w[j];
-        }
-        p[y] = make_uint4(pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7]));
-      }
-#pragma unroll
-      for (int y = 0; y < 4; y++)
-#pragma unroll
-        for (int d = 0; d < DT32; d++) o[d] = mfma32<DT>(s.v[(y * 2 + half) * D + d * 32 + col], p[y], o[d]);
     }
+    float m = st.m, l = st.l;
+    const f32x16(&o)[DT32] = st.o;
     l += xor_lane<32>(l);
     if (__ballot(bad)) l = __builtin_nanf("");  // (every wave read every entry)
     if (i >= a.M) return;
@@ -295,11 +350,33 @@ hipError_t wide_run(const AttnArgs& a, hipStream_t st) {
 
 template <typename DT, int D>
 hipError_t wide_dim(const AttnArgs& a, int qw, hipStream_t st) {
-  if (qw == 2) return wide_run<DT, D, 2>(a, st);
+  if constexpr (D <= 128)
+    if (qw == 2) return wide_run<DT, D, 2>(a, st);
   if (qw == 4) return wide_run<DT, D, 4>(a, st);
   if constexpr (D <= 128)
     if (qw == 8) return wide_run<DT, D, 8>(a, st);
   return hipErrorInvalidValue;
+}
+template <typename DT, int D, int QW>
+hipError_t wide_lds() {
+  return hipFuncSetAttribute((const void*)wide_kernel<DT, D, QW>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)sizeof(typename Wide<DT, D, QW>::Shared));
+}
+template <typename DT>
+hipError_t wide_lds_type() {
+  hipError_t e = hipSuccess;
+  auto take = [&](hipError_t x) { e = x != hipSuccess ? x : e; };
+  take(wide_lds<DT, 64, 2>());
+  take(wide_lds<DT, 64, 4>());
+  take(wide_lds<DT, 64, 8>());
+  take(wide_lds<DT, 96, 2>());
+  take(wide_lds<DT, 96, 4>());
+  take(wide_lds<DT, 96, 8>());
+  take(wide_lds<DT, 128, 2>());
+  take(wide_lds<DT, 128, 4>());
+  take(wide_lds<DT, 128, 8>());
+  take(wide_lds<DT, 256, 4>());
+  return e;
 }
 template <typename DT>
 hipError_t wide_type(const AttnArgs& a, int qw, hipStream_t st) {
@@ -325,14 +402,14 @@ AttnPlan attn_plan(int M, int D) {
     p.qw = M <= 16 ? 1 : 2;
     p.tile = attn::NTILE;
     p.QB = 16 * p.qw;
-    p.per_cu = 1;
-    p.least = 8;  // one per wave
+    p.per_cu = D == 256 ? 1 : 2;
+    p.least = 4;  // one per wave
   } else {
     p.wide = 1;
-    p.qw = M <= 64 ? 2 : M <= 128 || D == 256 ? 4 : 8;
+    p.qw = D == 256 ? 4 : M <= 64 ? 2 : M <= 128 ? 4 : 8;
     p.tile = attn::WTILE;
     p.QB = 32 * p.qw;
-    p.per_cu = D == 256 ? 1 : 8 / p.qw;
+    p.per_cu = D == 256 || p.qw == 8 ? 1 : 2;
     p.least = 4;
   }
   p.nqb = (M + p.QB - 1) / p.QB;
@@ -343,6 +420,9 @@ hipError_t launch_attn(const AttnArgs& a, const AttnPlan& p, int dtype, hipStrea
   return p.wide ? launch_attn_wide(a, p, dtype, st) : launch_attn_narrow(a, p, dtype, st);
 }
 
-hipError_t set_attn_lds_limit(size_t bytes) { return set_attn_narrow_lds(bytes); }
+hipError_t set_attn_lds_limit(size_t bytes) {
+  const hipError_t e = set_attn_narrow_lds(bytes), f = attn::wide_lds_type<attn::BF16>(), g = attn::wide_lds_type<attn::F16>();
+  return e != hipSuccess ? e : f != hipSuccess ? f : g;
+}
 
 }  // namespace tgs

@@ -36,6 +36,11 @@ struct tgs_ctx {
 
 namespace tgs {
 
+// 8-byte words of workspace that tree attention's parts take when a launch
+// fills the chip: two parts per CU of 256 rows of 128 values (128 rows of
+// 256), a maximum and a sum each.
+inline size_t attn_ws_words(int num_cu) { return (size_t)num_cu * 256 * (128 + 2); }
+
 struct DeviceGuard {
   int prev = -1;
   bool ok = false;
