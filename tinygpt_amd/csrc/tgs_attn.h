@@ -159,10 +159,17 @@ __device__ __forceinline__ int lane_tiles(const AttnArgs& a, int b) {
   return (clamp_len(a, a.lens[b]) + TILE - 1) / TILE;
 }
 
+// What a (sequence, key head) costs beyond its tiles (queries, the first
+// tile's latency, the result), counted in tiles when shares are cut: a worker
+// whose share lies in short sequences would else end last (32 sequences of 100
+// to 4096 tokens, 8 key heads of 128: 86 us without, 63 with 4 or more).
+template <int TILE>
+constexpr int extra() { return TILE == NTILE ? 8 : 4; }
+
 // Tiles of sequences before b (of one key head), and of all: by one wave.
 template <int TILE>
 __device__ __forceinline__ void tiles_before(const AttnArgs& a, int b, int& before, int& all) {
-  const int tree = (a.T + TILE - 1) / TILE;
+  const int tree = (a.T + TILE - 1) / TILE + extra<TILE>();
   int x = 0, y = 0;
   for (int i = lane_id(); i < a.B; i += 64) {
     const int n = lane_tiles<TILE>(a, i) + tree;
@@ -173,38 +180,64 @@ __device__ __forceinline__ void tiles_before(const AttnArgs& a, int b, int& befo
   all = uniform(wave_sum(y));
 }
 
-// The sequence that holds tile t of one key head's tiles in order, and the tiles before it: by one wave.
-template <int TILE>
-__device__ __forceinline__ void find_tile(const AttnArgs& a, long long t, int heads, int& b, long long& before) {
-  const int tree = (a.T + TILE - 1) / TILE, lane = lane_id();
-  before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int n = b0 + lane < a.B ? lane_tiles<TILE>(a, b0 + lane) + tree : 0;
-    const int incl = wave_incl_scan(n);
-    const u64 ends = __ballot(b0 + lane < a.B && before + (long long)incl * heads > t);
-    if (ends) {
-      const int at = __ffsll((long long)ends) - 1;
-      b = b0 + at;
-      const int prev = (int)readlane_u32((uint32_t)incl, at) - (int)readlane_u32((uint32_t)n, at);
-      before += (long long)prev * heads;
-      return;
-    }
-    before += (long long)(int)readlane_u32((uint32_t)incl, 63) * heads;
-  }
-  b = a.B;
+// First tile of worker w's share: floor(U w / N), in 32 bits where U allows
+// (w < N <= 2^16: with U = q N + r it is w q + floor(w r / N)).
+__device__ __forceinline__ long long share_start(long long U, int N, int w) {
+  if (U >> 31) return U * w / N;
+  const unsigned q = (unsigned)U / (unsigned)N, r = (unsigned)U - q * (unsigned)N;
+  return (long long)w * q + (unsigned)w * r / (unsigned)N;
 }
 
-__device__ __forceinline__ long long share_start(long long U, int N, int w) { return U * w / N; }
+// A worker's place: its share [u0, u1), and of tile u0 the sequence, key head
+// and tile in them, with the tiles of that sequence (drafted nodes and the
+// extra ones, behind which nothing lies, included).
+struct Place {
+  long long u0, u1;
+  int b, h, at, nt;
+};
+template <int TILE>
+__device__ __forceinline__ Place find_place(const AttnArgs& a, int w) {
+  const int tree = (a.T + TILE - 1) / TILE + extra<TILE>(), lane = lane_id();
+  const int mine = lane < a.B ? lane_tiles<TILE>(a, lane) + tree : 0;  // (of the first 64 sequences)
+  int y = mine;
+  for (int i = lane + 64; i < a.B; i += 64) y += lane_tiles<TILE>(a, i) + tree;
+  const long long U = (long long)uniform(wave_sum(y)) * a.Hkv;
+  Place p{share_start(U, a.nwg, w), share_start(U, a.nwg, w + 1), 0, 0, 0, 0};
+  if (p.u0 == p.u1) return p;
+  long long before = 0;
+  for (int b0 = 0;; b0 += 64) {
+    const int n = b0 == 0 ? mine : b0 + lane < a.B ? lane_tiles<TILE>(a, b0 + lane) + tree : 0;
+    const int incl = wave_incl_scan(n);
+    const u64 ends = __ballot(b0 + lane < a.B && before + (long long)incl * a.Hkv > p.u0);
+    if (ends) {
+      const int at = __ffsll((long long)ends) - 1;
+      p.b = b0 + at;
+      p.nt = (int)readlane_u32((uint32_t)n, at);
+      before += (long long)((int)readlane_u32((uint32_t)incl, at) - p.nt) * a.Hkv;
+      const long long in = p.u0 - before;
+      p.h = in >> 31 ? (int)(in / p.nt) : (int)((unsigned)in / (unsigned)p.nt);
+      p.at = (int)(in - (long long)p.h * p.nt);
+      return p;
+    }
+    before += (long long)(int)readlane_u32((uint32_t)incl, 63) * a.Hkv;
+  }
+}
 
 // ------------------------------------------------------------------ the tree
 
-// Ancestors of each node, itself among them, as bits: by one wave, node in
-// lane.  A parent that is not an earlier node makes a root.
-__device__ __forceinline__ u64 ancestors(const AttnArgs& a, int b) {
+// The parent of node `lane` of sequence b: an earlier node, or -1.
+__device__ __forceinline__ int parent_of(const AttnArgs& a, int b) {
+  const int lane = lane_id();
+  if (!a.parents) return lane - 1;
+  const int par = lane < a.T ? a.parents[(long long)b * a.T + lane] : -1;
+  return par < lane ? par : -1;
+}
+
+// Ancestors of each node, itself among them, as bits, from its parent: by one
+// wave, node in lane.
+__device__ __forceinline__ u64 ancestors(const AttnArgs& a, int par) {
   const int lane = lane_id();
   if (!a.parents) return lane == 63 ? ~0ull : (2ull << lane) - 1;
-  int par = lane < a.T ? a.parents[(long long)b * a.T + lane] : -1;
-  if (par >= lane) par = -1;
   u64 m = 1ull << lane;
 #pragma unroll
   for (int i = 0; i < 6; i++) {  // paths double
@@ -219,10 +252,17 @@ __device__ __forceinline__ u64 ancestors(const AttnArgs& a, int b) {
   return m;
 }
 
-// Of the eight 16-bit values of x those with index < n stay (n <= 0: none), the others become 0.
-__device__ __forceinline__ Vec keep_first(Vec x, int n) {
-  auto word = [&](uint32_t w, int i) { return n >= i + 2 ? w : n == i + 1 ? w & 0xFFFFu : 0u; };
-  return vec16(word(x[0], 0), word(x[1], 2), word(x[2], 4), word(x[3], 6));
+// A mask of the first n of eight 16-bit values (n <= 0: none).
+__device__ __forceinline__ Vec first_of(int n) {
+  const u64 lo = n >= 4 ? ~0ull : n <= 0 ? 0ull : (1ull << (16 * n)) - 1;
+  const u64 hi = n >= 8 ? ~0ull : n <= 4 ? 0ull : (1ull << (16 * n - 64)) - 1;
+  return vec16((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+}
+
+// x where bit i of bits is set, else -inf.
+__device__ __forceinline__ float seen(float x, uint32_t bits, int i) {
+  const uint32_t m = (uint32_t)((int)(bits << (31 - i)) >> 31);
+  return tg_u2f((tg_f2u(x) & m) | (0xFF800000u & ~m));
 }
 
 // 8 x 8 16-bit values, rows x[j], turned: x[i] becomes the i-th of every row.
@@ -239,14 +279,6 @@ __device__ __forceinline__ void transpose8(Vec (&x)[8]) {
     x[2 * i] = vec16(lo(i, 0), lo(i, 2), lo(i, 4), lo(i, 6));
     x[2 * i + 1] = vec16(hi(i, 0), hi(i, 2), hi(i, 4), hi(i, 6));
   }
-}
-
-// Eight tokens' values of one d, tok .. tok + 7 of the drafted nodes; past the last 0.
-__device__ __forceinline__ Vec tree_values(const uint16_t* v, long long stride, int tok, int T) {
-  uint32_t x[8];
-#pragma unroll
-  for (int j = 0; j < 8; j++) x[j] = tok + j < T ? v[(tok + j) * stride] : 0u;
-  return vec16(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
 }
 
 // ------------------------------------------------------------------ results
@@ -274,75 +306,191 @@ __device__ __forceinline__ float wave_sumf(float x) {
   return x + xor_lane<1>(x);
 }
 
-// Joins the parts of (sequence, key head)s that several workers hold: a wave
-// per output row, in the workers' order.
-template <typename DT, int TILE>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
-  const int lane = lane_id();
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);  // (b, h, query row)
-  if (row >= (long long)a.B * a.Hkv * a.M) return;
-  const int i = (int)(row % a.M), bh = (int)(row / a.M), h = bh % a.Hkv, b = bh / a.Hkv;
-  int before, all;
-  tiles_before<TILE>(a, b, before, all);
-  const int nt = cache_tiles<TILE>(a, b) + (a.T + TILE - 1) / TILE;
-  const long long U = (long long)all * a.Hkv, s0 = (long long)before * a.Hkv + (long long)h * nt, s1 = s0 + nt;
-  const int N = a.nwg;
-  const int w0 = (int)(((s0 + 1) * N - 1) / U), w1 = (int)((s1 * N - 1) / U);
-  if (w0 == w1) return;
-  // A lane per part (64 at a time): its place, maximum and sum.  A worker's
-  // second part is the one that starts past its share's first tile.
-  const int qb = i / a.QB, r = i - qb * a.QB;
-  auto part_of = [&](int w) -> int {
-    if (w > w1) return -1;
-    const long long from = share_start(U, N, w);
-    if (from == share_start(U, N, w + 1)) return -1;
-    return ((qb * N + w) * 2 + (from < s0)) * a.QB + r;
-  };
-  float m = NEG;
-  for (int w = w0; w <= w1; w += 64) {
-    const int p = part_of(w + lane);
-    m = fmaxf(m, p < 0 ? NEG : a.part_ml[2ll * p]);
-  }
-  m = wave_maxf(m);
-  float l = 0.0f;
-  float o[4] = {0, 0, 0, 0};
-  for (int w = w0; w <= w1; w += 64) {
-    int p = part_of(w + lane);
-    const float f = p < 0 ? 0.0f : exp2_hw(a.part_ml[2ll * p] - m);
-    l += p < 0 ? 0.0f : f * a.part_ml[2ll * p + 1];
-    p = p < 0 ? 0 : p;  // (its factor is 0)
-    const int n = w1 - w + 1 < 64 ? w1 - w + 1 : 64;
-    for (int j = 0; j < n; j += 4) {
-      float x[4][4];
+// Joins the parts of (sequence, key head)s that several workers hold.  A
+// workgroup takes R rows of one (sequence, key head): with R = 1 its four
+// waves share the row's parts (few rows, many parts), with R = 16 each takes
+// four rows (the places of the parts are found once for them).  Every sum runs
+// in an order that the lengths alone fix.
+struct JoinShared {
+  int part[1024];  // rows of the workspace, of the parts of this (sequence, key head)
+  int n;
+  float o[4][256];
+  float ml[4][2];
+};
+constexpr int JOIN_NT = 256;
+
+// Row i of (b, h): its sums over its weights' sum; d = 64 z + lane.
+template <typename DT>
+__device__ __forceinline__ void write_row(const AttnArgs& a, int b, int h, int i, const float (&o)[4], float m, float l) {
+  const int lane = lane_id(), t = i / a.G, hq = h * a.G + i - t * a.G;
+  const long long out = ((long long)b * a.T + t) * a.Hq + hq;
+  const float rl = 1.0f / l;
 #pragma unroll
-      for (int y = 0; y < 4; y++) {  // (past the last part: part 0's values, not used)
-        const long long at = (long long)(int)readlane_u32((uint32_t)p, j + y < n ? j + y : j) * a.D;
+  for (int z = 0; z < 4; z++)
+    if (z * 64 + lane < a.D) ((uint16_t*)a.out)[out * a.D + z * 64 + lane] = (uint16_t)pack2<DT>(o[z] * rl, 0.0f);
+  if (a.lse && lane == 0) a.lse[out] = row_lse(m, l);
+}
+
+// Row i of (b, h) from n parts, a quarter of them a wave.
+template <typename DT>
+__device__ __forceinline__ void join_one(const AttnArgs& a, JoinShared& s, int b, int h, int i, int n) {
+  const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
+  const int j0 = n * wave / 4, j1 = n * (wave + 1) / 4;
+  float m = NEG;
+  for (int j = j0 + lane; j < j1; j += 64) m = fmaxf(m, a.part_ml[2ll * s.part[j]]);
+  m = wave_maxf(m);
+  float l = 0.0f, o[4] = {0, 0, 0, 0};
+  for (int c = j0; c < j1; c += 64) {
+    float f = 0.0f;
+    if (c + lane < j1) {
+      const long long p = s.part[c + lane];
+      const float pm = a.part_ml[2 * p];
+      f = pm == NEG ? 0.0f : exp2_hw(pm - m);
+      l += f * a.part_ml[2 * p + 1];
+    }
+    const int cn = j1 - c < 64 ? j1 - c : 64;
+    for (int j = 0; j < cn; j += 8) {
+      float x[8][4];
+#pragma unroll
+      for (int y = 0; y < 8; y++) {  // (past the last part: the last one's, not used)
+        const long long at = (long long)s.part[j + y < cn ? c + j + y : c + cn - 1] * a.D;
 #pragma unroll
         for (int z = 0; z < 4; z++) x[y][z] = z * 64 + lane < a.D ? a.part_o[at + z * 64 + lane] : 0.0f;
       }
 #pragma unroll
-      for (int y = 0; y < 4; y++) {
-        const float g = j + y < n ? readlane_f32(f, j + y < n ? j + y : j) : 0.0f;
+      for (int y = 0; y < 8; y++) {
+        if (j + y >= cn) break;
+        const float fy = readlane_f32(f, j + y);
 #pragma unroll
-        for (int z = 0; z < 4; z++) o[z] += g == 0.0f ? 0.0f : g * x[y][z];
+        for (int z = 0; z < 4; z++) o[z] += fy * x[y][z];
       }
     }
   }
   l = wave_sumf(l);
-  const int t = i / a.G, hq = h * a.G + i % a.G;
-  const long long out = ((long long)b * a.T + t) * a.Hq + hq;
+  s.ml[wave][0] = m;
+  s.ml[wave][1] = l;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int d = j * 64 + lane;
-    if (d < a.D) ((uint16_t*)a.out)[out * a.D + d] = (uint16_t)pack2<DT>(o[j] / l, 0.0f);
+  for (int z = 0; z < 4; z++) s.o[wave][z * 64 + lane] = o[z];
+  __syncthreads();
+  if (wave > 0) return;
+  float top = NEG;
+#pragma unroll
+  for (int w = 0; w < 4; w++) top = fmaxf(top, s.ml[w][0]);
+  l = 0.0f;
+#pragma unroll
+  for (int z = 0; z < 4; z++) o[z] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const float f = s.ml[w][0] == NEG ? 0.0f : exp2_hw(s.ml[w][0] - top);
+    l += f * s.ml[w][1];
+#pragma unroll
+    for (int z = 0; z < 4; z++) o[z] += f * s.o[w][z * 64 + lane];
   }
-  if (a.lse && lane == 0) a.lse[out] = row_lse(m, l);
+  write_row<DT>(a, b, h, i, o, top, l);
+}
+
+template <typename DT, int TILE, int R>
+__global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
+  TGS_STATIC_SMEM(JoinShared, s);
+  const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
+  const int g = blockIdx.x % groups, bh = blockIdx.x / groups, h = bh % a.Hkv, b = bh / a.Hkv;
+  int before, all;
+  tiles_before<TILE>(a, b, before, all);
+  const int nt = cache_tiles<TILE>(a, b) + (a.T + TILE - 1) / TILE;
+  const long long U = (long long)all * a.Hkv, s0 = (long long)before * a.Hkv + (long long)h * (nt + extra<TILE>()), s1 = s0 + nt;
+  const int N = a.nwg;
+  const int w0 = (int)(((s0 + 1) * N - 1) / U), w1 = (int)((s1 * N - 1) / U);
+  if (w0 == w1) return;
+  const int i0 = g * R;  // (R divides QB: the rows lie in one row group)
+  const int qb = i0 / a.QB, r0 = i0 - qb * a.QB;
+  if (wave == 0) {
+    // a worker's second part is the one that starts past its share's first
+    // tile; a worker whose share is empty has none
+    int n = 0;
+    for (int w = w0 + lane; w - lane <= w1; w += 64) {
+      long long from = 0;
+      bool has = w <= w1;
+      if (has) {
+        from = share_start(U, N, w);
+        has = from != share_start(U, N, w + 1);
+      }
+      const u64 m = __ballot(has);
+      if (has) s.part[n + lanes_below(m)] = ((qb * N + w) * 2 + (from < s0)) * a.QB + r0;
+      n += __popcll(m);
+    }
+    if (lane == 0) s.n = n;
+  }
+  __syncthreads();
+  const int n = s.n;
+  if constexpr (R == 1) {
+    join_one<DT>(a, s, b, h, i0, n);
+    return;
+  }
+  // Four rows a wave, 16 lanes each for the parts' maxima and sums.
+  const int y0 = lane >> 4, j0 = lane & 15, r = wave + 4 * y0;
+  float m = NEG;
+  for (int j = j0; j < n; j += 16) m = fmaxf(m, a.part_ml[2ll * (s.part[j] + r)]);
+  m = fmaxf(m, xor_lane<1>(m));
+  m = fmaxf(m, xor_lane<2>(m));
+  m = fmaxf(m, xor_lane<4>(m));
+  m = fmaxf(m, xor_lane<8>(m));
+  float l = 0.0f, o[4][4] = {};
+  for (int c = 0; c < n; c += 16) {
+    float f = 0.0f;
+    if (c + j0 < n) {
+      const long long p = s.part[c + j0] + r;
+      const float pm = a.part_ml[2 * p];
+      f = pm == NEG ? 0.0f : exp2_hw(pm - m);
+      l += f * a.part_ml[2 * p + 1];
+    }
+    const int cn = n - c < 16 ? n - c : 16;
+    for (int j = 0; j < cn; j += 2) {
+      float x[2][4][4];
+#pragma unroll
+      for (int k = 0; k < 2; k++)  // (past the last part: the last one's, not used)
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+          const long long at = (long long)(s.part[c + (j + k < cn ? j + k : j)] + wave + 4 * y) * a.D;
+#pragma unroll
+          for (int z = 0; z < 4; z++) x[k][y][z] = z * 64 + lane < a.D ? a.part_o[at + z * 64 + lane] : 0.0f;
+        }
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        if (j + k >= cn) break;
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+          const float fy = readlane_f32(f, 16 * y + j + k);
+#pragma unroll
+          for (int z = 0; z < 4; z++) o[y][z] += fy * x[k][y][z];
+        }
+      }
+    }
+  }
+  l += xor_lane<1>(l);
+  l += xor_lane<2>(l);
+  l += xor_lane<4>(l);
+  l += xor_lane<8>(l);
+#pragma unroll
+  for (int y = 0; y < 4; y++)
+    if (i0 + wave + 4 * y < a.M) write_row<DT>(a, b, h, i0 + wave + 4 * y, o[y], readlane_f32(m, 16 * y), readlane_f32(l, 16 * y));
+}
+
+// Few rows: one a workgroup, so that their parts are read by many.
+template <typename DT, int TILE>
+hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
+  if ((long long)a.B * a.Hkv * a.M <= 2048)
+    hipLaunchKernelGGL((join_kernel<DT, TILE, 1>), dim3(a.B * a.Hkv * a.M), dim3(JOIN_NT), 0, st, a, a.M);
+  else {
+    const int groups = (a.M + 15) / 16;
+    hipLaunchKernelGGL((join_kernel<DT, TILE, 16>), dim3(a.B * a.Hkv * groups), dim3(JOIN_NT), 0, st, a, groups);
+  }
+  return hipGetLastError();
 }
 
 }  // namespace attn
 
-hipError_t launch_attn_narrow(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st);
-hipError_t launch_attn_wide(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st);
+hipError_t launch_attn_narrow(const AttnArgs& a, int dtype, hipStream_t st);
+hipError_t launch_attn_wide(const AttnArgs& a, int dtype, hipStream_t st);
 hipError_t set_attn_narrow_lds(size_t bytes);
 
 }  // namespace tgs

@@ -77,31 +77,39 @@ struct Narrow {
     for (int d = 0; d < DT16; d++) v[d] = *(const Vec*)(base + d * 128);
   }
 
-  // The same of the drafted nodes from node t0 on.  Their values come row by
-  // row and turn into blocks of eight tokens in registers and through `turn`,
-  // the wave's own 4 D vectors of LDS.
-  __device__ __forceinline__ void load_tree(int t0, Vec* turn, Vec (&k)[2][KK], Vec (&v)[DT16]) const {
+  // The same of the drafted nodes (T <= NTILE: one tile).  Their values come
+  // row by row, 16 chunks a go, and turn into blocks of eight tokens in
+  // registers and through `turn`, the wave's own 4 D vectors of LDS.
+  static constexpr int GO = (D / 8 + 15) / 16;
+  static constexpr bool EARLY = false;
+  __device__ __forceinline__ void load_tree_values(Vec (&x)[GO][8]) const {
+    const uint16_t* vb = (const uint16_t*)a.v_new + b * a.vn_b + h * a.vn_h;
+#pragma unroll
+    for (int n = 0; n < GO; n++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int c = n * 16 + col, p = grp * 8 + j;
+        x[n][j] = vec16(0, 0, 0, 0);
+        if (p < a.T && c < D / 8) x[n][j] = load16(vb + p * a.vn_t + c * 8);
+      }
+  }
+  __device__ __forceinline__ void load_tree_keys(Vec (&k)[2][KK]) const {
     const uint16_t* kb = (const uint16_t*)a.k_new + b * a.kn_b + h * a.kn_h + grp * 8;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-      int p = t0 + (col >> 2) * 8 + (col & 3) + 4 * t;
+      int p = (col >> 2) * 8 + (col & 3) + 4 * t;
       p = p < a.T ? p : a.T - 1;
 #pragma unroll
       for (int kk = 0; kk < KK; kk++) k[t][kk] = load16(kb + p * a.kn_t + kk * 32);
     }
-    const uint16_t* vb = (const uint16_t*)a.v_new + b * a.vn_b + h * a.vn_h;
-#pragma unroll 1
-    for (int c = col; c < D / 8; c += 16) {
-      Vec x[8];
+  }
+  __device__ __forceinline__ void turn_tree(Vec* turn, Vec (&x)[GO][8], Vec (&v)[DT16]) const {
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int p = t0 + grp * 8 + j;
-        x[j] = vec16(0, 0, 0, 0);
-        if (p < a.T) x[j] = load16(vb + p * a.vn_t + c * 8);
-      }
-      transpose8(x);
+    for (int n = 0; n < GO; n++) {
+      transpose8(x[n]);
+      if (n * 16 + col < D / 8)
 #pragma unroll
-      for (int j = 0; j < 8; j++) turn[grp * D + c * 8 + j] = x[j];
+        for (int j = 0; j < 8; j++) turn[grp * D + (n * 16 + col) * 8 + j] = x[n][j];
     }
     wave_lds_sync();
 #pragma unroll
@@ -160,6 +168,7 @@ struct Narrow {
     nc = (len + NTILE - 1) / NTILE;
     table = a.tables + (long long)b * a.P;
     bad = false;
+    const int par = t1 > nc ? parent_of(a, b) : -1;
     Vec q[QT][KK];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
@@ -179,6 +188,7 @@ struct Narrow {
     }
     Vec k[2][KK], v[DT16], p[QT];
     f32x4 sc[QT][2];
+    Vec x[GO][8];
     int i = t0 + wave;
     const int tc = t1 < nc ? t1 : nc;  // the end of the cache's tiles
     if (i < tc) {
@@ -207,31 +217,36 @@ struct Narrow {
       scores(k, q, sc);
       const int left = len - i * NTILE - grp * 8;  // of the lane's eight tokens
       if ((i + 1) * NTILE > len) {
+        const uint32_t bits = left >= 8 ? 0xFFu : left <= 0 ? 0u : (1u << left) - 1;
 #pragma unroll
         for (int t = 0; t < QT; t++)
 #pragma unroll
-          for (int j = 0; j < 8; j++)
-            if (j >= left) sc[t][j >> 2][j & 3] = NEG;
+          for (int j = 0; j < 8; j++) sc[t][j >> 2][j & 3] = seen(sc[t][j >> 2][j & 3], bits, j);
         // what lies past the end is not 0 (it may be anything, NaN too)
+        const Vec keep = first_of(left);
 #pragma unroll
-        for (int d = 0; d < DT16; d++) v[d] = keep_first(v[d], left);
+        for (int d = 0; d < DT16; d++) v[d] &= keep;
       }
+      i += NW;
+      if (EARLY && i < t1) load_tree_values(x);  // (the keys' registers serve)
       weights(sc, st, p);
       add(v, p, st);
-      i += NW;
+    } else if (EARLY && i < t1) {
+      load_tree_values(x);
     }
-    for (; i < t1; i += NW) {
-      const u64 anc = ancestors(a, b);  // of node `lane`
-      load_tree((i - nc) * NTILE, (Vec*)s.o[wave], k, v);
+    if (i < t1) {
+      if (!EARLY) load_tree_values(x);
+      load_tree_keys(k);
+      const u64 anc = ancestors(a, par);  // of node `lane`
       scores(k, q, sc);
+      turn_tree((Vec*)s.o[wave], x, v);
 #pragma unroll
       for (int t = 0; t < QT; t++) {
         const int node = t * 16 + col < a.M ? (t * 16 + col) / a.G : 0;
         const u64 sees = ((u64)(uint32_t)__shfl((int)(anc >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)anc, node, 64);
-        const uint32_t in = (uint32_t)(sees >> ((i - nc) * NTILE + grp * 8));
+        const uint32_t in = (uint32_t)(sees >> (grp * 8));
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-          if (!((in >> j) & 1)) sc[t][j >> 2][j & 3] = NEG;
+        for (int j = 0; j < 8; j++) sc[t][j >> 2][j & 3] = seen(sc[t][j >> 2][j & 3], in, j);
       }
       weights(sc, st, p);
       add(v, p, st);
@@ -305,25 +320,22 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void narrow_kernel(AttnA
     n.segment(s, 0, cache_tiles<NTILE>(a, n.b) + tree, true, 0);
     return;
   }
-  int before, all, b;
-  tiles_before<NTILE>(a, 0, before, all);
-  const long long U = (long long)all * a.Hkv;
-  const long long u0 = share_start(U, a.nwg, blockIdx.x), u1 = share_start(U, a.nwg, blockIdx.x + 1);
-  if (u0 == u1) return;
-  long long skip;
-  find_tile<NTILE>(a, u0, a.Hkv, b, skip);
-  int nt = cache_tiles<NTILE>(a, b) + tree;
-  int h = (int)((u0 - skip) / nt), at = (int)((u0 - skip) - (long long)h * nt);
+  const Place at0 = find_place<NTILE>(a, blockIdx.x);
+  const long long u0 = at0.u0, u1 = at0.u1;
+  int b = at0.b, h = at0.h, at = at0.at, nt = at0.nt;
   for (long long u = u0; u < u1;) {
     const int end = nt - at < u1 - u ? nt : at + (int)(u1 - u);
-    n.b = b;
-    n.h = h;
-    n.segment(s, at, end, at == 0 && end == nt, ((long long)blockIdx.x * 2 + (u != u0)) * a.QB);
+    const int real = nt - extra<NTILE>();
+    if (at < real) {
+      n.b = b;
+      n.h = h;
+      n.segment(s, at, end < real ? end : real, at == 0 && end >= real, ((long long)blockIdx.x * 2 + (u != u0)) * a.QB);
+    }
     u += end - at;
     at = 0;
     if (++h == a.Hkv) {
       h = 0;
-      if (++b < a.B) nt = cache_tiles<NTILE>(a, b) + tree;
+      if (++b < a.B) nt = cache_tiles<NTILE>(a, b) + tree + extra<NTILE>();
     }
   }
 }
@@ -336,9 +348,7 @@ hipError_t narrow_run(const AttnArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((narrow_kernel<DT, D, QT, NW>), dim3(grid), dim3(NW * 64), sizeof(typename K::Shared), st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.nwg == 0) return e;
-  const long long rows = (long long)a.B * a.Hkv * a.M;
-  hipLaunchKernelGGL((join_kernel<DT, NTILE>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
-  return hipGetLastError();
+  return launch_join<DT, NTILE>(a, st);
 }
 template <typename DT, int D, int QT>
 hipError_t narrow_lds() {
@@ -378,8 +388,8 @@ hipError_t narrow_lds_type() {
 
 }  // namespace attn
 
-hipError_t launch_attn_narrow(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st) {
-  return dtype == TGS_BF16 ? attn::narrow_type<attn::BF16>(a, p.qw, st) : attn::narrow_type<attn::F16>(a, p.qw, st);
+hipError_t launch_attn_narrow(const AttnArgs& a, int dtype, hipStream_t st) {
+  return dtype == TGS_BF16 ? attn::narrow_type<attn::BF16>(a, a.QB / 16, st) : attn::narrow_type<attn::F16>(a, a.QB / 16, st);
 }
 hipError_t set_attn_narrow_lds(size_t) {
   const hipError_t e = attn::narrow_lds_type<attn::BF16>(), f = attn::narrow_lds_type<attn::F16>();

@@ -19,7 +19,7 @@ struct Wide {
   static constexpr int NTHR = QW * 64, KK = D / 16, DT32 = D / 32, C = D / 8;
   static constexpr int NCH = (WTILE * C + NTHR - 1) / NTHR;  // chunks a thread moves, of keys and of values
   static constexpr bool EVEN = WTILE * C % NTHR == 0;
-  static constexpr int AHEAD = NCH <= 4 ? 2 : 1;  // tiles on their way (a tile takes 8 NCH registers)
+  static constexpr int AHEAD = NCH <= 2 ? 2 : 1;  // tiles on their way (a tile takes 8 NCH registers)
   struct Shared {
     Vec k[2][WTILE * C];
     Vec v[2][WTILE * C];
@@ -91,28 +91,56 @@ struct Wide {
 
   // To buffer f; what lies past the sequence's end is not 0 there (it may be
   // anything, NaN too), and is 0 here.
-  __device__ __forceinline__ void store(Shared& s, int f, int i, const Vec (&k)[NCH], const Vec (&v)[NCH]) {
-    const bool tail = (i + 1) * WTILE > len;
+  __device__ __forceinline__ void store(Shared& s, int f, int i, const Vec (&k)[NCH], Vec (&v)[NCH]) {
+    if ((i + 1) * WTILE > len) {
+#pragma unroll
+      for (int n = 0; n < NCH; n++) v[n] &= first_of(len - i * WTILE - block_of<D>(n) * 8);
+    }
 #pragma unroll
     for (int n = 0; n < NCH; n++) {
       const int c = n * NTHR + tid;
       if (EVEN || c < WTILE * C) {
         s.k[f][at_key(c / C, c % C)] = k[n];
-        s.v[f][c] = tail ? keep_first(v[n], len - i * WTILE - c / D * 8) : v[n];
+        s.v[f][c] = v[n];
       }
     }
   }
 
-  // The drafted nodes' tile, from their own rows.
-  __device__ __forceinline__ void store_tree(Shared& s, int t0) {
+  // The drafted nodes' tile, from their own rows, to buffer 1 (T <= WTILE: one
+  // tile).  Values come row by row and turn into blocks of eight tokens.
+  static constexpr int TURN = (8 * C + NTHR - 1) / NTHR;  // (block, chunk)s a thread turns
+  __device__ __forceinline__ void load_tree(Vec (&k)[NCH], Vec (&v)[TURN][8]) const {
     const uint16_t* kb = (const uint16_t*)a.k_new + b * a.kn_b + h * a.kn_h;
     const uint16_t* vb = (const uint16_t*)a.v_new + b * a.vn_b + h * a.vn_h;
-#pragma unroll 1
-    for (int c = tid; c < WTILE * C; c += NTHR) {
-      const int tok = c / C, ch = c - tok * C, p = t0 + tok < a.T ? t0 + tok : a.T - 1;
-      s.k[0][at_key(tok, ch)] = load16(kb + p * a.kn_t + ch * 8);
-      const int blk = c / D, d = c - blk * D;
-      s.v[0][c] = tree_values(vb + d, a.vn_t, t0 + blk * 8, a.T);
+#pragma unroll
+    for (int n = 0; n < NCH; n++) {
+      const int c = chunk(n), p = c / C;
+      k[n] = load16(kb + (p < a.T ? p : a.T - 1) * a.kn_t + c % C * 8);
+    }
+#pragma unroll
+    for (int n = 0; n < TURN; n++) {
+      const int c = n * NTHR + tid;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int p = c / C * 8 + j;
+        v[n][j] = vec16(0, 0, 0, 0);
+        if (c < 8 * C && p < a.T) v[n][j] = load16(vb + p * a.vn_t + c % C * 8);
+      }
+    }
+  }
+  __device__ __forceinline__ void store_tree(Shared& s, const Vec (&k)[NCH], Vec (&v)[TURN][8]) const {
+#pragma unroll
+    for (int n = 0; n < NCH; n++) {
+      const int c = n * NTHR + tid;
+      if (EVEN || c < WTILE * C) s.k[1][at_key(c / C, c % C)] = k[n];
+    }
+#pragma unroll
+    for (int n = 0; n < TURN; n++) {
+      const int c = n * NTHR + tid;
+      transpose8(v[n]);
+      if (c < 8 * C)
+#pragma unroll
+        for (int j = 0; j < 8; j++) s.v[1][c / C * D + c % C * 8 + j] = v[n][j];
     }
   }
 
@@ -129,10 +157,26 @@ struct Wide {
     for (int x = 0; x < 2; x++)
 #pragma unroll
       for (int j = 0; j < 16; j++) sc[x][j] = 0.0f;
+    // four operands ahead of the products
+    constexpr int N = 2 * KK;
+    Vec x[4];
 #pragma unroll
-    for (int kk = 0; kk < KK; kk++)
+    for (int j = 0; j < 4; j++) x[j] = s.k[f][at_key(j % 2 * 32 + tok, j / 2 * 2 + half)];
 #pragma unroll
-      for (int x = 0; x < 2; x++) sc[x] = mfma32<DT>(s.k[f][at_key(x * 32 + tok, kk * 2 + half)], q[kk], sc[x]);
+    for (int j = 0; j < N; j++) {
+      sched_fence();
+      sc[j % 2] = mfma32<DT>(x[j % 4], q[j / 2], sc[j % 2]);
+      if (j + 4 < N) x[j % 4] = s.k[f][at_key(j % 2 * 32 + tok, (j + 4) / 2 * 2 + half)];
+    }
+    sched_fence();
+  }
+
+  // Scores of tokens whose bit (16 x + j) is clear become -inf.
+  static __device__ __forceinline__ void mask(f32x16 (&sc)[2], uint32_t bits) {
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) sc[x][j] = seen(sc[x][j], bits, 16 * x + j);
   }
 
   __device__ __forceinline__ void add(const Shared& s, int f, const f32x16 (&sc)[2], State& st) const {
@@ -152,18 +196,34 @@ struct Wide {
       for (int d = 0; d < DT32; d++) st.o[d] *= g;
     }
     const float base = st.m == NEG ? 0.0f : st.m;
+    // Two neighbouring tokens' weights: word i of the 16 tokens 16 y ...
+    auto word = [&](int y, int i) {
+      const float u = exp2_hw(__builtin_fmaf(sc[y >> 1][(y & 1) * 8 + 2 * i], a.scale_log2, -base));
+      const float w = exp2_hw(__builtin_fmaf(sc[y >> 1][(y & 1) * 8 + 2 * i + 1], a.scale_log2, -base));
+      st.l += u + w;
+      return pack2<DT>(u, w);
+    };
+    // each product runs beside the weights and the operand of the next 16 tokens'
+    Vec x[DT32];
 #pragma unroll
-    for (int y = 0; y < 4; y++) {  // the 16 tokens 16 y .. of the tile
-      float w[8];
+    for (int d = 0; d < DT32; d++) x[d] = s.v[f][half * D + d * 32 + col];
+    Vec p = vec16(word(0, 0), word(0, 1), word(0, 2), word(0, 3));
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        w[j] = exp2_hw(__builtin_fmaf(sc[y >> 1][(y & 1) * 8 + j], a.scale_log2, -base));
-        st.l += w[j];
+    for (int y = 0; y < 4; y++) {
+      Vec next = p;
+#pragma unroll
+      for (int d = 0; d < DT32; d++) {
+        sched_fence();
+        st.o[d] = mfma32<DT>(x[d], p, st.o[d]);
+        if (y < 3) {
+          x[d] = s.v[f][((y + 1) * 2 + half) * D + d * 32 + col];
+#pragma unroll
+          for (int i = d * 4 / DT32; i < (d + 1) * 4 / DT32; i++) next[i] = word(y + 1, i);
+        }
       }
-      const Vec p = vec16(pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7]));
-#pragma unroll
-      for (int d = 0; d < DT32; d++) st.o[d] = mfma32<DT>(s.v[f][(y * 2 + half) * D + d * 32 + col], p, st.o[d]);
+      p = next;
     }
+    sched_fence();
   }
 
   __device__ __forceinline__ void segment(Shared& s, int t0, int t1, bool full, long long part) {
@@ -175,6 +235,18 @@ struct Wide {
     const bool work = row0 < a.M;
     const int i = row0 + col;
     const int node = i < a.M ? i / a.G : 0, hg = i < a.M ? i - node * a.G : 0;
+    // Requests first: page entries, queries, the drafted nodes' tile (a worker
+    // that has it starts with it), the first tile.
+    const int tc = t1 < nc ? t1 : nc;  // the end of the cache's tiles
+    auto cut = [&](int t) { return t < tc ? t : tc - 1; };
+    const bool cached = t0 < tc, drafted = t1 > nc;
+    int e = 0, next = 0;
+    if (cached) {
+      e = entries(t0);
+      next = entries(cut(t0 + 1));
+    }
+    int par = -1;
+    if (drafted) par = parent_of(a, b);
     Vec q[KK];
     {
       const uint16_t* p = (const uint16_t*)a.q + b * a.q_b + node * a.q_t + (long long)(h * a.G + hg) * a.q_h + half * 8;
@@ -189,17 +261,23 @@ struct Wide {
 #pragma unroll
       for (int x = 0; x < 16; x++) st.o[d][x] = 0.0f;
     f32x16 sc[2];
-    const int tc = t1 < nc ? t1 : nc;  // the end of the cache's tiles
-    lds_barrier();                     // (the buffers are free)
-    if (t0 < tc) {
+    Vec k0[NCH], v0[NCH], k1[NCH], v1[NCH];
+    if (drafted) {
+      Vec kt[NCH], vt[TURN][8];
+      load_tree(kt, vt);
+      if (cached) load(t0, e, k0, v0);
+      sched_fence();
+      lds_barrier();  // (the buffers are free)
+      store_tree(s, kt, vt);
+    } else {
+      load(t0, e, k0, v0);
+      sched_fence();
+      lds_barrier();
+    }
+    if (cached) {
       // Tile t is worked on in one buffer while t + 1 goes to the other and
       // the next AHEAD ones are on their way to registers; requests past the
       // last tile ask for it again, so that the number in flight is known.
-      auto cut = [&](int t) { return t < tc ? t : tc - 1; };
-      Vec k0[NCH], v0[NCH], k1[NCH], v1[NCH];
-      int e = entries(t0), next = entries(cut(t0 + 1));
-      load(t0, e, k0, v0);
-      sched_fence();
       store(s, 0, t0, k0, v0);
       e = next;
       next = entries(cut(t0 + 2));
@@ -213,7 +291,23 @@ struct Wide {
         load(cut(t0 + 2), e, k1, v1);
         sched_fence();
       }
+    }
+    lds_barrier();
+    if (drafted) {
+      if (work) {
+        u64 sees = ancestors(a, par);
+        sees = ((u64)(uint32_t)__shfl((int)(sees >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)sees, node, 64);
+        scores(s, 1, q, sc);
+        const u64 in = sees >> (8 * half);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int y = 0; y < 4; y++) bits |= ((uint32_t)(in >> (16 * y)) & 0xFFu) << (8 * y);
+        mask(sc, bits);
+        add(s, 1, sc, st);
+      }
       lds_barrier();
+    }
+    if (cached) {
       auto step = [&](int t, int f, Vec (&ks)[NCH], Vec (&vs)[NCH]) {
         store(s, f ^ 1, cut(t + 1), ks, vs);
         e = next;
@@ -225,41 +319,27 @@ struct Wide {
           scores(s, f, q, sc);
           if ((t + 1) * WTILE > len) {
             const int left = len - t * WTILE - 8 * half;
+            uint32_t bits = 0;
 #pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-              for (int j = 0; j < 16; j++)
-                if (32 * x + 16 * (j >> 3) + (j & 7) >= left) sc[x][j] = NEG;
+            for (int y = 0; y < 4; y++) {
+              const int n = left - 16 * y;
+              bits |= (n >= 8 ? 0xFFu : n <= 0 ? 0u : (1u << n) - 1) << (8 * y);
+            }
+            mask(sc, bits);
           }
           add(s, f, sc, st);
         }
         lds_barrier();
       };
-      for (int t = t0;;) {
+      int t = t0;
+      for (; t + 1 < tc; t += 2) {  // (an exit between the two would merge their requests' order)
         step(t, 0, k0, v0);
-        if (++t == tc) break;
         if constexpr (AHEAD == 2)
-          step(t, 1, k1, v1);
+          step(t + 1, 1, k1, v1);
         else
-          step(t, 1, k0, v0);
-        if (++t == tc) break;
+          step(t + 1, 1, k0, v0);
       }
-    }
-    if (t1 > nc) {
-      store_tree(s, 0);
-      u64 sees = ancestors(a, b);
-      sees = ((u64)(uint32_t)__shfl((int)(sees >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)sees, node, 64);
-      lds_barrier();
-      if (work) {
-        scores(s, 0, q, sc);
-        const u64 in = sees >> (8 * half);
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-#pragma unroll
-          for (int j = 0; j < 16; j++)
-            if (!((in >> (32 * x + 16 * (j >> 3) + (j & 7))) & 1)) sc[x][j] = NEG;
-        add(s, 0, sc, st);
-      }
+      if (t < tc) step(t, 0, k0, v0);
     }
     float m = st.m, l = st.l;
     const f32x16(&o)[DT32] = st.o;
@@ -313,25 +393,22 @@ __global__ __launch_bounds__(QW * 64, D == 256 ? 1 : 2) void wide_kernel(AttnArg
   const int x = blockIdx.x;
   const int w = a.nwg % 8 == 0 ? x / (8 * a.nqb) * 8 + x % 8 : x / a.nqb;
   n.qb = a.nwg % 8 == 0 ? x / 8 % a.nqb : x % a.nqb;
-  int before, all, b;
-  tiles_before<WTILE>(a, 0, before, all);
-  const long long U = (long long)all * a.Hkv;
-  const long long u0 = share_start(U, a.nwg, w), u1 = share_start(U, a.nwg, w + 1);
-  if (u0 == u1) return;
-  long long skip;
-  find_tile<WTILE>(a, u0, a.Hkv, b, skip);
-  int nt = cache_tiles<WTILE>(a, b) + tree;
-  int h = (int)((u0 - skip) / nt), at = (int)((u0 - skip) - (long long)h * nt);
+  const Place at0 = find_place<WTILE>(a, w);
+  const long long u0 = at0.u0, u1 = at0.u1;
+  int b = at0.b, h = at0.h, at = at0.at, nt = at0.nt;
   for (long long u = u0; u < u1;) {
     const int end = nt - at < u1 - u ? nt : at + (int)(u1 - u);
-    n.b = b;
-    n.h = h;
-    n.segment(s, at, end, at == 0 && end == nt, ((long long)(n.qb * a.nwg + w) * 2 + (u != u0)) * a.QB);
+    const int real = nt - extra<WTILE>();
+    if (at < real) {
+      n.b = b;
+      n.h = h;
+      n.segment(s, at, end < real ? end : real, at == 0 && end >= real, ((long long)(n.qb * a.nwg + w) * 2 + (u != u0)) * a.QB);
+    }
     u += end - at;
     at = 0;
     if (++h == a.Hkv) {
       h = 0;
-      if (++b < a.B) nt = cache_tiles<WTILE>(a, b) + tree;
+      if (++b < a.B) nt = cache_tiles<WTILE>(a, b) + tree + extra<WTILE>();
     }
   }
 }
@@ -343,9 +420,7 @@ hipError_t wide_run(const AttnArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((wide_kernel<DT, D, QW>), dim3(grid), dim3(QW * 64), sizeof(typename K::Shared), st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.nwg == 0) return e;
-  const long long rows = (long long)a.B * a.Hkv * a.M;
-  hipLaunchKernelGGL((join_kernel<DT, WTILE>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
-  return hipGetLastError();
+  return launch_join<DT, WTILE>(a, st);
 }
 
 template <typename DT, int D>
@@ -391,25 +466,23 @@ hipError_t wide_type(const AttnArgs& a, int qw, hipStream_t st) {
 
 }  // namespace attn
 
-hipError_t launch_attn_wide(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st) {
-  return dtype == TGS_BF16 ? attn::wide_type<attn::BF16>(a, p.qw, st) : attn::wide_type<attn::F16>(a, p.qw, st);
+hipError_t launch_attn_wide(const AttnArgs& a, int dtype, hipStream_t st) {
+  return dtype == TGS_BF16 ? attn::wide_type<attn::BF16>(a, a.QB / 32, st) : attn::wide_type<attn::F16>(a, a.QB / 32, st);
 }
 
 AttnPlan attn_plan(int M, int D) {
   AttnPlan p;
   if (M <= 32) {
     p.wide = 0;
-    p.qw = M <= 16 ? 1 : 2;
     p.tile = attn::NTILE;
-    p.QB = 16 * p.qw;
+    p.QB = M <= 16 ? 16 : 32;
     p.per_cu = D == 256 ? 1 : 2;
     p.least = 4;  // one per wave
   } else {
     p.wide = 1;
-    p.qw = D == 256 ? 4 : M <= 64 ? 2 : M <= 128 ? 4 : 8;
     p.tile = attn::WTILE;
-    p.QB = 32 * p.qw;
-    p.per_cu = D == 256 || p.qw == 8 ? 1 : 2;
+    p.QB = D == 256 ? 128 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    p.per_cu = D == 256 || p.QB == 256 ? 1 : 2;
     p.least = 4;
   }
   p.nqb = (M + p.QB - 1) / p.QB;
@@ -417,7 +490,7 @@ AttnPlan attn_plan(int M, int D) {
 }
 
 hipError_t launch_attn(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st) {
-  return p.wide ? launch_attn_wide(a, p, dtype, st) : launch_attn_narrow(a, p, dtype, st);
+  return p.wide ? launch_attn_wide(a, dtype, st) : launch_attn_narrow(a, dtype, st);
 }
 
 hipError_t set_attn_lds_limit(size_t bytes) {

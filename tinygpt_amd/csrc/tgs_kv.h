@@ -107,7 +107,6 @@ struct AttnArgs {
 };
 struct AttnPlan {
   int wide;   // 0: a wave owns its tiles; 1: tiles shared through LDS
-  int qw;     // wide: waves over query rows; narrow: 16-row query tiles per wave
   int tile;   // tokens of a unit of work
   int QB, nqb;
   int per_cu;  // workgroups that a CU holds
