@@ -2,13 +2,16 @@
 // each, the n largest of score[w] + x[w][v] - logsumexp(x[w]), and the
 // histories that go with them.
 //
-// One read of the logits bounds it.  chunk_kernel holds a chunk of a row in
-// registers: thread maxima give a bound that at most a few more than n ids
-// pass (the n-th largest of the maxima), these are collected and sorted, and
-// the chunk's maximum and sum of exponentials come from the same registers.
-// Inside a row the order is the logits' own, so it needs no arithmetic; join_kernel
-// then orders the candidates of different beams by totals held in 64 bits,
-// since those of different beams may lie closer than 32 bits tell apart.
+// One read of the logits bounds it, and the operations on every element next
+// to that.  chunk_kernel holds a chunk of a row in registers: thread maxima give
+// a bound that a few more than n ids pass (the n-th largest of the maxima),
+// vectors whose maximum passes it are searched, and what is found is sorted.
+// The sum of exponentials comes from the same registers, each thread's terms
+// relative to a power of two of its own, so that no thread waits for the
+// chunk's maximum and joining the sums is exact.  Inside a row the order is the
+// logits' own, so it needs no arithmetic; join_kernel orders the candidates of
+// different beams by totals held in 64 bits, since those of different beams
+// may lie closer than 32 bits tell apart.
 #include "tgs_device.h"
 #include "tgs_kv.h"
 #include "tgs_row.h"
@@ -31,19 +34,36 @@ struct ChunkShared {
   uint32_t top[BEAM_NT / 64][64];
   u64 cand[BEAM_CAP];
   double sum[BEAM_NT / 64];
+  float base[BEAM_NT / 64];
   unsigned n;
 };
 
+// The vector as a new value to the compiler, in program order: a pass over the
+// chunk unpacks it again instead of keeping every id's 32 bits from the pass
+// before (which spilled hundreds of registers).
+__device__ __forceinline__ uint4 again(uint4 x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w));
+#endif
+  return x;
+}
+
+constexpr float NEG = -__builtin_inff();
+constexpr float NO_BASE = -1e30f;  // (the exponent of a sum of nothing)
+
+// x 2^e for a whole e <= 0; 0 far below.
+__device__ __forceinline__ double scaled(double x, float e) { return __builtin_ldexp(x, (int)fmaxf(e, -4000.0f)); }
+
 // Workgroup (row, chunk): ids [c L, min(V, (c + 1) L)), NVT vectors a thread.
 template <typename Tin, int NVT>
-__global__ __launch_bounds__(BEAM_NT) void chunk_kernel(BeamArgs a) {
+__global__ __launch_bounds__(BEAM_NT, 4) void chunk_kernel(BeamArgs a) {
   constexpr int EPV = Elem<Tin>::EPV;
   TGS_STATIC_SMEM(ChunkShared, s);
   const int row = blockIdx.x / a.S, c = blockIdx.x % a.S, tid = threadIdx.x, w = tid >> 6;
   const Tin* rowp = (const Tin*)a.logits + (long long)row * a.row_stride;
   const int v0 = c * a.L, v1 = v0 + a.L < a.V ? v0 + a.L : a.V;
   const int nvec = (v1 - v0) / EPV, tail0 = v0 + nvec * EPV;
-  constexpr uint32_t NB = Elem<Tin>::NAN_BITS;
+  constexpr uint32_t NB = sizeof(Tin) == 2 ? 0xFF80FF80u : 0xFF800000u;  // -inf
   uint4 raw[NVT];
 #pragma unroll
   for (int j = 0; j < NVT; j++) {
@@ -52,60 +72,83 @@ __global__ __launch_bounds__(BEAM_NT) void chunk_kernel(BeamArgs a) {
     if (i < nvec) raw[j] = load_row16<true>(rowp + v0 + i * EPV);
   }
   // the last ids of a row that is not whole vectors, one a thread
-  const float xt = tid < v1 - tail0 ? Elem<Tin>::scalar(rowp, tail0 + tid) : -__builtin_inff();
+  const float xt = tid < v1 - tail0 ? Elem<Tin>::scalar(rowp, tail0 + tid) : NEG;
   if (tid == 0) s.n = 0;
-  float tm = fmaxf(xt, -__builtin_inff());  // (of a NaN and a number the number)
-#pragma unroll
-  for (int j = 0; j < NVT; j++)
-#pragma unroll
-    for (int e = 0; e < EPV; e++) tm = fmaxf(tm, Elem<Tin>::get(raw[j], e));
-  uint32_t top = wave_sort_desc(tg_key(tm));
-  s.top[w][lane_id()] = top;
-  __syncthreads();
-  top = s.top[0][lane_id()];
-#pragma unroll
-  for (int i = 1; i < BEAM_NT / 64; i++) top = wave_merge_top64(top, s.top[i][lane_id()]);
-  const float m = tg_unkey(readlane_u32(top, 0)), bound = tg_unkey(readlane_u32(top, a.n - 1));
-  // candidates and the sum; exp(x - m) as 2^(d log2 e) with the constant in two parts
-  constexpr float L2H = 0x1.715476p+0f, L2L = 0x1.4ae0cp-26f;
-  double sum = 0.0;
-  auto each = [&](auto f) {
-#pragma unroll
-    for (int j = 0; j < NVT; j++)
-#pragma unroll
-      for (int e = 0; e < EPV; e++)
-        f(Elem<Tin>::get(raw[j], e), v0 + (j * BEAM_NT + tid) * EPV + e);
-    f(xt, tail0 + tid);
-  };
-  each([&](float x, int v) {
-    if (x >= bound && x > -__builtin_inff()) {
-      const unsigned at = atomicAdd(&s.n, 1u);
-      if (at < (unsigned)BEAM_CAP) s.cand[at] = comp_key(tg_key(x), v);
-    }
-  });
-  auto term = [&](float x) {
-    const float d = x - m;
-    const float e = exp2_hw(__builtin_fmaf(d, L2H, d * L2L));
-    return x > -__builtin_inff() ? e : 0.0f;
-  };
+  float tm = fmaxf(xt, NEG), vm[NVT];  // (of a NaN and a number the number)
 #pragma unroll
   for (int j = 0; j < NVT; j++) {
+    vm[j] = NEG;
+#pragma unroll
+    for (int e = 0; e < EPV; e++) vm[j] = fmaxf(vm[j], Elem<Tin>::get(raw[j], e));
+    tm = fmaxf(tm, vm[j]);
+  }
+  const uint32_t mine = wave_sort_desc(tg_key(tm));
+  s.top[w][lane_id()] = mine;
+  // Terms 2^(x log2 e - base), the constant in two parts, base the whole
+  // number at the thread's maximum.
+  constexpr float L2H = 0x1.715476p+0f, L2L = 0x1.4ae0cp-26f;
+  const bool some = tm > NEG && tm < -NEG;
+  float base = some ? __builtin_rintf(tm * L2H) : 0.0f;
+  auto term = [&](float x) { return exp2_hw(__builtin_fmaf(x, L2L, __builtin_fmaf(x, L2H, -base))); };
+  double sum = (double)term(xt);
+#pragma unroll
+  for (int j = 0; j < NVT; j++) {
+    raw[j] = again(raw[j]);
     float part = 0.0f;  // (of one vector's terms)
 #pragma unroll
     for (int e = 0; e < EPV; e++) part += term(Elem<Tin>::get(raw[j], e));
     sum += (double)part;
   }
-  sum += (double)term(xt);
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < NVT; j++) {
+      raw[j] = again(raw[j]);
+#pragma unroll
+      for (int e = 0; e < EPV; e++) f(Elem<Tin>::get(raw[j], e), v0 + (j * BEAM_NT + tid) * EPV + e);
+    }
+    f(xt, tail0 + tid);
+  };
+  if (sum != sum) {  // NaN logits count as -inf (+inf ones leave an infinite sum)
+    sum = 0.0;
+    each([&](float x, int) { sum += x > NEG ? (double)term(x) : 0.0; });
+  }
+  if (sum == 0.0) base = NO_BASE;
+  const float wbase = wave_maxf(base);
+  sum = scaled(sum, base - wbase);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  if (lane_id() == 0) s.sum[w] = sum;
+  if (lane_id() == 0) {
+    s.base[w] = wbase;
+    s.sum[w] = sum;
+  }
+  __syncthreads();
+  uint32_t top = s.top[0][lane_id()];
+#pragma unroll
+  for (int i = 1; i < BEAM_NT / 64; i++) top = wave_merge_top64(top, s.top[i][lane_id()]);
+  const float bound = tg_unkey(readlane_u32(top, a.n - 1));
+  auto keep = [&](float x, int v) {
+    if (x >= bound && x > NEG) {
+      const unsigned at = atomicAdd(&s.n, 1u);
+      if (at < (unsigned)BEAM_CAP) s.cand[at] = comp_key(tg_key(x), v);
+    }
+  };
+  if (tm >= bound) {
+#pragma unroll
+    for (int j = 0; j < NVT; j++)
+      if (vm[j] >= bound) {
+        raw[j] = again(raw[j]);
+#pragma unroll
+        for (int e = 0; e < EPV; e++) keep(Elem<Tin>::get(raw[j], e), v0 + (j * BEAM_NT + tid) * EPV + e);
+      }
+    keep(xt, tail0 + tid);
+  }
   __syncthreads();
   unsigned n = s.n;
   if (n > (unsigned)BEAM_CAP) {  // many equal logits: the exact n-th by its composite
     const u64 least = block_select_kth<u64, 64, BEAM_NT>(
         [&](auto f) {
           each([&](float x, int v) {
-            if (x > -__builtin_inff()) f(comp_key(tg_key(x), v));
+            if (x > NEG) f(comp_key(tg_key(x), v));
           });
         },
         (unsigned)a.n, s.bs);
@@ -113,7 +156,7 @@ __global__ __launch_bounds__(BEAM_NT) void chunk_kernel(BeamArgs a) {
     if (tid == 0) s.n = 0;
     __syncthreads();
     each([&](float x, int v) {
-      if (x > -__builtin_inff() && comp_key(tg_key(x), v) >= least) {
+      if (x > NEG && comp_key(tg_key(x), v) >= least) {
         const unsigned at = atomicAdd(&s.n, 1u);
         if (at < (unsigned)BEAM_CAP) s.cand[at] = comp_key(tg_key(x), v);
       }
@@ -128,10 +171,13 @@ __global__ __launch_bounds__(BEAM_NT) void chunk_kernel(BeamArgs a) {
       best = wave_merge_top64(best, wave_sort_desc(i + lane < n ? s.cand[i + lane] : 0ull));
     if (lane < a.n) a.lists[(long long)blockIdx.x * a.n + lane] = best;
     if (lane == 0) {
+      float b = s.base[0];
+#pragma unroll
+      for (int i = 1; i < BEAM_NT / 64; i++) b = fmaxf(b, s.base[i]);
       double t = 0.0;
 #pragma unroll
-      for (int i = 0; i < BEAM_NT / 64; i++) t += s.sum[i];
-      a.sums[2 * (long long)blockIdx.x] = (double)m;
+      for (int i = 0; i < BEAM_NT / 64; i++) t += scaled(s.sum[i], s.base[i] - b);
+      a.sums[2 * (long long)blockIdx.x] = (double)b;
       a.sums[2 * (long long)blockIdx.x + 1] = t;
     }
   }
@@ -147,29 +193,31 @@ struct JoinShared {
 // Workgroup per request.  A wave per beam joins its chunks; a candidate's
 // place among all is its place in its own sorted list plus, by bisection, the
 // number of candidates ahead of it in every other.
-__global__ __launch_bounds__(BEAM_NT) void join_kernel(BeamArgs a) {
+constexpr int JOIN_NT = 512;
+__global__ __launch_bounds__(JOIN_NT) void join_kernel(BeamArgs a) {
   TGS_STATIC_SMEM(JoinShared, s);
   const int g = blockIdx.x, tid = threadIdx.x, lane = lane_id();
   const int W = a.W, n = a.n;
   const double NINF = -__builtin_inf();
-  for (int w = tid >> 6; w < W; w += BEAM_NT / 64) {
+  for (int w = tid >> 6; w < W; w += JOIN_NT / 64) {
     const long long row = (long long)g * W + w;
     const u64* lists = a.lists + row * a.S * n;
     const double* sums = a.sums + row * a.S * 2;
-    double m = lane < a.S ? sums[2 * lane] : NINF, t = lane < a.S ? sums[2 * lane + 1] : 0.0;
-    u64 best = lane < n ? lists[lane] : 0ull;
-    for (int i = 1; i < a.S; i++) best = wave_merge_top64(best, lane < n ? lists[i * n + lane] : 0ull);
-    double top = m;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const double y = __shfl_xor(top, o, 64);
-      top = y > top ? y : top;
+    const float score = a.scores[row];
+    const float m = lane < a.S ? (float)sums[2 * lane] : NO_BASE;
+    double t = lane < a.S ? sums[2 * lane + 1] : 0.0;
+    const int per = 64 / n, li = lane / n;  // lists a batch; the lane's list and entry
+    u64 best = 0ull;
+    for (int i = 0; i < a.S; i += per) {
+      u64 x = li < per && i + li < a.S ? lists[(i + li) * n + lane - li * n] : 0ull;
+      if (per > 1) x = wave_sort_desc(x);
+      best = i == 0 ? x : wave_merge_top64(best, x);
     }
-    t = m == top ? t : t * exp(m - top);
+    const float top = wave_maxf(m);
+    t = scaled(t, m - top);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
-    const double lse = top + log(t);
-    const float score = a.scores[row];
+    const double lse = (double)top * 0.69314718055994530942 + log(t);
     // a beam that has ended (its score not a number above -inf), or whose row
     // holds +inf or nothing, has no candidates
     const bool live = __builtin_isfinite(score) && __builtin_isfinite(lse);
@@ -179,13 +227,13 @@ __global__ __launch_bounds__(BEAM_NT) void join_kernel(BeamArgs a) {
       s.id[w][lane] = has ? comp_id(best) : -1;
     }
   }
-  for (int i = tid; i < n; i += BEAM_NT) {
+  for (int i = tid; i < n; i += JOIN_NT) {
     s.best[i] = NINF;
     s.parent[i] = -1;
     s.token[i] = -1;
   }
   __syncthreads();
-  for (int i = tid; i < W * n; i += BEAM_NT) {
+  for (int i = tid; i < W * n; i += JOIN_NT) {
     const int w = i / n, j = i - w * n;
     const double x = s.total[w][j];
     if (x == NINF) continue;
@@ -211,13 +259,13 @@ __global__ __launch_bounds__(BEAM_NT) void join_kernel(BeamArgs a) {
   }
   __syncthreads();
   const long long out = (long long)g * n;
-  for (int i = tid; i < n; i += BEAM_NT) {
+  for (int i = tid; i < n; i += JOIN_NT) {
     a.out_scores[out + i] = (float)s.best[i];
     a.out_parents[out + i] = s.parent[i];
     a.out_tokens[out + i] = s.token[i];
   }
   if (a.H == 0) return;
-  for (int r = tid >> 6; r < n; r += BEAM_NT / 64) {
+  for (int r = tid >> 6; r < n; r += JOIN_NT / 64) {
     const int p = s.parent[r], H = a.H;
     int have = p < 0 ? 0 : a.hist_len[p];
     have = have < 0 ? 0 : have > H ? H : have;
@@ -239,7 +287,7 @@ hipError_t launch_t(const BeamArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((chunk_kernel<Tin, BEAM_NVT>), grid, dim3(BEAM_NT), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(join_kernel, dim3(a.G), dim3(BEAM_NT), 0, st, a);
+  hipLaunchKernelGGL(join_kernel, dim3(a.G), dim3(JOIN_NT), 0, st, a);
   return hipGetLastError();
 }
 

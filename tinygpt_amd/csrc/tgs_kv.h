@@ -61,7 +61,7 @@ hipError_t set_kv_fork_lds_limit(size_t bytes);
 // Selection over beams and vocabulary.
 constexpr int BEAM_NT = 256;
 constexpr int BEAM_MAX = 64;  // beams of a request, and entries selected from it, at most
-constexpr int BEAM_NVT = 16;  // 16-byte vectors a thread holds of its chunk
+constexpr int BEAM_NVT = 8;   // 16-byte vectors a thread holds of its chunk
 constexpr int BEAM_CAP = 1024;
 struct BeamArgs {
   const void* logits;  // [G * W] rows of V
