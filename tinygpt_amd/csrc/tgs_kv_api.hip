@@ -247,8 +247,8 @@ int tgs_tree_commit(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* 
   a.n_acc = d_n_acc;
   a.tokens = d_tokens;
   a.path = d_path;
-  a.nblk = 1;
-  if ((int64_t)a.B * cache->layers > INT32_MAX) return fail(h, TGS_ETOOBIG, "rows");
+  a.nblk = T < 3 ? 1 : 2;  // (a path is seldom longer than two blocks)
+  if ((int64_t)a.nblk * a.B * cache->layers > INT32_MAX) return fail(h, TGS_ETOOBIG, "rows");
   DeviceGuard g(h->device);
   if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
   hipError_t e = tgs::launch_tree_commit(a, (hipStream_t)stream);
