@@ -138,7 +138,7 @@ def load() -> C.CDLL:
     L.tgs_token_logprobs.argtypes = [P, P, I, I, I, C.c_int64, P, P, P, P]
     L.tgs_mask_rows_from_dfa.restype = I
     L.tgs_mask_rows_from_dfa.argtypes = [P, P, P, I, P, I, P, P, C.c_int64, I, I, P, P, I, P]
-    # argument blocks (tgs_kv_cache, tgs_kv_rows, tgs_kv_seqs, tgs_attn) come as packed bytes
+    # (the calls of `CacheOps` go through the native module; argument blocks are pointers to structs)
     L.tgs_beam_select.restype = I
     L.tgs_beam_select.argtypes = [P, P, I, I, I, I, C.c_int64, P, I, P, P, I, P, P, P, P, P, P]
     L.tgs_tree_attention.restype = I

@@ -19,8 +19,11 @@ OUT = os.path.join(HERE, "libtgs_sampler.so")
 # its own library: not part of the sampler's C ABI)
 FLOOR_SRC = "tgs_floor.hip"
 FLOOR_OUT = os.path.join(HERE, "libtgs_floor.so")
-SOURCES = ["tgs_kernels.hip", "tgs_k64.hip", "tgs_spec.hip", "tgs_topp.hip", "tgs_topp_split.hip", "tgs_topk.hip", "tgs_logprob.hip",
-           "tgs_mask.hip", "tgs_kv.hip", "tgs_beam.hip", "tgs_attn_narrow.hip", "tgs_attn_wide.hip", "tgs_kv_api.hip", "tgs_api.hip"]
+SOURCES = ["tgs_attn_wide.hip", "tgs_attn_narrow.hip", "tgs_kernels.hip", "tgs_k64.hip", "tgs_spec.hip", "tgs_topp.hip", "tgs_topp_split.hip", "tgs_topk.hip", "tgs_logprob.hip",
+           "tgs_mask.hip", "tgs_kv.hip", "tgs_beam.hip", "tgs_kv_api.hip", "tgs_api.hip"]
+# the Python side's checks of the cache calls (host code against torch's headers)
+PY_SRC = "tgs_cache_py.cpp"
+PY_OUT = os.path.join(HERE, "_cache_calls.so")
 ARCH = os.environ.get("TGS_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -48,6 +51,18 @@ def hipcc() -> str:
     return "hipcc"
 
 
+def build_calls() -> subprocess.CompletedProcess:
+    """The checking module, to PY_OUT + ".tmp"."""
+    import sysconfig
+
+    from torch.utils import cpp_extension as ext
+
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D_GLIBCXX_USE_CXX11_ABI=1",
+           "-I" + sysconfig.get_paths()["include"], *["-I" + p for p in ext.include_paths()], os.path.join(CSRC, PY_SRC),
+           "-o", PY_OUT + ".tmp", *["-L" + p for p in ext.library_paths()], "-ltorch_python", "-ltorch_cpu", "-lc10", "-ldl"]
+    return subprocess.run(cmd, capture_output=True, text=True)
+
+
 def build(verbose: bool = False) -> str:
     """Compiles every source to an object in parallel, then links the library."""
     from concurrent.futures import ThreadPoolExecutor
@@ -62,8 +77,12 @@ def build(verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         return src, obj, cmd, r
 
-    with ThreadPoolExecutor(max_workers=min(8, len(SOURCES) + 1)) as ex:
+    with ThreadPoolExecutor(max_workers=min(8, len(SOURCES) + 2)) as ex:
+        calls = ex.submit(build_calls)
         results = list(ex.map(compile_one, SOURCES + [FLOOR_SRC]))
+        calls = calls.result()
+    if calls.returncode != 0:
+        raise RuntimeError(f"{PY_SRC} failed ({calls.returncode}):\n{' '.join(calls.args)}\n{calls.stderr}")
     floor = results.pop()
     msgs = []
     for src, obj, cmd, r in results:
@@ -89,6 +108,7 @@ def build(verbose: bool = False) -> str:
         print("\n".join(msgs), file=sys.stderr)
     os.replace(tmp, OUT)
     os.replace(ftmp, FLOOR_OUT)
+    os.replace(PY_OUT + ".tmp", PY_OUT)
     return OUT
 
 
