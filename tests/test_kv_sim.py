@@ -336,4 +336,4 @@ def test_refusals(sim):
     lens = torch.zeros(1, dtype=torch.int32)
     assert C.sim_append(sim, kn, vn, k.float(), v.float(), tabs, lens, None)[0] == -1       # dtype
     assert C.sim_fork(sim, k, v, tabs, lens, lens, -1)[0] == -1
-    assert C.sim_fork(sim, k, v, tabs, lens, lens, 1, ws_words=2)[0] == -5
+    assert C.sim_fork(sim, k, v, tabs, lens, lens, 1, ws_words=1)[0] == -5

@@ -51,11 +51,11 @@ struct KvForkArgs {
   int* lens_out;       // [R]
   int R, P, room, page_shift;
   int* owner;          // [n_pages] workspace, for pools beyond the planning kernel's LDS
-  int* fresh;          // [R * P] workspace: the free pages, in order
+  int* fresh;          // [n_pages] workspace, likewise: the free pages, in order
   int4* copies;        // [R] workspace: source page, new page, 8-token blocks, -
 };
-size_t kv_fork_lds(int n_pages);  // dynamic LDS of the planning kernel (0: its owners lie in the workspace)
-hipError_t launch_kv_fork(const KvForkArgs& a, hipStream_t st);
+size_t kv_fork_lds(int n_pages, int rows);  // dynamic LDS of the planning kernel (0: its lists lie in the workspace)
+hipError_t launch_kv_fork(const KvForkArgs& a, int num_cu, hipStream_t st);
 hipError_t set_kv_fork_lds_limit(size_t bytes);
 
 // Selection over beams and vocabulary.

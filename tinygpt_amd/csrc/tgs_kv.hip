@@ -172,7 +172,7 @@ __device__ __forceinline__ int owner_get(const int* o, int p) {
 
 struct PlanShared {
   int wave[KV_PLAN_NT / 64];
-  int base;
+  int4 copy;
 };
 
 // Exclusive sum of x over the workgroup, and the total.
@@ -192,39 +192,46 @@ __device__ __forceinline__ int block_excl(int x, PlanShared& s, int& total) {
   return before + incl - x;
 }
 
+// A new row: its parent, length and slots: shared [0, full), its own [full, end).
+struct ForkRow {
+  int par, len, full, end;
+};
+__device__ __forceinline__ ForkRow fork_row(const KvForkArgs& a, int par, int len) {
+  const long long cap = (long long)a.P << a.page_shift;
+  if (par < 0 || len < 0 || len > cap) return ForkRow{-1, 0, 0, 0};
+  const long long end = ((long long)len + a.room + (1 << a.page_shift) - 1) >> a.page_shift;
+  return ForkRow{par, len, len >> a.page_shift, end < a.P ? (int)end : a.P};
+}
+
 // One workgroup plans the fork: owners of the pages, the free list, the new
-// tables and the copies.
+// tables and the copies (with `out`; else only row `want`'s copy, to s.copy).
+// LDS: the rows (at most one a thread), owners and free list lie there.
 template <bool LDS>
-__global__ __launch_bounds__(KV_PLAN_NT) void plan_kernel(KvForkArgs a) {
-  TGS_STATIC_SMEM(PlanShared, s);
-  TGS_DYN_SMEM(dyn);
+__device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigned char* dyn, bool out, int want) {
+  const int tid = threadIdx.x, N = a.c.n_pages, P = a.P;
   int* owner = LDS ? (int*)dyn : a.owner;
-  const int tid = threadIdx.x, N = a.c.n_pages, P = a.P, page = 1 << a.page_shift;
-  const long long room_cap = (long long)P << a.page_shift;
+  int* fresh = LDS ? owner + N : a.fresh;
+  int2* rows = (int2*)(owner + 2 * (LDS ? N : 0));
+  auto load_row = [&](int r) {
+    const int par = a.parents[r];
+    return make_int2(par, (unsigned)par < (unsigned)a.R ? a.lens[par] : -1);
+  };
+  auto row_of = [&](int r) {
+    const int2 x = LDS ? rows[r] : load_row(r);
+    return fork_row(a, x.x, x.y);
+  };
+  if (LDS && tid < a.R) rows[tid] = load_row(tid);
   for (int i = tid; i < N; i += KV_PLAN_NT) owner[i] = OWNER_FREE;
   if (!LDS) __threadfence();
   __syncthreads();
-  // a row's parent, length and slots: shared [0, full), its own [full, end)
-  struct Row {
-    int par, len, full, end;
-  };
-  auto row_of = [&](int r) {
-    Row w{a.parents[r], 0, 0, 0};
-    if (w.par < 0 || w.par >= a.R) return Row{-1, 0, 0, 0};
-    w.len = a.lens[w.par];
-    if (w.len < 0 || w.len > room_cap) return Row{-1, 0, 0, 0};
-    w.full = w.len >> a.page_shift;
-    const long long end = ((long long)w.len + a.room + page - 1) >> a.page_shift;
-    w.end = end < P ? (int)end : P;
-    return w;
-  };
   for (int r = tid >> 6; r < a.R; r += KV_PLAN_NT / 64) {
-    const Row w = row_of(r);
+    const ForkRow w = row_of(r);
     if (w.par < 0) continue;
     const int* t = a.tables + (long long)w.par * P;
     for (int i = lane_id(); i < w.end; i += 64) {
       const int p = t[i];
       if ((unsigned)p < (unsigned)N) atomicMin(&owner[p], i < w.full ? -1 : r * P + i);
+      if (out && i < w.full) a.tables_out[(long long)r * P + i] = p;
     }
   }
   if (!LDS) __threadfence();
@@ -236,15 +243,14 @@ __global__ __launch_bounds__(KV_PLAN_NT) void plan_kernel(KvForkArgs a) {
   for (int i = n0; i < n1; i++) mine += owner_get<LDS>(owner, i) == OWNER_FREE;
   int n_free;
   int at = block_excl(mine, s, n_free);
-  const int most = a.R * P;
-  for (int i = n0; i < n1 && at < most; i++)
-    if (owner_get<LDS>(owner, i) == OWNER_FREE) a.fresh[at++] = i;
-  __threadfence();
+  for (int i = n0; i < n1; i++)
+    if (owner_get<LDS>(owner, i) == OWNER_FREE) fresh[at++] = i;
+  if (!LDS) __threadfence();
   __syncthreads();
   int base = 0;
   for (int r0 = 0; r0 < a.R; r0 += KV_PLAN_NT) {
     const int r = r0 + tid;
-    const Row w = r < a.R ? row_of(r) : Row{-1, 0, 0, 0};
+    const ForkRow w = r < a.R ? row_of(r) : ForkRow{-1, 0, 0, 0};
     const int* t = a.tables + (long long)(w.par < 0 ? 0 : w.par) * P;
     int need = 0;
     for (int i = w.full; i < w.end; i++) {
@@ -256,48 +262,68 @@ __global__ __launch_bounds__(KV_PLAN_NT) void plan_kernel(KvForkArgs a) {
     base += total;
     if (r >= a.R) continue;
     const bool fits = next + need <= n_free;
-    int* out = a.tables_out + (long long)r * P;
+    int* to_row = a.tables_out + (long long)r * P;
     int4 copy = make_int4(-1, -1, 0, 0);
     for (int i = w.full; i < w.end; i++) {
       const int p = t[i];
       const bool named = (unsigned)p < (unsigned)N;
       int to = p;
       if (!(named && owner_get<LDS>(owner, p) == r * P + i)) {
-        to = fits ? a.fresh[next++] : -1;
+        to = fits ? fresh[next++] : -1;
         const int held = w.len - (i << a.page_shift);
         if (held > 0 && named && fits) copy = make_int4(p, to, (held + 7) >> 3, 0);
       }
-      out[i] = to;
+      if (out) to_row[i] = to;
     }
-    a.copies[r] = copy;
+    if (r == want) s.copy = copy;
+    if (!out) continue;
+    if (want < 0) a.copies[r] = copy;
     // -1: the pool ran out of pages
-    a.lens_out[r] = w.par < 0 ? 0 : fits && ((long long)w.len + a.room <= room_cap) ? w.len : -1;
+    a.lens_out[r] = w.par < 0 ? 0 : fits && (long long)w.len + a.room <= ((long long)P << a.page_shift) ? w.len : -1;
   }
+  if (!out) return;
   for (int r = tid >> 6; r < a.R; r += KV_PLAN_NT / 64) {
-    const Row w = row_of(r);
-    const int* t = a.tables + (long long)(w.par < 0 ? 0 : w.par) * P;
-    int* out = a.tables_out + (long long)r * P;
-    for (int i = lane_id(); i < P; i += 64)
-      if (i < w.full || i >= w.end) out[i] = i < w.full ? t[i] : -1;
+    const ForkRow w = row_of(r);
+    for (int i = w.end + lane_id(); i < P; i += 64) a.tables_out[(long long)r * P + i] = -1;
   }
 }
 
-// Workgroup (row r, layer l, keys or values): the blocks of r's page that are
-// in use lie contiguous per head.
-__global__ __launch_bounds__(KV_NT) void copy_kernel(KvForkArgs a) {
-  const int r = blockIdx.x;
-  const int4 c = a.copies[r];
+// The blocks of row r's page that are in use lie contiguous per head: copies
+// those of layer y / 2, keys or values.
+__device__ __forceinline__ void copy_page(const KvForkArgs& a, const int4& c, int y) {
   if (c.z == 0) return;
-  const int l = blockIdx.y >> 1, D = a.c.head_dim, H = a.c.kv_heads;
-  const bool val = blockIdx.y & 1;
+  const int l = y >> 1, D = a.c.head_dim, H = a.c.kv_heads;
+  const bool val = y & 1;
   uint16_t* pool = (uint16_t*)(val ? a.c.v : a.c.k) + l * (val ? a.c.v_layer : a.c.k_layer);
   const long long ps = val ? a.c.v_page : a.c.k_page;
   const uint4* from = (const uint4*)(pool + c.x * ps);
   uint4* to = (uint4*)(pool + c.y * ps);
   const int n = c.z * D;  // 16-byte vectors of a head's blocks
   const int hs = D << a.page_shift >> 3;  // and of its page
-  for (int h = 0; h < H; h++)
-    for (int i = threadIdx.x; i < n; i += KV_NT) to[h * hs + i] = from[h * hs + i];
+  // a wave a head, so that every thread has work where a head's blocks are few
+  for (int h = threadIdx.x >> 6; h < H; h += blockDim.x >> 6)
+    for (int i = lane_id(); i < n; i += 64) to[(long long)h * hs + i] = from[(long long)h * hs + i];
+}
+
+template <bool LDS>
+__global__ __launch_bounds__(KV_PLAN_NT) void plan_kernel(KvForkArgs a) {
+  TGS_STATIC_SMEM(PlanShared, s);
+  TGS_DYN_SMEM(dyn);
+  plan<LDS>(a, s, dyn, true, -1);
+}
+
+// Workgroup (row, layer and pool).
+__global__ __launch_bounds__(KV_NT) void copy_kernel(KvForkArgs a) { copy_page(a, a.copies[blockIdx.x], blockIdx.y); }
+
+// Both in one launch, every workgroup planning for itself: where no more than
+// a workgroup a CU copies, planning 256 times at once costs less than a second
+// launch (4 beams of 530 tokens, 16 layers: kernels of 12 us in two, 6.6 in one).
+__global__ __launch_bounds__(KV_PLAN_NT) void fork_kernel(KvForkArgs a) {
+  TGS_STATIC_SMEM(PlanShared, s);
+  TGS_DYN_SMEM(dyn);
+  plan<true>(a, s, dyn, blockIdx.x == 0 && blockIdx.y == 0, blockIdx.x);
+  __syncthreads();
+  copy_page(a, s.copy, blockIdx.y);
 }
 
 }  // namespace kv
@@ -312,11 +338,18 @@ hipError_t launch_tree_commit(const KvWriteArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-constexpr size_t FORK_LDS = 128 * 1024;  // owners held in LDS at most
-size_t kv_fork_lds(int n_pages) { return (size_t)n_pages * 4 <= FORK_LDS ? (size_t)n_pages * 4 : 0; }
+constexpr size_t FORK_LDS = 128 * 1024;  // of the planning workgroup at most
+size_t kv_fork_lds(int n_pages, int rows) {
+  const size_t n = (size_t)n_pages * 8 + 16 + (size_t)rows * 8;
+  return rows <= KV_PLAN_NT && n <= FORK_LDS ? n : 0;
+}
 
-hipError_t launch_kv_fork(const KvForkArgs& a, hipStream_t st) {
-  const size_t lds = kv_fork_lds(a.c.n_pages);
+hipError_t launch_kv_fork(const KvForkArgs& a, int num_cu, hipStream_t st) {
+  const size_t lds = kv_fork_lds(a.c.n_pages, a.R);
+  if (lds && (long long)a.R * 2 * a.c.layers <= num_cu) {
+    hipLaunchKernelGGL(kv::fork_kernel, dim3(a.R, 2 * a.c.layers), dim3(KV_PLAN_NT), lds, st, a);
+    return hipGetLastError();
+  }
   if (lds)
     hipLaunchKernelGGL(kv::plan_kernel<true>, dim3(1), dim3(KV_PLAN_NT), lds, st, a);
   else
@@ -328,8 +361,10 @@ hipError_t launch_kv_fork(const KvForkArgs& a, hipStream_t st) {
 }
 
 hipError_t set_kv_fork_lds_limit(size_t bytes) {
-  return hipFuncSetAttribute((const void*)kv::plan_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(bytes < FORK_LDS ? bytes : FORK_LDS));
+  const int n = (int)(bytes < FORK_LDS ? bytes : FORK_LDS);
+  const hipError_t e = hipFuncSetAttribute((const void*)kv::plan_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, n);
+  const hipError_t f = hipFuncSetAttribute((const void*)kv::fork_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, n);
+  return e != hipSuccess ? e : f;
 }
 
 }  // namespace tgs

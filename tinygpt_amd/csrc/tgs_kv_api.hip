@@ -268,9 +268,9 @@ int tgs_kv_fork(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_seqs* seqs
   if (d_tables_out == seqs->tables || d_lens_out == seqs->lens)
     return fail(h, TGS_EINVAL, "fork: outputs must not be inputs");
   if ((int64_t)R * P >= INT32_MAX || cache->layers > 32767) return fail(h, TGS_ETOOBIG, "fork: rows");
-  // workspace: copies, free pages, owners
-  const size_t own = tgs::kv_fork_lds(cache->n_pages) ? 0 : (size_t)cache->n_pages;
-  if ((size_t)R * 2 + ((size_t)R * P + own + 1) / 2 > h->ws_words)
+  // workspace: copies, and for pools beyond the planning kernel's LDS owners and free pages
+  const size_t pages = tgs::kv_fork_lds(cache->n_pages, R) ? 0 : (size_t)cache->n_pages;
+  if ((size_t)R * 2 + pages > h->ws_words)
     return fail(h, TGS_ETOOBIG, "fork: pages beyond the handle's workspace");
   DeviceGuard g(h->device);
   if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
@@ -288,9 +288,9 @@ int tgs_kv_fork(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_seqs* seqs
   a.room = room;
   a.page_shift = shift_of(cache->page);
   a.copies = (int4*)h->ws;
-  a.fresh = (int*)(a.copies + R);
-  a.owner = a.fresh + (size_t)R * P;
-  hipError_t e = tgs::launch_kv_fork(a, (hipStream_t)stream);
+  a.owner = (int*)(a.copies + R);
+  a.fresh = a.owner + pages;
+  hipError_t e = tgs::launch_kv_fork(a, h->num_cu, (hipStream_t)stream);
   if (e != hipSuccess) return hip_fail(h, e, "fork kernel launch");
   return TGS_OK;
 }
