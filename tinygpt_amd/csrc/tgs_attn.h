@@ -311,8 +311,19 @@ __device__ __forceinline__ float wave_sumf(float x) {
 // waves share the row's parts (few rows, many parts), with R = 16 each takes
 // four rows (the places of the parts are found once for them).  Every sum runs
 // in an order that the lengths alone fix.
+//
+// A part's sums lie as its kernel holds them: the narrow kernel's row by row,
+// the wide kernel's by 32 rows, [D / 8][half][row][4], a lane's four next to the
+// neighbouring rows' (its stores are 1 KB each; 64-byte pieces took 5 us more
+// of 16 sequences' 63 nodes).
+template <int TILE>
+__device__ __forceinline__ int part_at(int D, int row, int d) {
+  if (TILE == NTILE) return row * D + d;
+  return (row >> 5) * 32 * D + ((d >> 3) * 64 + ((d >> 2) & 1) * 32 + (row & 31)) * 4 + (d & 3);
+}
+
 struct JoinShared {
-  int part[1024];  // rows of the workspace, of the parts of this (sequence, key head)
+  int part[1024];  // of this (sequence, key head)
   int n;
   float o[4][256];
   float ml[4][2];
@@ -332,18 +343,19 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, int b, int h, int i
 }
 
 // Row i of (b, h) from n parts, a quarter of them a wave.
-template <typename DT>
+template <typename DT, int TILE>
 __device__ __forceinline__ void join_one(const AttnArgs& a, JoinShared& s, int b, int h, int i, int n) {
+  const int r = i % a.QB, part = a.QB * a.D;
   const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
   const int j0 = n * wave / 4, j1 = n * (wave + 1) / 4;
   float m = NEG;
-  for (int j = j0 + lane; j < j1; j += 64) m = fmaxf(m, a.part_ml[2ll * s.part[j]]);
+  for (int j = j0 + lane; j < j1; j += 64) m = fmaxf(m, a.part_ml[2ll * (s.part[j] * a.QB + r)]);
   m = wave_maxf(m);
   float l = 0.0f, o[4] = {0, 0, 0, 0};
   for (int c = j0; c < j1; c += 64) {
     float f = 0.0f;
     if (c + lane < j1) {
-      const long long p = s.part[c + lane];
+      const long long p = s.part[c + lane] * a.QB + r;
       const float pm = a.part_ml[2 * p];
       f = pm == NEG ? 0.0f : exp2_hw(pm - m);
       l += f * a.part_ml[2 * p + 1];
@@ -353,9 +365,10 @@ __device__ __forceinline__ void join_one(const AttnArgs& a, JoinShared& s, int b
       float x[8][4];
 #pragma unroll
       for (int y = 0; y < 8; y++) {  // (past the last part: the last one's, not used)
-        const long long at = (long long)s.part[j + y < cn ? c + j + y : c + cn - 1] * a.D;
+        const long long at = (long long)s.part[j + y < cn ? c + j + y : c + cn - 1] * part;
 #pragma unroll
-        for (int z = 0; z < 4; z++) x[y][z] = z * 64 + lane < a.D ? a.part_o[at + z * 64 + lane] : 0.0f;
+        for (int z = 0; z < 4; z++)
+          x[y][z] = z * 64 + lane < a.D ? a.part_o[at + part_at<TILE>(a.D, r, z * 64 + lane)] : 0.0f;
       }
 #pragma unroll
       for (int y = 0; y < 8; y++) {
@@ -415,7 +428,7 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
         has = from != share_start(U, N, w + 1);
       }
       const u64 m = __ballot(has);
-      if (has) s.part[n + lanes_below(m)] = ((qb * N + w) * 2 + (from < s0)) * a.QB + r0;
+      if (has) s.part[n + lanes_below(m)] = (qb * N + w) * 2 + (from < s0);
       n += __popcll(m);
     }
     if (lane == 0) s.n = n;
@@ -423,56 +436,45 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
   __syncthreads();
   const int n = s.n;
   if constexpr (R == 1) {
-    join_one<DT>(a, s, b, h, i0, n);
+    join_one<DT, TILE>(a, s, b, h, i0, n);
     return;
   }
-  // Four rows a wave, 16 lanes each for the parts' maxima and sums.
-  const int y0 = lane >> 4, j0 = lane & 15, r = wave + 4 * y0;
+  // A lane takes one row and, of the row's D / 4 fours, every sixteenth.
+  const int i = i0 + (lane & 15), r = r0 + (lane & 15), sub = wave * 4 + (lane >> 4);
+  const long long part = (long long)a.QB * a.D;
   float m = NEG;
-  for (int j = j0; j < n; j += 16) m = fmaxf(m, a.part_ml[2ll * (s.part[j] + r)]);
-  m = fmaxf(m, xor_lane<1>(m));
-  m = fmaxf(m, xor_lane<2>(m));
-  m = fmaxf(m, xor_lane<4>(m));
-  m = fmaxf(m, xor_lane<8>(m));
-  float l = 0.0f, o[4][4] = {};
-  for (int c = 0; c < n; c += 16) {
-    float f = 0.0f;
-    if (c + j0 < n) {
-      const long long p = s.part[c + j0] + r;
-      const float pm = a.part_ml[2 * p];
-      f = pm == NEG ? 0.0f : exp2_hw(pm - m);
-      l += f * a.part_ml[2 * p + 1];
+  for (int j = 0; j < n; j++) m = fmaxf(m, a.part_ml[2ll * (s.part[j] * a.QB + r)]);
+  float l = 0.0f;
+  f32x4 o[4] = {};
+  for (int j = 0; j < n; j += 2) {
+    f32x4 x[2][4];
+    float f[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int p = s.part[j + k < n ? j + k : j];  // (past the last part: not used)
+      const float pm = a.part_ml[2ll * (p * a.QB + r)], pl = a.part_ml[2ll * (p * a.QB + r) + 1];
+#pragma unroll
+      for (int z = 0; z < 4; z++)
+        if ((sub + 16 * z) * 4 < a.D) x[k][z] = *(const f32x4*)(a.part_o + p * part + part_at<TILE>(a.D, r, (sub + 16 * z) * 4));
+      f[k] = j + k >= n || pm == NEG ? 0.0f : exp2_hw(pm - m);
+      if (j + k < n) l += pm == NEG ? pl : f[k] * pl;  // (a part without weights has the sum 0, or NaN)
     }
-    const int cn = n - c < 16 ? n - c : 16;
-    for (int j = 0; j < cn; j += 2) {
-      float x[2][4][4];
 #pragma unroll
-      for (int k = 0; k < 2; k++)  // (past the last part: the last one's, not used)
+    for (int k = 0; k < 2; k++) {
+      if (j + k >= n) break;
 #pragma unroll
-        for (int y = 0; y < 4; y++) {
-          const long long at = (long long)(s.part[c + (j + k < cn ? j + k : j)] + wave + 4 * y) * a.D;
-#pragma unroll
-          for (int z = 0; z < 4; z++) x[k][y][z] = z * 64 + lane < a.D ? a.part_o[at + z * 64 + lane] : 0.0f;
-        }
-#pragma unroll
-      for (int k = 0; k < 2; k++) {
-        if (j + k >= cn) break;
-#pragma unroll
-        for (int y = 0; y < 4; y++) {
-          const float fy = readlane_f32(f, 16 * y + j + k);
-#pragma unroll
-          for (int z = 0; z < 4; z++) o[y][z] += fy * x[k][y][z];
-        }
-      }
+      for (int z = 0; z < 4; z++)
+        if ((sub + 16 * z) * 4 < a.D) o[z] += x[k][z] * f[k];
     }
   }
-  l += xor_lane<1>(l);
-  l += xor_lane<2>(l);
-  l += xor_lane<4>(l);
-  l += xor_lane<8>(l);
+  if (i >= a.M) return;
+  const int t = i / a.G;
+  const long long out = ((long long)b * a.T + t) * a.Hq + h * a.G + (i - t * a.G);
+  const float rl = 1.0f / l;
 #pragma unroll
-  for (int y = 0; y < 4; y++)
-    if (i0 + wave + 4 * y < a.M) write_row<DT>(a, b, h, i0 + wave + 4 * y, o[y], readlane_f32(m, 16 * y), readlane_f32(l, 16 * y));
+  for (int z = 0; z < 4; z++)
+    if ((sub + 16 * z) * 4 < a.D) store4<DT>((uint16_t*)a.out + out * a.D + (sub + 16 * z) * 4, o[z] * rl);
+  if (a.lse && sub == 0) a.lse[out] = row_lse(m, l);
 }
 
 // Few rows: one a workgroup, so that their parts are read by many.

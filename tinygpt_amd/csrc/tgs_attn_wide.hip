@@ -45,24 +45,24 @@ struct Wide {
     }
   }
 
-  // Page of each of cache tile i's eight 8-token blocks, block lane % 8 in a
-  // lane; of a block past the end, the last one's.
+  // Pages of the 8-token blocks from cache tile i on, one a lane (eight a tile);
+  // of a block past the end, the last one's.
   __device__ __forceinline__ int entries(int i) const {
-    const int blk = i * WTILE + (lane & 7) * 8, last = len - 1;
+    const int blk = i * WTILE + lane * 8, last = len - 1;
     return table[(blk < last ? blk : last) >> a.page_shift];
   }
 
   // Where chunk c's 8-token block blk of tile i lies in its pool, in elements.
   // The chunks of a wave belong to one block (but for rows of 12 chunks), so this is
   // scalar arithmetic.
-  __device__ __forceinline__ long long block_at(int i, int blk, int entry, long long page) const {
+  __device__ __forceinline__ long long block_at(int i, int blk, int entry, int off, long long page) const {
     const int last = (len - 1) >> 3, x = i * (WTILE / 8) + blk;
     const int in_page = ((x < last ? x : last) << 3) & ((1 << a.page_shift) - 1);
     long long pg;
     if constexpr (C == 12)
-      pg = __shfl(entry, blk, 64);
+      pg = __shfl(entry, off * 8 + blk, 64);
     else
-      pg = (int)readlane_u32((uint32_t)entry, blk);
+      pg = (int)readlane_u32((uint32_t)entry, off * 8 + blk);
     return pg * page + (((long long)h * D) << a.page_shift) + (long long)in_page * D;
   }
   // A chunk's index, its wave's for the block's sake.
@@ -76,17 +76,18 @@ struct Wide {
     return (n * NTHR + wave * 64) / PER;
   }
 
-  __device__ __forceinline__ void load(int i, int entry, Vec (&k)[NCH], Vec (&v)[NCH]) {
+  // Tile i; entry: entries(i - off).
+  __device__ __forceinline__ void load(int i, int entry, int off, Vec (&k)[NCH], Vec (&v)[NCH]) {
     if ((unsigned)entry >= (unsigned)a.n_pages) {
       bad = true;  // (its sequence's rows become NaN)
       entry = 0;
     }
 #pragma unroll
     for (int n = 0; n < NCH; n++)
-      k[n] = *(const Vec*)((const uint16_t*)a.k + block_at(i, block_of<8 * C>(n), entry, a.k_page) + chunk(n) % (8 * C) * 8);
+      k[n] = *(const Vec*)((const uint16_t*)a.k + block_at(i, block_of<8 * C>(n), entry, off, a.k_page) + chunk(n) % (8 * C) * 8);
 #pragma unroll
     for (int n = 0; n < NCH; n++)
-      v[n] = *(const Vec*)((const uint16_t*)a.v + block_at(i, block_of<D>(n), entry, a.v_page) + chunk(n) % D * 8);
+      v[n] = *(const Vec*)((const uint16_t*)a.v + block_at(i, block_of<D>(n), entry, off, a.v_page) + chunk(n) % D * 8);
   }
 
   // To buffer f; what lies past the sequence's end is not 0 there (it may be
@@ -241,10 +242,7 @@ struct Wide {
     auto cut = [&](int t) { return t < tc ? t : tc - 1; };
     const bool cached = t0 < tc, drafted = t1 > nc;
     int e = 0, next = 0;
-    if (cached) {
-      e = entries(t0);
-      next = entries(cut(t0 + 1));
-    }
+    if (cached) e = entries(t0);  // (of the first eight tiles)
     int par = -1;
     if (drafted) par = parent_of(a, b);
     Vec q[KK];
@@ -265,12 +263,12 @@ struct Wide {
     if (drafted) {
       Vec kt[NCH], vt[TURN][8];
       load_tree(kt, vt);
-      if (cached) load(t0, e, k0, v0);
+      if (cached) load(t0, e, 0, k0, v0);
       sched_fence();
       lds_barrier();  // (the buffers are free)
       store_tree(s, kt, vt);
     } else {
-      load(t0, e, k0, v0);
+      load(t0, e, 0, k0, v0);
       sched_fence();
       lds_barrier();
     }
@@ -279,16 +277,12 @@ struct Wide {
       // the next AHEAD ones are on their way to registers; requests past the
       // last tile ask for it again, so that the number in flight is known.
       store(s, 0, t0, k0, v0);
-      e = next;
-      next = entries(cut(t0 + 2));
+      next = entries(cut(t0 + 1 + AHEAD));
       sched_fence();
-      load(cut(t0 + 1), e, k0, v0);
+      load(cut(t0 + 1), e, cut(t0 + 1) - t0, k0, v0);
       sched_fence();
       if constexpr (AHEAD == 2) {
-        e = next;
-        next = entries(cut(t0 + 3));
-        sched_fence();
-        load(cut(t0 + 2), e, k1, v1);
+        load(cut(t0 + 2), e, cut(t0 + 2) - t0, k1, v1);
         sched_fence();
       }
     }
@@ -313,7 +307,7 @@ struct Wide {
         e = next;
         next = entries(cut(t + 2 + AHEAD));
         sched_fence();
-        load(cut(t + 1 + AHEAD), e, ks, vs);
+        load(cut(t + 1 + AHEAD), e, 0, ks, vs);
         sched_fence();
         if (work) {
           scores(s, f, q, sc);
@@ -345,7 +339,7 @@ struct Wide {
     const f32x16(&o)[DT32] = st.o;
     l += xor_lane<32>(l);
     if (__ballot(bad)) l = __builtin_nanf("");  // (every wave read every entry)
-    if (i >= a.M) return;
+    if (i >= a.M) return;  // (a part's rows past M are not read)
     if (full) {
       const long long row = ((long long)b * a.T + node) * a.Hq + h * a.G + hg;
       const float r = 1.0f / l;
@@ -358,14 +352,14 @@ struct Wide {
         }
       if (a.lse && half == 0) a.lse[row] = row_lse(m, l);
     } else {
-      const long long row = part + wave * 32 + col;
+      float* to = a.part_o + part * D + wave * 32 * D + lane * 4;
 #pragma unroll
       for (int d = 0; d < DT32; d++)
 #pragma unroll
         for (int x = 0; x < 4; x++)
-          *(f32x4*)(a.part_o + row * D + d * 32 + x * 8 + half * 4) =
-              f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+          *(f32x4*)(to + (d * 4 + x) * 256) = f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
       if (half == 0) {
+        const long long row = part + wave * 32 + col;
         a.part_ml[row * 2] = m;
         a.part_ml[row * 2 + 1] = l;
       }
@@ -425,8 +419,6 @@ hipError_t wide_run(const AttnArgs& a, hipStream_t st) {
 
 template <typename DT, int D>
 hipError_t wide_dim(const AttnArgs& a, int qw, hipStream_t st) {
-  if constexpr (D <= 128)
-    if (qw == 2) return wide_run<DT, D, 2>(a, st);
   if (qw == 4) return wide_run<DT, D, 4>(a, st);
   if constexpr (D <= 128)
     if (qw == 8) return wide_run<DT, D, 8>(a, st);
@@ -441,13 +433,10 @@ template <typename DT>
 hipError_t wide_lds_type() {
   hipError_t e = hipSuccess;
   auto take = [&](hipError_t x) { e = x != hipSuccess ? x : e; };
-  take(wide_lds<DT, 64, 2>());
   take(wide_lds<DT, 64, 4>());
   take(wide_lds<DT, 64, 8>());
-  take(wide_lds<DT, 96, 2>());
   take(wide_lds<DT, 96, 4>());
   take(wide_lds<DT, 96, 8>());
-  take(wide_lds<DT, 128, 2>());
   take(wide_lds<DT, 128, 4>());
   take(wide_lds<DT, 128, 8>());
   take(wide_lds<DT, 256, 4>());
@@ -481,7 +470,7 @@ AttnPlan attn_plan(int M, int D) {
   } else {
     p.wide = 1;
     p.tile = attn::WTILE;
-    p.QB = D == 256 ? 128 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+    p.QB = D == 256 || M <= 128 ? 128 : 256;  // (48 rows in 64: 43 us where in 128 they take 35; two groups of 128 a CU 98 where one of 256 takes 87)
     p.per_cu = D == 256 || p.QB == 256 ? 1 : 2;
     p.least = 4;
   }
