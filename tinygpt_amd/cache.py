@@ -100,7 +100,7 @@ class CacheOps:
         if out is None:
             out = self._new(q.dtype, *q.shape)
         self._call("tree_attention", stream, q, k_new, v_new, k, v, tables, lens, parents, -1 if max_len is None else max_len,
-                   q.shape[-1] ** -0.5 if scale is None else scale, out, lse)
+                   scale, out, lse)
         return out
 
     def kv_append(self, k_new, v_new, k, v, tables, lens, counts=None, lens_out=None, stream=None):

@@ -9,6 +9,8 @@
 
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <dlfcn.h>
 #include <initializer_list>
@@ -191,8 +193,8 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
       PyErr_SetString(PyExc_TypeError, "beam_select: logits must be float32 or bfloat16");
       throw Raised{};
     }
-    if (!c.here(x)) bad(c.fn, "logits must be on the handle's device");
     const int64_t rows = x.size(0), W = c.number(a[5]), no = c.number(a[6]);
+    if (!c.here(x)) bad(c.fn, "logits must be on the handle's device");
     int64_t V = c.number(a[7]);
     if (V < 0) V = x.size(1);
     if (V < 1 || V > x.size(1)) bad(c.fn, "vocab outside the logits' width");
@@ -222,7 +224,7 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// handle, device, stream, q, k_new, v_new, k, v, tables, lens, parents, max_len (-1: the tables'), scale, out, lse
+// handle, device, stream, q, k_new, v_new, k, v, tables, lens, parents, max_len (-1: the tables'), scale (None: 1 / sqrt(D)), out, lse
 PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
     Call c("tree_attention", a, n, 15);
@@ -230,9 +232,9 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     tgs_kv_rows rows;
     tgs_kv_seqs seqs;
     tgs_attn t;
+    const at::Tensor& q = c.tensor(a[3], "q");
     const at::ScalarType dt = c.cache(a[6], a[7], false, cache);
     c.seqs(a[8], a[9], seqs);
-    const at::Tensor& q = c.tensor(a[3], "q");
     if (q.dim() != 4 || q.size(1) > INT32_MAX || q.size(2) > INT32_MAX) bad(c.fn, "q must be [B, T, q_heads, D]");
     const int64_t B = seqs.B, T = q.size(1), Hq = q.size(2), H = cache.kv_heads, D = cache.head_dim;
     c.rows(a[3], "q", dt, {B, T, Hq, D});
@@ -245,7 +247,7 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     t.q_heads = (int)Hq;
     const long most = c.number(a[11]);
     t.max_len = most >= 0 ? (int)most : (int)std::min<int64_t>((int64_t)seqs.width * cache.page, INT32_MAX);
-    t.scale = (float)PyFloat_AsDouble(a[12]);
+    t.scale = a[12] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)PyFloat_AsDouble(a[12]);
     if (PyErr_Occurred()) throw Raised{};
     t.out = c.exact(c.tensor(a[13], "out"), "out", dt, {B, T, Hq, D});
     const at::Tensor* lse = c.maybe(a[14], "lse");
