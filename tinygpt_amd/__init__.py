@@ -2,7 +2,10 @@
 
 The product is libtgs_sampler.so (C ABI in include/tgs_sampler.h): gfx950
 HIP kernels for penalties, temperature, the grammar mask, top-k, top-p, the
-categorical draw and speculative verification.  This package holds the
+categorical draw and speculative verification, and for what a decode step
+runs next to them: beam selection, attention of drafted nodes over a paged
+key/value cache, and the cache's writes, commits and forks (`cache`, whose
+methods `Sampler` has).  This package holds the
 kernels' sources (csrc/), the in-tree build, a ctypes binding (`Sampler`,
 `sample_noalloc`), the host grammar compilers whose automata fill
 mask-table rows on the device (`grammar` for GBNF, `json_schema` for JSON

@@ -12,6 +12,12 @@
 // logits' own, so it needs no arithmetic; join_kernel orders the candidates of
 // different beams by totals held in 64 bits, since those of different beams
 // may lie closer than 32 bits tell apart.
+//
+// 32 requests of 8 beams over 128,256 ids, bf16 (66 MB): chunks 27 us, 2.4 TB/s,
+// in two rounds of four workgroups a CU that each load, sort and collect in
+// turn; join 10 us.  4 beams over 32,000 ids, fp32: 5.4 and 5.8 us, the latency
+// of dependent steps.  Joining in the last workgroup to finish, in one launch,
+// took 0.5 and 7 us more: it has to wait for its stores to drain first.
 #include "tgs_device.h"
 #include "tgs_kv.h"
 #include "tgs_row.h"
