@@ -5,8 +5,8 @@
 // each other for each d, which is the operand order of the attention's second
 // product.  No arithmetic: every kernel here moves 16-bit values and is bound
 // by bytes, or by latency for single tokens.  Measured: prompts of 300 to 2048
-// tokens, 16 layers, 175 us (923 MB, 5.3 TB/s read and written); pages of 128
-// forked beams 95 us (403 MB, 4.3 TB/s).
+// tokens, 16 layers, 176 us (923 MB, 5.2 TB/s read and written); pages of 128
+// forked beams 93 us (403 MB, 4.3 TB/s).
 #include "tgs_device.h"
 #include "tgs_kv.h"
 #include "tgs_row.h"
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(KV_NT) void copy_kernel(KvForkArgs a) { copy_page(a
 
 // Both in one launch, every workgroup planning for itself: where no more than
 // a workgroup a CU copies, planning 256 times at once costs less than a second
-// launch (4 beams of 530 tokens, 16 layers: kernels of 12 us in two, 6.0 in one).
+// launch (4 beams of 530 tokens, 16 layers: kernels of 12 us in two, 5.8 in one).
 __global__ __launch_bounds__(KV_PLAN_NT) void fork_kernel(KvForkArgs a) {
   TGS_STATIC_SMEM(PlanShared, s);
   TGS_DYN_SMEM(dyn);
