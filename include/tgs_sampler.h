@@ -342,7 +342,8 @@ typedef struct {
  * to it.  A sequence of which a page lies outside the pool gives NaN; lengths are taken
  * within [0, width page].  What the cache's pages hold past a sequence's end
  * is never used.  Products and sums are 32-bit; softmax weights are rounded
- * to the cache's type before they multiply values. */
+ * to the cache's type before they multiply values.  Outputs must not overlap
+ * inputs. */
 int tgs_tree_attention(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs,
                        const tgs_attn* attn, tgs_stream stream);
 
@@ -350,7 +351,8 @@ int tgs_tree_attention(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_row
  * to positions lens[b] + i in every layer, and d_lens_out[b] = lens[b] +
  * counts[b].  A sequence whose rows do not fit (a count outside [0, T], a
  * position past its table, a page outside the pool) keeps its cache and gets
- * -1.  Tables of different sequences must not name one page where rows are written. */
+ * -1.  Tables of different sequences must not name one page where rows are
+ * written.  d_lens_out must not overlap an input. */
 int tgs_kv_append(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs, int T,
                   const int32_t* d_counts, int32_t* d_lens_out, tgs_stream stream);
 
@@ -363,7 +365,8 @@ int tgs_kv_append(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* ro
  *   d_n_acc  [B] nodes accepted, the root not counted
  *   d_tokens [B][T] accepted tokens, then the id sampled at the last, -1 padded
  *   d_path   [B][T] the root and the accepted nodes, -1 padded
- *   d_lens_out [B] lens + 1 + n_acc; -1: the rows did not fit */
+ *   d_lens_out [B] lens + 1 + n_acc; -1: the rows did not fit
+ * Outputs must not overlap inputs. */
 int tgs_tree_commit(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs, int T,
                     const int32_t* d_parents, const int32_t* d_draft, const int32_t* d_sampled, int32_t* d_n_acc,
                     int32_t* d_tokens, int32_t* d_path, int32_t* d_lens_out, tgs_stream stream);

@@ -336,3 +336,15 @@ def test_refusals(sampler):
         sampler.kv_fork(k[None], v[None], tabs, lens, lens.clone(), tables_out=tabs)
     with pytest.raises(ValueError):
         sampler.kv_append(kn[None], vn[None], k[None], v[None], tabs, lens, lens_out=lens)
+
+
+@pytest.mark.parametrize("name", ["scores", "parents", "tokens", "hist", "hist_len"])
+def test_beam_outputs_that_are_inputs_are_refused(sampler, name):
+    H.log(f"beam outputs that are inputs: {name}")
+    ints = dict(dtype=torch.int32, device=DEV)
+    x, s, hist, n = torch.zeros(4, 50, device=DEV), torch.zeros(4, device=DEV), torch.zeros(4, 1, **ints), torch.zeros(4, **ints)
+    out = {"scores": torch.zeros(4, device=DEV), "parents": torch.zeros(4, **ints), "tokens": torch.zeros(4, **ints),
+           "hist": torch.zeros(4, 1, **ints), "hist_len": torch.zeros(4, **ints)}
+    out[name] = {"scores": s, "hist": hist}.get(name, n)
+    with pytest.raises(ValueError):
+        sampler.beam_select(x, s, 2, 2, hist=hist, hist_len=n, out=out)

@@ -213,12 +213,14 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
       lp = c.ints(a[9], "hist_len", {rows});
       ohp = c.ints(a[13], "out hist", {m, H});
       olp = c.ints(a[14], "out hist_len", {m});
-      c.apart(ohp, "out hist", {hp});
-      c.apart(olp, "out hist_len", {lp});
+      c.apart(ohp, "out hist", {hp, lp});
+      c.apart(olp, "out hist_len", {hp, lp});
     }
     float* os = (float*)c.exact(c.tensor(a[10], "out scores"), "out scores", at::kFloat, {m});
     int32_t *op = c.ints(a[11], "out parents", {m}), *ot = c.ints(a[12], "out tokens", {m});
     c.apart(os, "out scores", {scores});
+    c.apart(op, "out parents", {hp, lp});
+    c.apart(ot, "out tokens", {hp, lp});
     return p_beam(c.h, x.data_ptr(), dt == at::kFloat ? TGS_F32 : TGS_BF16, (int)G, (int)W, (int)V, x.stride(0), scores,
                   (int)no, hp, lp, (int)H, os, op, ot, ohp, olp, c.stream);
   });
