@@ -8,10 +8,11 @@
 // vectors whose maximum passes it are searched, and what is found is sorted.
 // The sum of exponentials comes from the same registers, each thread's terms
 // relative to a power of two of its own, so that no thread waits for the
-// chunk's maximum and joining the sums is exact.  Inside a row the order is the
-// logits' own, so it needs no arithmetic; join_kernel orders the candidates of
-// different beams by totals held in 64 bits, since those of different beams
-// may lie closer than 32 bits tell apart.
+// chunk's maximum and scaling the sums to a common power is exact.  The terms and
+// the sum of a vector's are 32-bit (the logsumexp is right to 2^-21), what is
+// summed from them is 64-bit.  Inside a row the order is the logits' own, so it
+// needs no arithmetic; join_kernel orders the candidates of different beams by
+// totals in 64 bits, so that no further rounding to 32 decides between them.
 //
 // 32 requests of 8 beams over 128,256 ids, bf16 (66 MB): chunks 27 us, 2.4 TB/s,
 // in two rounds of four workgroups a CU that each load, sort and collect in
@@ -26,7 +27,7 @@ namespace tgs {
 namespace beam {
 
 // 2^x by the hardware instruction; results below 2^-126 are 0, next to a sum
-// of at least 1.
+// that holds its maximum's own term, 2^-0.5 or more.
 __device__ __forceinline__ float exp2_hw(float x) {
 #if defined(__HIP_DEVICE_COMPILE__)
   return __builtin_amdgcn_exp2f(x);
@@ -56,9 +57,21 @@ __device__ __forceinline__ uint4 again(uint4 x) {
 
 constexpr float NEG = -__builtin_inff();
 constexpr float NO_BASE = -1e30f;  // (the exponent of a sum of nothing)
+constexpr double LN2 = 0.69314718055994530942;
+
+// Logits of a magnitude beyond this (masks by large finite numbers) are far: a
+// whole number of 32 bits cannot stand for x log2 e there, or not closely.  A
+// wave that holds a far maximum takes its terms as e^(x - maximum) instead, and
+// its sum is handed on negative, with the maximum in the exponent's place.
+constexpr float FAR = 4194304.0f;
 
 // x 2^e for a whole e <= 0; 0 far below.
 __device__ __forceinline__ double scaled(double x, float e) { return __builtin_ldexp(x, (int)fmaxf(e, -4000.0f)); }
+
+// The natural logarithm of a sum and its base as they are handed on.
+__device__ __forceinline__ double log_sum(double base, double sum) {
+  return sum < 0.0 ? base + log(-sum) : sum == 0.0 ? -__builtin_inf() : base * LN2 + log(sum);
+}
 
 // Workgroup (row, chunk): ids [c L, min(V, (c + 1) L)), NVT vectors a thread.
 template <typename Tin, int NVT>
@@ -119,13 +132,24 @@ __global__ __launch_bounds__(BEAM_NT, 4) void chunk_kernel(BeamArgs a) {
     each([&](float x, int) { sum += x > NEG ? (double)term(x) : 0.0; });
   }
   if (sum == 0.0) base = NO_BASE;
-  const float wbase = wave_maxf(base);
+  float wbase = wave_maxf(base);
+  bool far = false;
+  if (__ballot(some && fabsf(tm) > FAR)) {
+    wbase = wave_maxf(tm);
+    far = fabsf(wbase) > FAR && wbase < -NEG;
+    base = far ? wbase : __builtin_rintf(wbase * L2H);
+    sum = 0.0;
+    each([&](float x, int) {
+      if (x > NEG) sum += (double)(far ? exp2_hw((x - base) * L2H) : term(x));
+    });
+    wbase = base;
+  }
   sum = scaled(sum, base - wbase);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if (lane_id() == 0) {
     s.base[w] = wbase;
-    s.sum[w] = sum;
+    s.sum[w] = far ? -sum : sum;
   }
   __syncthreads();
   uint32_t top = s.top[0][lane_id()];
@@ -178,12 +202,22 @@ __global__ __launch_bounds__(BEAM_NT, 4) void chunk_kernel(BeamArgs a) {
     if (lane < a.n) a.lists[(long long)blockIdx.x * a.n + lane] = best;
     if (lane == 0) {
       float b = s.base[0];
+      bool far = s.sum[0] < 0.0;
 #pragma unroll
-      for (int i = 1; i < BEAM_NT / 64; i++) b = fmaxf(b, s.base[i]);
-      double t = 0.0;
+      for (int i = 1; i < BEAM_NT / 64; i++) {
+        b = fmaxf(b, s.base[i]);
+        far |= s.sum[i] < 0.0;
+      }
+      double at = (double)b, t = 0.0;
+      if (far) {
+        at = -__builtin_inf();
+        for (int i = 0; i < BEAM_NT / 64; i++) at = fmax(at, log_sum((double)s.base[i], s.sum[i]));
+        for (int i = 0; i < BEAM_NT / 64; i++) t -= exp(log_sum((double)s.base[i], s.sum[i]) - at);
+      } else {
 #pragma unroll
-      for (int i = 0; i < BEAM_NT / 64; i++) t += scaled(s.sum[i], s.base[i] - b);
-      a.sums[2 * (long long)blockIdx.x] = (double)b;
+        for (int i = 0; i < BEAM_NT / 64; i++) t += scaled(s.sum[i], s.base[i] - b);
+      }
+      a.sums[2 * (long long)blockIdx.x] = at;
       a.sums[2 * (long long)blockIdx.x + 1] = t;
     }
   }
@@ -210,7 +244,7 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(BeamArgs a) {
     const u64* lists = a.lists + row * a.S * n;
     const double* sums = a.sums + row * a.S * 2;
     const float score = a.scores[row];
-    const float m = lane < a.S ? (float)sums[2 * lane] : NO_BASE;
+    const double base = lane < a.S ? sums[2 * lane] : (double)NO_BASE;
     double t = lane < a.S ? sums[2 * lane + 1] : 0.0;
     const int per = 64 / n, li = lane / n;  // lists a batch; the lane's list and entry
     u64 best = 0ull;
@@ -219,11 +253,22 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(BeamArgs a) {
       if (per > 1) x = wave_sort_desc(x);
       best = i == 0 ? x : wave_merge_top64(best, x);
     }
-    const float top = wave_maxf(m);
-    t = scaled(t, m - top);
+    double top;
+    const bool far = __ballot(t < 0.0) != 0;
+    if (far) {
+      const double x = log_sum(base, t);
+      top = x;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) top = fmax(top, __shfl_xor(top, o, 64));
+      t = exp(x - top);
+    } else {
+      const float m = (float)base, mt = wave_maxf(m);
+      t = scaled(t, m - mt);
+      top = (double)mt * LN2;
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o, 64);
-    const double lse = (double)top * 0.69314718055994530942 + log(t);
+    const double lse = top + log(t);
     // a beam that has ended (its score not a number above -inf), or whose row
     // holds +inf or nothing, has no candidates
     const bool live = __builtin_isfinite(score) && __builtin_isfinite(lse);

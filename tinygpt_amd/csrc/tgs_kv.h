@@ -78,7 +78,7 @@ struct BeamArgs {
   int* out_hist_len;
   int S, L;                   // chunks per row, ids per chunk (whole vectors)
   unsigned long long* lists;  // [G * W * S][n] largest composites of each chunk, 0 padded
-  double* sums;               // [G * W * S][2] maximum and sum of exp(x - maximum)
+  double* sums;               // [G * W * S][2] e and the sum of 2^(x log2 e - e), or m and minus the sum of e^(x - m)
 };
 int beam_chunk_ids(int dtype);
 hipError_t launch_beam(const BeamArgs& a, int dtype, hipStream_t st);
