@@ -380,8 +380,9 @@ int tgs_tree_commit(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* 
  * blocks of eight).  Free are the pages of the pool that no row names any
  * more, so the pool must belong to these rows alone.
  *   d_tables_out [B][width]: -1 past the slots in use; d_lens_out [B]
- * A parent outside [0, B) gives an empty row (its pages become free); a row
- * that finds no free page, or whose table has no slots for its room, gets the length -1.
+ * A parent outside [0, B) gives an empty row (its pages become free).  A row
+ * for whose needs too few free pages are left by the rows ahead of it gets none
+ * and the length -1, and so a row whose table has no slots for its room.
  * Outputs must not overlap inputs. */
 int tgs_kv_fork(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_seqs* seqs, const int32_t* d_parents, int room,
                 int32_t* d_tables_out, int32_t* d_lens_out, tgs_stream stream);

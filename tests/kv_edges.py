@@ -65,3 +65,81 @@ def check_beam(got, want, x):
     assert torch.equal(fin, torch.isfinite(got["scores"]))
     err = (got["scores"].double() - w).abs()
     assert (err <= w.abs() * 2**-24 + 2**-21 + 4 * top * 2**-53)[fin].all(), float(err[fin].max())
+
+
+# ------------------------------------------------------------------ forks
+
+def fork(k, v, tabs, lens, parents, room):
+    """Forks in plain form: pages are given to rows in order, to a row all that it needs or none."""
+    k, v = k.clone(), v.clone()
+    R, P = tabs.shape
+    N, page = k.shape[1], k.shape[3]
+    to, out = torch.full((R, P), -1, dtype=torch.int32), torch.zeros(R, dtype=torch.int32)
+    rows = []
+    for r in range(R):
+        p = int(parents[r])
+        n = int(lens[p]) if 0 <= p < R else -1
+        rows.append((tabs[p].tolist(), n, n // page, min((n + room + page - 1) // page, P)) if 0 <= n <= P * page else None)
+    shared = {x for row in rows if row for x in row[0][:row[2]]}
+    writer = {}
+    for r, row in enumerate(rows):
+        for i in range(row[2], row[3]) if row else ():
+            if 0 <= row[0][i] < N and row[0][i] not in shared:
+                writer.setdefault(row[0][i], (r, i))
+    free = [x for x in range(N) if x not in shared and x not in writer]
+    for r, row in enumerate(rows):
+        if row is None:
+            continue
+        t, n, full, end = row
+        to[r, :full] = torch.tensor(t[:full], dtype=torch.int32)
+        fresh = [i for i in range(full, end) if writer.get(t[i]) != (r, i)]
+        fits = len(fresh) <= len(free)
+        for i in range(full, end):
+            if i not in fresh:
+                to[r, i] = t[i]
+            elif fits:
+                to[r, i] = new = free.pop(0)
+                if 0 <= t[i] < N:
+                    blocks = (min(max(n - i * page, 0), page) + 7) // 8
+                    k[:, new, :, : blocks * 8] = k[:, t[i], :, : blocks * 8].clone()
+                    v[:, new, :, :blocks] = v[:, t[i], :, :blocks].clone()
+        out[r] = n if fits and n + room <= P * page else -1
+    return k, v, to, out
+
+
+def fork_case(tabs, lens, parents, pages, L=1, H=1, page=8, D=16, dt=BF16, seed=0):
+    g = gen(seed)
+    k = torch.randn(L, pages, H, page, D, generator=g).to(dt)
+    v = torch.randn(L, pages, H, page // 8, D, 8, generator=g).to(dt)
+    return k, v, *(torch.tensor(x, dtype=torch.int32) for x in (tabs, lens, parents))
+
+
+# (the case, room, the expected tables and lengths): pools that run out
+SHORT_POOLS = {
+    # rows 1 and 3 find no page; row 2 keeps its own
+    "kept": (fork_case([[0, 1], [0, 1], [2, 3], [2, 3]], [12] * 4, [0, 0, 2, 2], 4), 1,
+             [[0, 1], [0, -1], [2, 3], [2, -1]], [12, -1, 12, -1]),
+    # row 1 would take two pages of the one there is: row 3 gets it, and row 2, whose page no one writes to, needs none
+    "smaller": (fork_case([[0, 1, 2], [0, 1, 2], [3, 4, -1], [3, 4, -1]], [12, 12, 12, 12], [0, 0, 2, 2], 6), 9,
+                [[0, 1, 2], [0, -1, -1], [3, 4, 5], [3, -1, -1]], [12, -1, 12, -1]),
+    # row 0 would take two of the one free page, row 2 takes it
+    "later": (fork_case([[0, -1, -1], [2, 3, -1], [2, 3, -1]], [8, 12, 12], [0, 1, 1], 4), 9,
+              [[0, -1, -1], [2, 3, 1], [2, -1, -1]], [-1, 12, -1]),
+    # nothing to copy and no page for the room
+    "no room": (fork_case([[0], [1]], [8, 8], [0, 1], 2), 0, [[0], [1]], [8, 8]),
+}
+
+
+def many_short_rows(R=1100, seed=3):
+    """More rows than the planning workgroup has threads, in requests of four, and fewer pages than they need."""
+    g = gen(seed)
+    need = R // 4 * 4
+    lens = torch.randint(1, 24, (R // 4,), generator=g).repeat_interleave(4)
+    tabs = torch.full((need, 4), -1, dtype=torch.int32)
+    at = 0
+    for r in range(0, need, 4):
+        n = (int(lens[r]) + 7) // 8
+        tabs[r:r + 4, :n] = torch.arange(at, at + n, dtype=torch.int32)
+        at += n
+    parents = torch.arange(need) // 4 * 4 + torch.randint(0, 4, (need,), generator=g)
+    return *fork_case(tabs.tolist(), lens.tolist(), parents.tolist(), at + R // 2, page=8, D=8), 9

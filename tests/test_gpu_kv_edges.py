@@ -30,3 +30,29 @@ def test_beam_large_logits(sampler, dt):
     got = sampler.beam_select(dev(x), scores.to(DEV), 2, 6)
     torch.cuda.synchronize()
     E.check_beam(cpu(got), C.beam(x, scores, 2, 6), x)
+
+
+# ------------------------------------------------------------------ forks
+
+def run_fork(sampler, case, room):
+    H.log(f"fork rows={case[2].shape[0]} pages={case[0].shape[1]} room={room}")
+    k, v = dev(case[0]), dev(case[1])
+    t1, l1 = sampler.kv_fork(k, v, *(dev(x) for x in case[2:]), room=room)
+    torch.cuda.synchronize()
+    k2, v2, t2, l2 = E.fork(*case, room)
+    assert torch.equal(t1.cpu(), t2) and torch.equal(l1.cpu(), l2) and torch.equal(k.cpu(), k2) and torch.equal(v.cpu(), v2)
+    return t1.tolist(), l1.tolist()
+
+
+@pytest.mark.parametrize("name", list(E.SHORT_POOLS))
+@pytest.mark.parametrize("layers", [1, 200])
+def test_fork_short_pools(sampler, name, layers):
+    (k, v, *rest), room, tabs, lens = E.SHORT_POOLS[name]
+    case = (k.repeat(layers, 1, 1, 1, 1), v.repeat(layers, 1, 1, 1, 1, 1), *rest)
+    assert run_fork(sampler, case, room) == (tabs, lens)
+
+
+def test_fork_short_pool_of_many_rows(sampler):
+    case = E.many_short_rows()
+    _, lens = run_fork(sampler, case[:5], case[5])
+    assert -1 in lens[:1024] and max(lens[lens.index(-1):1024]) > 0

@@ -27,3 +27,28 @@ def test_beam_large_logits(sim, dt):  # noqa: F811
     rc, got = C.sim_beam(sim, x, scores, 2, 6)
     assert rc == 0
     E.check_beam(got, C.beam(x, scores, 2, 6), x)
+
+
+# ------------------------------------------------------------------ forks
+
+def run_fork(sim, case, room):  # noqa: F811
+    """The simulation's tables and lengths; they and the pools are the plain form's."""
+    rc, k1, v1, t1, l1 = C.sim_fork(sim, *case, room)
+    k2, v2, t2, l2 = E.fork(*case, room)
+    assert rc == 0 and torch.equal(t1, t2) and torch.equal(l1, l2) and torch.equal(k1, k2) and torch.equal(v1, v2)
+    return t1.tolist(), l1.tolist()
+
+
+@pytest.mark.parametrize("name", list(E.SHORT_POOLS))
+@pytest.mark.parametrize("layers", [1, 4])
+def test_fork_short_pools(sim, name, layers):  # noqa: F811
+    """Rows that need no page, or no more than are left, go on when the pool has run out for others."""
+    (k, v, *rest), room, tabs, lens = E.SHORT_POOLS[name]
+    case = (k.repeat(layers, 1, 1, 1, 1), v.repeat(layers, 1, 1, 1, 1, 1), *rest)
+    assert run_fork(sim, case, room) == (tabs, lens)
+
+
+def test_fork_short_pool_of_many_rows(sim):  # noqa: F811
+    case = E.many_short_rows()
+    _, lens = run_fork(sim, case[:5], case[5])
+    assert -1 in lens[:1024] and max(lens[lens.index(-1):1024]) > 0

@@ -162,7 +162,8 @@ __global__ __launch_bounds__(KV_NT) void write_kernel(KvWriteArgs a) {
 // writer.  A page that no row holds in full stays with the first row (in row,
 // then slot order) that names it there; the others get free pages, handed out
 // in ascending order to rows and slots in order, and copy what their parent's
-// page holds.  A page is free when no new row names it.
+// page holds.  A page is free when no new row names it.  Where they are too few,
+// a row gets all that it needs or none, and the rows behind it what is left.
 
 constexpr int OWNER_FREE = 0x7FFFFFFF;  // else the first row * P + slot that writes to the page, or -1: shared
 
@@ -174,6 +175,8 @@ __device__ __forceinline__ int owner_get(const int* o, int p) {
 
 struct PlanShared {
   int wave[KV_PLAN_NT / 64];
+  int at[KV_PLAN_NT];  // rows' needs, then the first free page of each (-1: too few left)
+  int given;
   int4 copy;
 };
 
@@ -261,9 +264,25 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
     }
     int total;
     int next = base + block_excl(need, s, total);
-    base += total;
+    if (total <= n_free - base) {
+      base += total;
+    } else {
+      s.at[tid] = need;
+      __syncthreads();
+      if (tid == 0) {
+        for (int i = 0; i < KV_PLAN_NT; i++) {
+          const int x = s.at[i];
+          s.at[i] = x <= n_free - base ? base : -1;
+          if (x <= n_free - base) base += x;
+        }
+        s.given = base;
+      }
+      __syncthreads();
+      next = s.at[tid];
+      base = s.given;
+    }
     if (r >= a.R) continue;
-    const bool fits = next + need <= n_free;
+    const bool fits = next >= 0;
     int* to_row = a.tables_out + (long long)r * P;
     int4 copy = make_int4(-1, -1, 0, 0);
     for (int i = w.full; i < w.end; i++) {
