@@ -70,7 +70,8 @@ def check_beam(got, want, x):
 # ------------------------------------------------------------------ forks
 
 def fork(k, v, tabs, lens, parents, room):
-    """Forks in plain form: pages are given to rows in order, to a row all that it needs or none."""
+    """Forks in plain form: pages are given to rows in order, to a row all that it needs or none.  A row with tokens in
+    a slot that names no page of the pool is given none and fails."""
     k, v = k.clone(), v.clone()
     R, P = tabs.shape
     N, page = k.shape[1], k.shape[3]
@@ -93,13 +94,14 @@ def fork(k, v, tabs, lens, parents, room):
         t, n, full, end = row
         to[r, :full] = torch.tensor(t[:full], dtype=torch.int32)
         fresh = [i for i in range(full, end) if writer.get(t[i]) != (r, i)]
-        fits = len(fresh) <= len(free)
+        bad = any(not 0 <= x < N for x in t[: (n + page - 1) // page])
+        fits = len(fresh) <= len(free) and not bad
         for i in range(full, end):
             if i not in fresh:
                 to[r, i] = t[i]
             elif fits:
                 to[r, i] = new = free.pop(0)
-                if 0 <= t[i] < N:
+                if n > i * page:
                     blocks = (min(max(n - i * page, 0), page) + 7) // 8
                     k[:, new, :, : blocks * 8] = k[:, t[i], :, : blocks * 8].clone()
                     v[:, new, :, :blocks] = v[:, t[i], :, :blocks].clone()
@@ -127,6 +129,21 @@ SHORT_POOLS = {
               [[0, -1, -1], [2, 3, 1], [2, -1, -1]], [-1, 12, -1]),
     # nothing to copy and no page for the room
     "no room": (fork_case([[0], [1]], [8, 8], [0, 1], 2), 0, [[0], [1]], [8, 8]),
+}
+
+
+# (the case, room, the expected tables and lengths): slots that hold tokens and name no page of the pool
+BAD_ENTRIES = {
+    # a partly filled page: the row's parent would give NaN and not be appended to, and the row must not look sound
+    "partial": (fork_case([[0, 99, -1], [1, 2, -1]], [12, 12], [0, 1], 8), 5, [[0, -1, -1], [1, 2, 3]], [-1, 12]),
+    "no page": (fork_case([[0, -1, -1]], [12], [0], 8), 1, [[0, -1, -1]], [-1]),
+    "below 0": (fork_case([[0, -7, -1]], [9], [0], 8), 1, [[0, -1, -1]], [-1]),
+    "full": (fork_case([[8, 5, -1], [0, 1, -1]], [12, 12], [0, 1], 8), 9, [[8, 5, -1], [0, 1, 2]], [-1, 12]),
+    # rows of one bad parent take none of the two free pages
+    "children": (fork_case([[0, 77], [1, 2], [1, 2], [3, 4]], [12, 12, 12, 12], [0, 0, 1, 1], 4), 1,
+                 [[0, -1], [0, -1], [1, 2], [1, 3]], [-1, -1, 12, 12]),
+    # an entry that holds no tokens is not looked at
+    "unused": (fork_case([[0, 99], [1, -5]], [8, 8], [0, 1], 8), 3, [[0, 2], [1, 3]], [8, 8]),
 }
 
 

@@ -56,3 +56,17 @@ def test_fork_short_pool_of_many_rows(sampler):
     case = E.many_short_rows()
     _, lens = run_fork(sampler, case[:5], case[5])
     assert -1 in lens[:1024] and max(lens[lens.index(-1):1024]) > 0
+
+
+@pytest.mark.parametrize("name", list(E.BAD_ENTRIES))
+@pytest.mark.parametrize("spare", [0, 20000])
+def test_fork_entries_outside_the_pool(sampler, name, spare):
+    """Reported by the length -1 (spare: pages of no row, so many that the plan's lists lie in the workspace)."""
+    (k, v, t, n, p), room, tabs, lens = E.BAD_ENTRIES[name]
+    if spare:
+        k = torch.cat([k, k.new_zeros(1, spare, *k.shape[2:])], 1)
+        v = torch.cat([v, v.new_zeros(1, spare, *v.shape[2:])], 1)
+        t = torch.where(t >= 8, t + spare, t)
+        tabs = [[x + spare if x >= 8 else x for x in row] for row in tabs]
+    case = (k, v, t, n, p)
+    assert run_fork(sampler, case, room) == (tabs, lens)

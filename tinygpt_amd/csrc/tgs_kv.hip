@@ -163,7 +163,8 @@ __global__ __launch_bounds__(KV_NT) void write_kernel(KvWriteArgs a) {
 // then slot order) that names it there; the others get free pages, handed out
 // in ascending order to rows and slots in order, and copy what their parent's
 // page holds.  A page is free when no new row names it.  Where they are too few,
-// a row gets all that it needs or none, and the rows behind it what is left.
+// a row gets all that it needs or none, and the rows behind it what is left.  A
+// row with tokens in a slot that names no page of the pool is given none.
 
 constexpr int OWNER_FREE = 0x7FFFFFFF;  // else the first row * P + slot that writes to the page, or -1: shared
 
@@ -175,7 +176,7 @@ __device__ __forceinline__ int owner_get(const int* o, int p) {
 
 struct PlanShared {
   int wave[KV_PLAN_NT / 64];
-  int at[KV_PLAN_NT];  // rows' needs, then the first free page of each (-1: too few left)
+  int at[KV_PLAN_NT];  // whether rows are bad (LDS), their needs, the first free page of each (-1: too few left)
   int given;
   int4 copy;
 };
@@ -231,12 +232,22 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
   __syncthreads();
   for (int r = tid >> 6; r < a.R; r += KV_PLAN_NT / 64) {
     const ForkRow w = row_of(r);
-    if (w.par < 0) continue;
-    const int* t = a.tables + (long long)w.par * P;
+    const int* t = a.tables + (long long)(w.par < 0 ? 0 : w.par) * P;
+    bool bad = false;
     for (int i = lane_id(); i < w.end; i += 64) {
       const int p = t[i];
-      if ((unsigned)p < (unsigned)N) atomicMin(&owner[p], i < w.full ? -1 : r * P + i);
+      if ((unsigned)p < (unsigned)N)
+        atomicMin(&owner[p], i < w.full ? -1 : r * P + i);
+      else
+        bad |= (long long)i << a.page_shift < w.len;
       if (out && i < w.full) a.tables_out[(long long)r * P + i] = p;
+    }
+    bad = __ballot(bad) != 0;
+    if (lane_id() == 0) {
+      if constexpr (LDS)
+        s.at[r] = bad;
+      else
+        a.copies[r].w = bad;
     }
   }
   if (!LDS) __threadfence();
@@ -257,8 +268,9 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
     const int r = r0 + tid;
     const ForkRow w = r < a.R ? row_of(r) : ForkRow{-1, 0, 0, 0};
     const int* t = a.tables + (long long)(w.par < 0 ? 0 : w.par) * P;
+    const bool bad = r < a.R && (LDS ? s.at[tid] : a.copies[r].w) != 0;
     int need = 0;
-    for (int i = w.full; i < w.end; i++) {
+    for (int i = w.full; i < w.end && !bad; i++) {
       const int p = t[i];
       need += !((unsigned)p < (unsigned)N && owner_get<LDS>(owner, p) == r * P + i);
     }
@@ -282,24 +294,23 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
       base = s.given;
     }
     if (r >= a.R) continue;
-    const bool fits = next >= 0;
+    const bool fits = next >= 0 && !bad;
     int* to_row = a.tables_out + (long long)r * P;
     int4 copy = make_int4(-1, -1, 0, 0);
     for (int i = w.full; i < w.end; i++) {
       const int p = t[i];
-      const bool named = (unsigned)p < (unsigned)N;
       int to = p;
-      if (!(named && owner_get<LDS>(owner, p) == r * P + i)) {
+      if (!((unsigned)p < (unsigned)N && owner_get<LDS>(owner, p) == r * P + i)) {
         to = fits ? fresh[next++] : -1;
         const int held = w.len - (i << a.page_shift);
-        if (held > 0 && named && fits) copy = make_int4(p, to, (held + 7) >> 3, 0);
+        if (held > 0 && fits) copy = make_int4(p, to, (held + 7) >> 3, 0);
       }
       if (out) to_row[i] = to;
     }
     if (r == want) s.copy = copy;
     if (!out) continue;
     if (want < 0) a.copies[r] = copy;
-    // -1: the pool ran out of pages
+    // -1: the pool ran out of pages, or the row is bad
     a.lens_out[r] = w.par < 0 ? 0 : fits && (long long)w.len + a.room <= ((long long)P << a.page_shift) ? w.len : -1;
   }
   if (!out) return;
