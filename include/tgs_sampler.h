@@ -383,7 +383,9 @@ int tgs_tree_commit(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* 
  * A parent outside [0, B) gives an empty row (its pages become free).  A row
  * for whose needs too few free pages are left by the rows ahead of it gets none
  * and the length -1, and so a row whose table has no slots for its room, and
- * a row with tokens in a slot that names no page of the pool.
+ * a row with tokens in a slot that names no page of the pool.  A row whose
+ * parent's length lies outside [0, width page] (-1: it failed before) gets -1
+ * and no slots (its pages become free).
  * Outputs must not overlap inputs. */
 int tgs_kv_fork(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_seqs* seqs, const int32_t* d_parents, int room,
                 int32_t* d_tables_out, int32_t* d_lens_out, tgs_stream stream);

@@ -71,7 +71,7 @@ def check_beam(got, want, x):
 
 def fork(k, v, tabs, lens, parents, room):
     """Forks in plain form: pages are given to rows in order, to a row all that it needs or none.  A row with tokens in
-    a slot that names no page of the pool is given none and fails."""
+    a slot that names no page of the pool is given none and fails; a length that is none stays a failure."""
     k, v = k.clone(), v.clone()
     R, P = tabs.shape
     N, page = k.shape[1], k.shape[3]
@@ -90,6 +90,7 @@ def fork(k, v, tabs, lens, parents, room):
     free = [x for x in range(N) if x not in shared and x not in writer]
     for r, row in enumerate(rows):
         if row is None:
+            out[r] = -1 if 0 <= int(parents[r]) < R else 0
             continue
         t, n, full, end = row
         to[r, :full] = torch.tensor(t[:full], dtype=torch.int32)
@@ -144,6 +145,17 @@ BAD_ENTRIES = {
                  [[0, -1], [0, -1], [1, 2], [1, 3]], [-1, -1, 12, 12]),
     # an entry that holds no tokens is not looked at
     "unused": (fork_case([[0, 99], [1, -5]], [8, 8], [0, 1], 8), 3, [[0, 2], [1, 3]], [8, 8]),
+}
+
+
+# (the case, room, the expected tables and lengths): lengths that are none, as an append, a commit or a fork before
+# returns them for rows that did not fit; the pages of such rows are free
+FAILED_LENGTHS = {
+    "failed": (fork_case([[0, 1], [2, 3], [4, 5]], [12, -1, 12], [1, 0, 1], 6), 1, [[-1, -1], [0, 1], [-1, -1]], [-1, 12, -1]),
+    "past the table": (fork_case([[0, 1], [2, 3]], [17, 16], [0, 1], 4), 0, [[-1, -1], [2, 3]], [-1, 16]),
+    "dead parents": (fork_case([[0, 1], [2, 3]], [-1, 9], [-1, 2], 4), 1, [[-1, -1], [-1, -1]], [0, 0]),
+    "pages go on": (fork_case([[0, 1], [2, 3], [2, 3]], [-1, 12, 12], [0, 1, 1], 4), 1,
+                    [[-1, -1], [2, 3], [2, 0]], [-1, 12, 12]),
 }
 
 

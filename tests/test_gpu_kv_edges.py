@@ -70,3 +70,10 @@ def test_fork_entries_outside_the_pool(sampler, name, spare):
         tabs = [[x + spare if x >= 8 else x for x in row] for row in tabs]
     case = (k, v, t, n, p)
     assert run_fork(sampler, case, room) == (tabs, lens)
+
+
+@pytest.mark.parametrize("name", list(E.FAILED_LENGTHS))
+def test_fork_failed_lengths(sampler, name):
+    """A row that failed before does not become an empty one."""
+    case, room, tabs, lens = E.FAILED_LENGTHS[name]
+    assert run_fork(sampler, case, room) == (tabs, lens)

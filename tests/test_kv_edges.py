@@ -66,3 +66,10 @@ def test_fork_entries_outside_the_pool(sim, name, spare):  # noqa: F811
         tabs = [[x + spare if x >= 8 else x for x in row] for row in tabs]
     case = (k, v, t, n, p)
     assert run_fork(sim, case, room) == (tabs, lens)
+
+
+@pytest.mark.parametrize("name", list(E.FAILED_LENGTHS))
+def test_fork_failed_lengths(sim, name):  # noqa: F811
+    """A row that failed before does not become an empty one."""
+    case, room, tabs, lens = E.FAILED_LENGTHS[name]
+    assert run_fork(sim, case, room) == (tabs, lens)

@@ -134,7 +134,8 @@ class CacheOps:
         tokens go to has one writer, the other rows get free pages of the pool
         (those that no row names any more) and copies.  Returns (tables_out
         [B, slots], lens_out [B]): -1 past the slots in use; length 0 for a
-        parent outside the rows, -1 for a row that found no page."""
+        parent outside the rows, -1 for a row that found no page, that names
+        none where it has tokens, or whose parent's length was -1."""
         if tables_out is None:
             tables_out = self._new(_torch().int32, *tables.shape)
         if lens_out is None:

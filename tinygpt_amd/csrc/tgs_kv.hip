@@ -199,12 +199,15 @@ __device__ __forceinline__ int block_excl(int x, PlanShared& s, int& total) {
 }
 
 // A new row: its parent, length and slots: shared [0, full), its own [full, end).
+// Without a parent (par -1) or of one whose length is none it has no slots, and
+// the length 0 or -1.
 struct ForkRow {
   int par, len, full, end;
 };
 __device__ __forceinline__ ForkRow fork_row(const KvForkArgs& a, int par, int len) {
   const long long cap = (long long)a.P << a.page_shift;
-  if (par < 0 || len < 0 || len > cap) return ForkRow{-1, 0, 0, 0};
+  if ((unsigned)par >= (unsigned)a.R) return ForkRow{-1, 0, 0, 0};
+  if (len < 0 || len > cap) return ForkRow{-1, -1, 0, 0};
   const long long end = ((long long)len + a.room + (1 << a.page_shift) - 1) >> a.page_shift;
   return ForkRow{par, len, len >> a.page_shift, end < a.P ? (int)end : a.P};
 }
@@ -311,7 +314,7 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
     if (!out) continue;
     if (want < 0) a.copies[r] = copy;
     // -1: the pool ran out of pages, or the row is bad
-    a.lens_out[r] = w.par < 0 ? 0 : fits && (long long)w.len + a.room <= ((long long)P << a.page_shift) ? w.len : -1;
+    a.lens_out[r] = w.par < 0 ? w.len : fits && (long long)w.len + a.room <= ((long long)P << a.page_shift) ? w.len : -1;
   }
   if (!out) return;
   for (int r = tid >> 6; r < a.R; r += KV_PLAN_NT / 64) {
