@@ -339,8 +339,9 @@ typedef struct {
  * ancestors and itself, q_heads / kv_heads query heads to a key head.  cache:
  * one layer (layers 1); head_dim 64, 96, 128 or 256; rows: the nodes' own
  * keys and values (layer strides unused), read beside the cache, not written
- * to it.  A sequence of which a page lies outside the pool gives NaN; lengths are taken
- * within [0, width page].  What the cache's pages hold past a sequence's end
+ * to it.  A sequence of which a page lies outside the pool gives NaN, and so one
+ * of the length -1 (an append, a commit or a fork of it failed); other lengths
+ * are taken within [0, width page].  What the cache's pages hold past a sequence's end
  * is never used.  Products and sums are 32-bit; softmax weights are rounded
  * to the cache's type before they multiply values.  Outputs must not overlap
  * inputs. */

@@ -2,7 +2,11 @@
 expected of them (shared by the CPU simulation's tests and the GPU's)."""
 from __future__ import annotations
 
+import math
+
 import torch
+
+import kv_cases as C
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
@@ -172,3 +176,22 @@ def many_short_rows(R=1100, seed=3):
         at += n
     parents = torch.arange(need) // 4 * 4 + torch.randint(0, 4, (need,), generator=g)
     return *fork_case(tabs.tolist(), lens.tolist(), parents.tolist(), at + R // 2, page=8, D=8), 9
+
+
+# ------------------------------------------------------------------ attention
+
+def failed_attention(T, dt=BF16):
+    """Inputs of five sequences, the second and the last of which failed before (length -1)."""
+    from test_kv_sim import attn_inputs
+
+    q, kn, vn, k, v, tabs, lens, par = attn_inputs(17, 5, T, 2, 1, 64, [40, 12, 0, 33, 20], 16, dt, slots=40)
+    lens[1], lens[4] = -1, -1
+    return q, kn, vn, k, v, tabs, lens, par
+
+
+def attention(args, scale=None):
+    """The plain form; NaN for a sequence of the length -1."""
+    q, kn, vn, k, v, tabs, lens, par = args
+    out, lse = C.attention(q, kn, vn, k, v, tabs, lens.clamp(min=0), par, q.shape[-1] ** -0.5 if scale is None else scale)
+    out[lens == -1], lse[lens == -1] = math.nan, math.nan
+    return out, lse

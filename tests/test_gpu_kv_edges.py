@@ -6,7 +6,7 @@ import torch
 import gpu_harness as H
 import kv_cases as C
 import kv_edges as E
-from test_gpu_kv import cpu, dev
+from test_gpu_kv import check_attn, cpu, dev
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -77,3 +77,23 @@ def test_fork_failed_lengths(sampler, name):
     """A row that failed before does not become an empty one."""
     case, room, tabs, lens = E.FAILED_LENGTHS[name]
     assert run_fork(sampler, case, room) == (tabs, lens)
+
+
+# ------------------------------------------------------------------ attention
+
+def run_attn(sampler, args, max_len=None):
+    q, kn, vn, k, v, tabs, lens, par = args
+    B, T, Hq, D = q.shape
+    H.log(f"attention B={B} T={T} Hq={Hq} Hkv={kn.shape[2]} D={D} lens={lens.tolist()[:4]} {q.dtype}")
+    lse = torch.empty(B, T, Hq, device=DEV)
+    out = sampler.tree_attention(*(dev(t) for t in args[:7]), parents=dev(par), max_len=max_len, lse=lse)
+    torch.cuda.synchronize()
+    want, want_lse = E.attention(args)
+    finite = [x.double()[torch.isfinite(x.double())].abs().max() for x in (vn, v)]
+    check_attn(out.cpu(), lse.cpu(), want, want_lse, float(max(finite)), q.dtype)
+
+
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_attention_of_failed_sequences(sampler, T):
+    run_attn(sampler, E.failed_attention(T))
+    run_attn(sampler, E.failed_attention(T), max_len=4000)

@@ -8,7 +8,7 @@ import torch
 
 import kv_cases as C
 import kv_edges as E
-from test_kv_sim import BF16, F16, F32, beam_inputs, gen, sim  # noqa: F401  (sim: a fixture)
+from test_kv_sim import BF16, F16, F32, attn_inputs, check_attn, sim  # noqa: F401  (sim: a fixture)
 
 
 # ------------------------------------------------------------------ beams
@@ -73,3 +73,21 @@ def test_fork_failed_lengths(sim, name):  # noqa: F811
     """A row that failed before does not become an empty one."""
     case, room, tabs, lens = E.FAILED_LENGTHS[name]
     assert run_fork(sim, case, room) == (tabs, lens)
+
+
+# ------------------------------------------------------------------ attention
+
+def run_attn(sim, args, **kw):  # noqa: F811
+    q, kn, vn, k, v, tabs, lens, par = args
+    rc, out, lse = C.sim_attention(sim, *args, **kw)
+    assert rc == 0
+    want, want_lse = E.attention(args)
+    finite = [x.double()[torch.isfinite(x.double())].abs().max() for x in (vn, v)]
+    check_attn(out, lse, want, want_lse, float(max(finite)), q.dtype)
+
+
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_attention_of_failed_sequences(sim, T):  # noqa: F811
+    """The length -1, by which an append, a commit or a fork reports a failure, gives NaN and no context of length 0."""
+    run_attn(sim, E.failed_attention(T))
+    run_attn(sim, E.failed_attention(T), num_cu=8, max_len=4000)

@@ -94,7 +94,8 @@ class CacheOps:
         v one layer's pools, tables int32 [B, slots], lens int32 [B], parents
         int32 [B, T] (an earlier node, -1: a root; None: a chain).  max_len:
         a bound of lens known on the host (sizes the launch), scale:
-        1 / sqrt(D) when None.  Returns out [B, T, q_heads, D]; lse float32
+        1 / sqrt(D) when None.  Returns out [B, T, q_heads, D] (NaN for a sequence
+        of the length -1 or with a page outside the pool); lse float32
         [B, T, q_heads], when given, gets the natural logsumexp of the scaled
         scores."""
         if out is None:

@@ -133,6 +133,10 @@ __device__ __forceinline__ void lds_barrier() {
 constexpr int NTILE = 32, WTILE = 64;  // tokens of a tile of the narrow and of the wide kernel
 constexpr float NEG = -__builtin_inff();
 
+// The length by which an append, a commit or a fork reports that rows did not
+// fit: such a sequence's rows become NaN.
+constexpr int FAILED = -1;
+
 // A query row's running state (maximum in units of log2, scaled) grows only
 // when a score passes it by more than SLACK: weights up to 2^SLACK keep their
 // relative precision in 16 bits and 32-bit sums, and most tiles skip the
@@ -149,10 +153,9 @@ __device__ __forceinline__ int clamp_len(const AttnArgs& a, int n) {
   const long long cap = (long long)a.P << a.page_shift;
   return n < 0 ? 0 : n > cap ? (int)cap : n;
 }
-__device__ __forceinline__ int seq_len(const AttnArgs& a, int b) { return uniform(clamp_len(a, a.lens[b])); }
 template <int TILE>
 __device__ __forceinline__ int cache_tiles(const AttnArgs& a, int b) {
-  return (seq_len(a, b) + TILE - 1) / TILE;
+  return (uniform(clamp_len(a, a.lens[b])) + TILE - 1) / TILE;
 }
 template <int TILE>  // (a sequence per lane)
 __device__ __forceinline__ int lane_tiles(const AttnArgs& a, int b) {

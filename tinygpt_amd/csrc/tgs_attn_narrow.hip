@@ -166,10 +166,11 @@ struct Narrow {
 
   // Tiles [t0, t1) of (b, h); full: they are all of it.  part: the workspace's rows otherwise.
   __device__ __forceinline__ void segment(Shared& s, int t0, int t1, bool full, long long part) {
-    len = seq_len(a, b);
+    const int given = uniform(a.lens[b]);
+    len = clamp_len(a, given);
     nc = (len + NTILE - 1) / NTILE;
     table = a.tables + (long long)b * a.P;
-    bad = false;
+    bad = given == FAILED;
     const int par = t1 > nc ? parent_of(a, b) : -1;
     Vec q[QT][KK];
 #pragma unroll

@@ -233,10 +233,11 @@ struct Wide {
   }
 
   __device__ __forceinline__ void segment(Shared& s, int t0, int t1, bool full, long long part) {
-    len = seq_len(a, b);
+    const int given = uniform(a.lens[b]);
+    len = clamp_len(a, given);
     nc = (len + WTILE - 1) / WTILE;
     table = a.tables + (long long)b * a.P;
-    bad = false;
+    bad = given == FAILED;
     const int row0 = qb * a.QB + wave * 32;  // of the M
     const bool work = row0 < a.M;
     const int i = row0 + col;
