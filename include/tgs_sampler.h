@@ -342,7 +342,8 @@ typedef struct {
  * to it.  A sequence of which a page lies outside the pool gives NaN, and so one
  * of the length -1 (an append, a commit or a fork of it failed); other lengths
  * are taken within [0, width page].  What the cache's pages hold past a sequence's end
- * is never used.  Products and sums are 32-bit; softmax weights are rounded
+ * is never used, and a drafted node's row, whatever it holds, reaches only the
+ * nodes that see it.  Products and sums are 32-bit; softmax weights are rounded
  * to the cache's type before they multiply values.  Outputs must not overlap
  * inputs. */
 int tgs_tree_attention(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs,

@@ -195,3 +195,39 @@ def attention(args, scale=None):
     out, lse = C.attention(q, kn, vn, k, v, tabs, lens.clamp(min=0), par, q.shape[-1] ** -0.5 if scale is None else scale)
     out[lens == -1], lse[lens == -1] = math.nan, math.nan
     return out, lse
+
+
+# shapes (T, q heads, kv heads, D, lens, page, type): both kernels, every count of waves and every kind of share
+UNSEEN = [(2, 1, 1, 64, [5, 0], 16, BF16), (8, 4, 2, 128, [70, 33], 16, F16), (16, 2, 1, 96, [40], 8, BF16),
+          (20, 2, 1, 64, [9], 16, BF16), (9, 4, 1, 96, [70], 16, F16), (64, 1, 1, 128, [30], 32, BF16),
+          (33, 8, 1, 64, [20], 16, F16), (20, 2, 1, 256, [40], 16, BF16), (6, 2, 1, 256, [33], 16, F16)]
+
+
+def unseen_garbage(T, Hq, Hkv, D, lens, page, dt, chain=False, slots=None):
+    """Drafted rows as a padded batch of trees holds them: nodes that others do not see with keys and values of NaN and
+    infinities (whole rows and single elements), and one of each among the values of nodes that others do see."""
+    from test_kv_sim import attn_inputs
+
+    q, kn, vn, k, v, tabs, lens, par = attn_inputs(T * D + 1, len(lens), T, Hq, Hkv, D, lens, page, dt, slots=slots)
+    par[:, T - 1] = 0  # leaves: the last nodes
+    vn[:, T - 1] = math.nan
+    kn[:, T - 1, :, ::3] = math.inf
+    if T > 4:
+        par[par == T - 2] = 0
+        vn[:, T - 2, :, 1::2] = math.inf
+        vn[:, T - 2, :, 2] = -math.inf
+        kn[:, T - 2] = math.nan
+        vn[:, 1, 0, 5] = math.nan
+        vn[:, 2, 0, 7] = -math.inf
+    return q, kn, vn, k, v, tabs, lens, None if chain else par
+
+
+def check_unseen(out, lse, args, check):
+    """Values that are no numbers reach the elements of the rows that see them, and nothing else."""
+    want, want_lse = attention(args)
+    huge = torch.isinf(want)
+    assert torch.equal(huge, torch.isinf(out)) and torch.equal(want[huge] > 0, out[huge] > 0)
+    # (check takes no infinities)
+    vn, v = args[2].double(), args[4].double()
+    vmax = max(float(x[torch.isfinite(x)].abs().max()) for x in (vn, v))
+    check(out.masked_fill(huge, 0), lse, want.masked_fill(huge, 0), want_lse, vmax, out.dtype)

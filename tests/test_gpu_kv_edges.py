@@ -97,3 +97,16 @@ def run_attn(sampler, args, max_len=None):
 def test_attention_of_failed_sequences(sampler, T):
     run_attn(sampler, E.failed_attention(T))
     run_attn(sampler, E.failed_attention(T), max_len=4000)
+
+
+@pytest.mark.parametrize("shape", [s[:-1] for s in E.UNSEEN] + [(6, 8, 2, 64, [3000, 7, 900], 16), (40, 4, 1, 128, [6000, 0], 16)], ids=str)
+@pytest.mark.parametrize("chain", [False, True])
+def test_attention_garbage_in_nodes_that_are_not_seen(sampler, shape, chain):
+    for dt in (E.BF16, E.F16):
+        args = E.unseen_garbage(*shape, dt, chain=chain)
+        q, kn, vn, k, v, tabs, lens, par = args
+        H.log(f"attention, garbage in unseen nodes {shape} {dt} chain={chain}")
+        lse = torch.empty(q.shape[:3], device=DEV)
+        out = sampler.tree_attention(*(dev(t) for t in args[:7]), parents=dev(par), lse=lse)
+        torch.cuda.synchronize()
+        E.check_unseen(out.cpu(), lse.cpu(), args, check_attn)

@@ -91,3 +91,21 @@ def test_attention_of_failed_sequences(sim, T):  # noqa: F811
     """The length -1, by which an append, a commit or a fork reports a failure, gives NaN and no context of length 0."""
     run_attn(sim, E.failed_attention(T))
     run_attn(sim, E.failed_attention(T), num_cu=8, max_len=4000)
+
+
+@pytest.mark.parametrize("shape", E.UNSEEN, ids=str)
+@pytest.mark.parametrize("chain", [False, True])
+def test_attention_garbage_in_nodes_that_are_not_seen(sim, shape, chain):  # noqa: F811
+    args = E.unseen_garbage(*shape, chain=chain)
+    rc, out, lse = C.sim_attention(sim, *args)
+    assert rc == 0
+    E.check_unseen(out, lse, args, check_attn)
+
+
+@pytest.mark.parametrize("shape", [(6, 2, 1, 64, [300, 7], 16, BF16), (40, 1, 1, 64, [600], 16, F16)], ids=str)
+def test_attention_garbage_in_shares(sim, shape):  # noqa: F811
+    """The same where the drafted nodes' part is joined with others."""
+    args = E.unseen_garbage(*shape)
+    rc, out, lse = C.sim_attention(sim, *args, num_cu=5)
+    assert rc == 0
+    E.check_unseen(out, lse, args, check_attn)

@@ -255,11 +255,63 @@ __device__ __forceinline__ u64 ancestors(const AttnArgs& a, int par) {
   return m;
 }
 
+// Lane `from`'s 64 bits.
+__device__ __forceinline__ u64 lane_bits(u64 m, int from) {
+  return ((u64)(uint32_t)__shfl((int)(m >> 32), from, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)m, from, 64);
+}
+
 // A mask of the first n of eight 16-bit values (n <= 0: none).
 __device__ __forceinline__ Vec first_of(int n) {
   const u64 lo = n >= 4 ? ~0ull : n <= 0 ? 0ull : (1ull << (16 * n)) - 1;
   const u64 hi = n >= 8 ? ~0ull : n <= 4 ? 0ull : (1ull << (16 * n - 64)) - 1;
   return vec16((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+}
+
+// A mask of the i-th of eight 16-bit values (i = 8: of none).
+__device__ __forceinline__ Vec only(int i) {
+  const uint32_t m = i & 1 ? 0xFFFF0000u : 0xFFFFu;
+  return vec16(i >> 1 == 0 ? m : 0u, i >> 1 == 1 ? m : 0u, i >> 1 == 2 ? m : 0u, i >> 1 == 3 ? m : 0u);
+}
+
+// A drafted value that is no finite number would reach the rows that do not see
+// its node as well, since 0 times it is NaN.  Where a drafted tile has such
+// values they are taken out of it and added to the rows that see them.
+// Of two 16-bit values: bits 15 and 31 of those that are not finite (a step of
+// the exponent carries out of it when all its bits are set).
+template <typename DT>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+  constexpr bool B = __is_same(DT, BF16);
+  return ((w & (B ? 0x7F807F80u : 0x7C007C00u)) + (B ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+template <typename DT>
+__device__ __forceinline__ uint32_t odd_bits(Vec x) {
+  return odd_bits<DT>(x[0]) | odd_bits<DT>(x[1]) | odd_bits<DT>(x[2]) | odd_bits<DT>(x[3]);
+}
+// Those values, and 0 for the others.
+template <typename DT>
+__device__ __forceinline__ Vec odd_of(Vec x) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t m = odd_bits<DT>(x[i]) >> 15;
+    x[i] &= (m << 16) - m;
+  }
+  return x;
+}
+// Elements d .. d + 3 of (b, h)'s drafted values: the sum of what is not finite
+// in the nodes of `sees`, 0 where all is.
+template <typename DT>
+__device__ __forceinline__ f32x4 odd_sum(const AttnArgs& a, int b, int h, u64 sees, int d) {
+  const uint16_t* p = (const uint16_t*)a.v_new + b * a.vn_b + h * a.vn_h + d;
+  f32x4 s = {0, 0, 0, 0};
+  for (int j = 0; j < a.T; j++, p += a.vn_t) {
+    if (!(sees >> j & 1)) continue;
+#pragma unroll
+    for (int z = 0; z < 4; z++) {
+      const uint32_t u = p[z], rest = u & (__is_same(DT, BF16) ? 0x7Fu : 0x3FFu);
+      if (odd_bits<DT>(u)) s[z] += tg_u2f((u & 0x8000u) << 16 | 0x7F800000u | (rest ? 0x400000u : 0u));
+    }
+  }
+  return s;
 }
 
 // x where bit i of bits is set, else -inf.

@@ -164,6 +164,30 @@ struct Narrow {
       for (int t = 0; t < QT; t++) s.o[t][d] = mfma16<DT>(v[d], p[t], s.o[t][d]);
   }
 
+  // Takes what is not finite out of the drafted tile's values, and adds it node
+  // by node to the rows that see the node.
+  __device__ __forceinline__ void add_odd(Vec (&v)[DT16], const Vec (&p)[QT], u64 anc, State& s) const {
+    u64 sees[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) sees[t] = lane_bits(anc, t * 16 + col < a.M ? (t * 16 + col) / a.G : 0);
+    for (int j = 0; j < a.T; j++) {
+      const Vec one = only(grp == j >> 3 ? j & 7 : 8);
+#pragma unroll
+      for (int d = 0; d < DT16; d++) {
+        const Vec x = odd_of<DT>(v[d]) & one;
+        if (__ballot((x[0] | x[1] | x[2] | x[3]) != 0) == 0) continue;
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          const f32x4 y = mfma16<DT>(x, p[t], f32x4{0, 0, 0, 0});
+#pragma unroll
+          for (int z = 0; z < 4; z++) s.o[t][d][z] += sees[t] >> j & 1 ? y[z] : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < DT16; d++) v[d] ^= odd_of<DT>(v[d]);
+  }
+
   // Tiles [t0, t1) of (b, h); full: they are all of it.  part: the workspace's rows otherwise.
   __device__ __forceinline__ void segment(Shared& s, int t0, int t1, bool full, long long part) {
     const int given = uniform(a.lens[b]);
@@ -238,17 +262,25 @@ struct Narrow {
       load_tree_values(x);
       load_tree_keys(k);
       const u64 anc = ancestors(a, par);  // of node `lane`
+      uint32_t odd = 0;
+      if (a.T > 1) {  // (one node: every row sees it)
+#pragma unroll
+        for (int n = 0; n < GO; n++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) odd |= odd_bits<DT>(x[n][j]);
+      }
       scores(k, q, sc);
       turn_tree((Vec*)s.o[wave], x, v);
 #pragma unroll
       for (int t = 0; t < QT; t++) {
         const int node = t * 16 + col < a.M ? (t * 16 + col) / a.G : 0;
-        const u64 sees = ((u64)(uint32_t)__shfl((int)(anc >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)anc, node, 64);
+        const u64 sees = lane_bits(anc, node);
         const uint32_t in = (uint32_t)(sees >> (grp * 8));
 #pragma unroll
         for (int j = 0; j < 8; j++) sc[t][j >> 2][j & 3] = seen(sc[t][j >> 2][j & 3], in, j);
       }
       weights(sc, st, p);
+      if (__ballot(odd != 0)) add_odd(v, p, anc, st);
       add(v, p, st);
     }
     // the waves' states

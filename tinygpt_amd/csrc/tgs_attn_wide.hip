@@ -28,6 +28,7 @@ struct Wide {
   struct Shared {
     Vec k[2][WTILE * C];
     Vec v[2][WTILE * C];
+    int odd[QW];  // whether what a wave brings of the drafted tile's values is not all finite
   };
 
   const AttnArgs& a;
@@ -140,6 +141,22 @@ struct Wide {
       const int c = n * NTHR + tid;
       if (EVEN || c < WTILE * C) s.k[1][at_key(c / C, c % C)] = k[n];
     }
+    int odd = 0;
+    if (a.T > 1) {  // (one node: every row sees it)
+      uint32_t bits = 0;
+#pragma unroll
+      for (int n = 0; n < TURN; n++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) bits |= odd_bits<DT>(v[n][j]);
+      odd = __ballot(bits != 0) != 0;
+      if (odd) {
+#pragma unroll
+        for (int n = 0; n < TURN; n++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[n][j] ^= odd_of<DT>(v[n][j]);
+      }
+    }
+    if (lane == 0) s.odd[wave] = odd;
 #pragma unroll
     for (int n = 0; n < TURN; n++) {
       const int c = n * NTHR + tid;
@@ -295,8 +312,7 @@ struct Wide {
     lds_barrier();
     if (drafted) {
       if (work) {
-        u64 sees = ancestors(a, par);
-        sees = ((u64)(uint32_t)__shfl((int)(sees >> 32), node, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)sees, node, 64);
+        const u64 sees = lane_bits(ancestors(a, par), node);
         scores(s, 1, q, sc);
         const u64 in = sees >> (8 * half);
         uint32_t bits = 0;
@@ -340,6 +356,26 @@ struct Wide {
           step(t + 1, 1, k0, v0);
       }
       if (t < tc) step(t, 0, k0, v0);
+    }
+    if (drafted) {
+      // What is not finite takes the place of a sum: no weight or addend that is
+      // finite changes it.  (s.odd is written again behind the next segment's
+      // first barrier.  The check costs 1 us of 34 for 16 sequences of 1000 to
+      // 3000 tokens and 48 rows of 128; adding at the drafted tile spills.)
+      int odd = 0;
+#pragma unroll
+      for (int w = 0; w < QW; w++) odd |= s.odd[w];
+      if (uniform(odd)) {
+        const u64 sees = lane_bits(ancestors(a, parent_of(a, b)), node);
+#pragma unroll
+        for (int d = 0; d < DT32; d++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            const f32x4 y = odd_sum<DT>(a, b, h, sees, d * 32 + x * 8 + half * 4);
+#pragma unroll
+            for (int z = 0; z < 4; z++) st.o[d][4 * x + z] = y[z] == 0.0f ? st.o[d][4 * x + z] : y[z];
+          }
+      }
     }
     float m = st.m, l = st.l;
     const f32x16(&o)[DT32] = st.o;
