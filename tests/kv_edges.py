@@ -231,3 +231,29 @@ def check_unseen(out, lse, args, check):
     vn, v = args[2].double(), args[4].double()
     vmax = max(float(x[torch.isfinite(x)].abs().max()) for x in (vn, v))
     check(out.masked_fill(huge, 0), lse, want.masked_fill(huge, 0), want_lse, vmax, out.dtype)
+
+
+def faint_tail(D, dt, n, page=32, T=1, Hq=1):
+    """One token in 32 far ahead of the others, whose weights are 2^-25.5 of its: it has the values 0 and they 1000, so
+    that the result is what they hold."""
+    N = (n + page - 1) // page
+    k = torch.zeros(N, 1, page, D, dtype=dt)
+    v = torch.full((N, 1, page // 8, D, 8), 1000.0).to(dt)
+    k[:, 0, 3] = 0.25
+    v[:, 0, 0, :, 3] = 0.0
+    q = torch.full((1, T, Hq, D), 4.0).to(dt)  # (products of D with it, and of 0)
+    kn, vn = torch.zeros(1, T, 1, D, dtype=dt), torch.full((1, T, 1, D), 1000.0).to(dt)
+    table = torch.arange(N, dtype=torch.int32)[None]
+    return (q, kn, vn, k, v, table, torch.tensor([n], dtype=torch.int32), None), 25.5 * math.log(2) / D
+
+
+def check_faint_tail(out, lse, args, scale):
+    """Half a step of each weight and of the result, and where weights are below the type's least normal number half a
+    step there, for weights held up to 2^9 of the largest: of tokens of 1000 over those ahead."""
+    want, want_lse = attention(args, scale)
+    half = torch.finfo(out.dtype).eps / 2
+    least = torch.finfo(out.dtype).tiny * half * 2.0**-9
+    tokens = int(args[6][0]) + out.shape[1]
+    bound = (2 * half + 2**-16) * want + least * 1000 * tokens / (int(args[6][0]) // 32)
+    assert ((out.double() - want).abs() <= bound).all(), (out.flatten()[0], want.flatten()[0])
+    assert ((lse.double() - want_lse).abs() <= 2**-18 * (1 + want_lse.abs())).all()

@@ -110,3 +110,14 @@ def test_attention_garbage_in_nodes_that_are_not_seen(sampler, shape, chain):
         out = sampler.tree_attention(*(dev(t) for t in args[:7]), parents=dev(par), lse=lse)
         torch.cuda.synchronize()
         E.check_unseen(out.cpu(), lse.cpu(), args, check_attn)
+
+
+@pytest.mark.parametrize("T,D,n", [(1, 128, 40000), (3, 256, 330), (40, 64, 9000), (36, 128, 200)])
+@pytest.mark.parametrize("dt", [E.BF16, E.F16])
+def test_attention_faint_tail(sampler, T, D, n, dt):
+    args, scale = E.faint_tail(D, dt, n, T=T)
+    H.log(f"attention of a faint tail T={T} D={D} n={n} {dt}")
+    lse = torch.empty(1, T, 1, device=DEV)
+    out = sampler.tree_attention(*(dev(t) for t in args[:7]), scale=scale, lse=lse)
+    torch.cuda.synchronize()
+    E.check_faint_tail(out.cpu(), lse.cpu(), args, scale)

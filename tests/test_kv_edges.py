@@ -109,3 +109,13 @@ def test_attention_garbage_in_shares(sim, shape):  # noqa: F811
     rc, out, lse = C.sim_attention(sim, *args, num_cu=5)
     assert rc == 0
     E.check_unseen(out, lse, args, check_attn)
+
+
+@pytest.mark.parametrize("T,D,n", [(1, 64, 600), (3, 256, 330), (40, 64, 700), (36, 128, 200)])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_attention_faint_tail(sim, T, D, n, dt):  # noqa: F811
+    """Weights far below the largest: fp16 holds them as well as half a step."""
+    args, scale = E.faint_tail(D, dt, n, T=T)
+    rc, out, lse = C.sim_attention(sim, *args, scale=scale)
+    assert rc == 0
+    E.check_faint_tail(out, lse, args, scale)

@@ -12,8 +12,8 @@
 // product's rows stand for are permuted such that a lane ends with eight
 // consecutive tokens, which is also one 16-byte vector of the values' layout.
 // No score goes through LDS or another lane.  The running maximum and sum are
-// 32-bit; P is rounded to the inputs' 16 bits (half a step of a weight in
-// [0, 1], the precision of the values it multiplies), O accumulates in 32.
+// 32-bit; P is rounded to the inputs' 16 bits (half a step of each weight, the
+// precision of the values it multiplies), O accumulates in 32.
 //
 // Work is cut by an even share of tiles per worker, not by sequence: worker w
 // of N takes tiles [w U / N, (w + 1) U / N) of the U tiles of all sequences
@@ -142,6 +142,13 @@ constexpr int FAILED = -1;
 // relative precision in 16 bits and 32-bit sums, and most tiles skip the
 // exchange between lanes and the scaling of O.
 constexpr float SLACK = 6.0f;
+
+// fp16 holds numbers below 2^-14 with fewer bits and none below 2^-25.  Its
+// weights are therefore relative to a maximum 2^9 lower: they reach 2^(9 + SLACK),
+// half of its largest number, and down to 2^-23 of the row's largest they
+// keep their precision.
+template <typename DT>
+constexpr float lift() { return __is_same(DT, BF16) ? 0.0f : 9.0f; }
 
 // ------------------------------------------------------------------ shares
 

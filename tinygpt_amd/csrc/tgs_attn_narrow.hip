@@ -135,7 +135,7 @@ struct Narrow {
       float top = sc[t][0][0];
 #pragma unroll
       for (int j = 1; j < 8; j++) top = fmaxf(top, sc[t][j >> 2][j & 3]);
-      top *= a.scale_log2;
+      top = top * a.scale_log2 - lift<DT>();
       if (__ballot(top > s.m[t] + SLACK)) {
         top = fmaxf(top, xor_lane<16>(top));
         top = fmaxf(top, xor_lane<32>(top));

@@ -208,7 +208,7 @@ struct Wide {
     for (int x = 0; x < 2; x++)
 #pragma unroll
       for (int j = 0; j < 16; j++) top = fmaxf(top, sc[x][j]);
-    top *= a.scale_log2;
+    top = top * a.scale_log2 - lift<DT>();
     if (__ballot(top > st.m + SLACK)) {
       top = fmaxf(top, xor_lane<32>(top));
       const float now = fmaxf(st.m, top);
