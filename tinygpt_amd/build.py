@@ -51,12 +51,14 @@ def hipcc() -> str:
     return "hipcc"
 
 
-def build_calls() -> subprocess.CompletedProcess:
-    """The checking module, to PY_OUT + ".tmp"."""
+def build_calls() -> subprocess.CompletedProcess | None:
+    """The checking module, to PY_OUT + ".tmp"; None without torch, which alone calls it."""
     import sysconfig
 
-    from torch.utils import cpp_extension as ext
-
+    try:
+        from torch.utils import cpp_extension as ext
+    except ImportError:
+        return None
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D_GLIBCXX_USE_CXX11_ABI=1",
            "-I" + sysconfig.get_paths()["include"], *["-I" + p for p in ext.include_paths()], os.path.join(CSRC, PY_SRC),
            "-o", PY_OUT + ".tmp", *["-L" + p for p in ext.library_paths()], "-ltorch_python", "-ltorch_cpu", "-lc10", "-ldl"]
@@ -64,7 +66,8 @@ def build_calls() -> subprocess.CompletedProcess:
 
 
 def build(verbose: bool = False) -> str:
-    """Compiles every source to an object in parallel, then links the library."""
+    """Compiles every source to an object in parallel, then links the library.  It is in place before a failure of the
+    checking module is raised: hosts without torch need only the library."""
     from concurrent.futures import ThreadPoolExecutor
 
     objdir = os.path.join(HERE, "_build")
@@ -80,9 +83,6 @@ def build(verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=min(8, len(SOURCES) + 2)) as ex:
         calls = ex.submit(build_calls)
         results = list(ex.map(compile_one, SOURCES + [FLOOR_SRC]))
-        calls = calls.result()
-    if calls.returncode != 0:
-        raise RuntimeError(f"{PY_SRC} failed ({calls.returncode}):\n{' '.join(calls.args)}\n{calls.stderr}")
     floor = results.pop()
     msgs = []
     for src, obj, cmd, r in results:
@@ -108,6 +108,15 @@ def build(verbose: bool = False) -> str:
         print("\n".join(msgs), file=sys.stderr)
     os.replace(tmp, OUT)
     os.replace(ftmp, FLOOR_OUT)
+    try:
+        r = calls.result()
+    except OSError as e:
+        raise RuntimeError(f"{PY_SRC}: {e}") from e
+    if r is None:
+        print(f"torch is not there: {PY_SRC}, the Python side's checks, is not built", file=sys.stderr)
+        return OUT
+    if r.returncode != 0:
+        raise RuntimeError(f"{PY_SRC} failed ({r.returncode}):\n{' '.join(r.args)}\n{r.stderr}")
     os.replace(PY_OUT + ".tmp", PY_OUT)
     return OUT
 
