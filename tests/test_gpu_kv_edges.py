@@ -6,7 +6,7 @@ import torch
 import gpu_harness as H
 import kv_cases as C
 import kv_edges as E
-from test_gpu_kv import check_attn, cpu, dev
+from test_gpu_kv import check_attn, cpu, dev, write_inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -121,3 +121,20 @@ def test_attention_faint_tail(sampler, T, D, n, dt):
     out = sampler.tree_attention(*(dev(t) for t in args[:7]), scale=scale, lse=lse)
     torch.cuda.synchronize()
     E.check_faint_tail(out.cpu(), lse.cpu(), args, scale)
+
+
+# ------------------------------------------------------------------ appends
+
+def test_append_of_few_of_many_rows(sampler):
+    """Rows of a shape whose blocks are more than a grid holds, of which the counts take a few."""
+    H.log("append, 140 million rows of which 21")
+    T = 140_000_000
+    kn, vn, k, v, tabs = write_inputs(5, 1, 2, 1, 1, 8, 8, 3, E.BF16)
+    lens = torch.tensor([3, 0], dtype=torch.int32)
+    counts = torch.tensor([21, 0], dtype=torch.int32)
+    kd, vd = dev(k), dev(v)
+    rows = [dev(x).expand(1, 2, T, 1, 8) for x in (kn, vn)]
+    l1 = sampler.kv_append(*rows, kd, vd, dev(tabs), dev(lens), counts=dev(counts))
+    torch.cuda.synchronize()
+    k2, v2, l2 = C.append(*(x.expand(1, 2, 21, 1, 8) for x in (kn, vn)), k, v, tabs, lens, counts)
+    assert torch.equal(kd.cpu(), k2) and torch.equal(vd.cpu(), v2) and torch.equal(l1.cpu(), l2)

@@ -8,7 +8,7 @@ import torch
 
 import kv_cases as C
 import kv_edges as E
-from test_kv_sim import BF16, F16, F32, attn_inputs, check_attn, sim  # noqa: F401  (sim: a fixture)
+from test_kv_sim import BF16, F16, F32, check_attn, sim, write_inputs  # noqa: F401  (sim: a fixture)
 
 
 # ------------------------------------------------------------------ beams
@@ -119,3 +119,15 @@ def test_attention_faint_tail(sim, T, D, n, dt):  # noqa: F811
     rc, out, lse = C.sim_attention(sim, *args, scale=scale)
     assert rc == 0
     E.check_faint_tail(out, lse, args, scale)
+
+
+# ------------------------------------------------------------------ appends
+
+def test_append_of_few_of_many_rows(sim):  # noqa: F811
+    """Rows of the largest shape, of which the counts take a few: the launch is sized by what the tables hold."""
+    T = 2**31 - 1
+    kn, vn, k, v, tabs = write_inputs(5, 1, 2, 1, 1, 8, 8, 3, BF16)
+    lens, counts = torch.tensor([3, 0], dtype=torch.int32), torch.tensor([21, 0], dtype=torch.int32)
+    rc, k1, v1, l1 = C.sim_append(sim, kn.expand(1, 2, T, 1, 8), vn.expand(1, 2, T, 1, 8), k, v, tabs, lens, counts)
+    k2, v2, l2 = C.append(*(x.expand(1, 2, 21, 1, 8) for x in (kn, vn)), k, v, tabs, lens, counts)
+    assert rc == 0 and torch.equal(k1, k2) and torch.equal(v1, v2) and torch.equal(l1, l2)

@@ -222,7 +222,8 @@ int tgs_kv_append(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* ro
   if (int rc = write_args(h, cache, rows, seqs, T, d_lens_out, a)) return rc;
   if (a.B == 0) return TGS_OK;
   a.counts = d_counts;
-  a.nblk = T == 1 ? 1 : (T + 7) / 8 + 1;
+  // blocks that T rows, or as many as a table holds, lie in at most
+  a.nblk = T == 1 ? 1 : (int)((std::min<int64_t>(T, (int64_t)a.P * cache->page) + 7) / 8 + 1);
   if ((int64_t)a.nblk * a.B * cache->layers > INT32_MAX) return fail(h, TGS_ETOOBIG, "rows");
   DeviceGuard g(h->device);
   if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
