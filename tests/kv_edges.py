@@ -257,3 +257,47 @@ def check_faint_tail(out, lse, args, scale):
     bound = (2 * half + 2**-16) * want + least * 1000 * tokens / (int(args[6][0]) // 32)
     assert ((out.double() - want).abs() <= bound).all(), (out.flatten()[0], want.flatten()[0])
     assert ((lse.double() - want_lse).abs() <= 2**-18 * (1 + want_lse.abs())).all()
+
+
+def named_tokens(B, T, G, Hkv, D, lens, page, dt, seed=0):
+    """A cache whose tokens have random keys and values of +-1: a query that is a token's key takes that token's value
+    alone.  Returns the pools, tables, lengths, the tokens' keys and values [B][Hkv, len, D], and drafted rows of 0."""
+    g = gen(seed)
+    P = max(1, max((n + page - 1) // page for n in lens))
+    tabs = torch.randperm(B * P + 2, generator=g)[: B * P].view(B, P).to(torch.int32)
+    k = torch.zeros(B * P + 2, Hkv, page, D, dtype=dt)
+    v = torch.zeros(B * P + 2, Hkv, page // 8, D, 8, dtype=dt)
+    keys, values = [], []
+    for b in range(B):
+        n = P * page
+        x, y = (torch.randint(0, 2, (Hkv, n, D), generator=g).mul(2).sub(1).to(dt) for _ in range(2))
+        for i in range(P):
+            k[tabs[b, i]] = x[:, i * page:(i + 1) * page]
+            v[tabs[b, i]] = y[:, i * page:(i + 1) * page].view(Hkv, page // 8, 8, D).transpose(2, 3)
+        keys.append(x)
+        values.append(y)
+    rows = torch.zeros(B, T, Hkv, D, dtype=dt)
+    return k, v, tabs, torch.tensor(lens, dtype=torch.int32), keys, values, rows
+
+
+def queries(keys, lens, T, G, first, step):
+    """Row i of a key head asks for token (first + step i) % len of its sequence: queries [B, T, Hkv G, D] and the tokens
+    [B, T, Hkv G]."""
+    B, (Hkv, _, D) = len(keys), keys[0].shape
+    t = torch.arange(T)[:, None, None] * G + torch.arange(G)[None, None] + 7 * torch.arange(Hkv)[None, :, None]
+    q, at = torch.zeros(B, T, Hkv, G, D, dtype=keys[0].dtype), []
+    for b in range(B):
+        tok = (first + step * t) % int(lens[b])
+        for h in range(Hkv):
+            q[b, :, h] = keys[b][h, tok[:, h]]
+        at.append(tok)
+    return q.view(B, T, Hkv * G, D), torch.stack(at)
+
+
+def check_named(out, at, values):
+    # the others' weights: a product at most 3/4 D of a token's own D at these sizes, so e^(-D / 4 scale) each
+    B, T, Hkv, G = at.shape
+    out = out.view(B, T, Hkv, G, -1)
+    for b in range(B):
+        for h in range(Hkv):
+            assert ((out[b, :, h].double() - values[b][h, at[b, :, h]].double()).abs() < 2**-7).all(), (b, h)

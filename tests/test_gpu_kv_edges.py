@@ -6,7 +6,7 @@ import torch
 import gpu_harness as H
 import kv_cases as C
 import kv_edges as E
-from test_gpu_kv import check_attn, cpu, dev, write_inputs
+from test_gpu_kv import attn_inputs, check_attn, cpu, dev, write_inputs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -138,3 +138,29 @@ def test_append_of_few_of_many_rows(sampler):
     torch.cuda.synchronize()
     k2, v2, l2 = C.append(*(x.expand(1, 2, 21, 1, 8) for x in (kn, vn)), k, v, tabs, lens, counts)
     assert torch.equal(kd.cpu(), k2) and torch.equal(vd.cpu(), v2) and torch.equal(l1.cpu(), l2)
+
+
+# ------------------------------------------------------------------ every token's value, many sequences
+
+@pytest.mark.parametrize("T,G,Hkv,D,lens", [
+    (1, 4, 2, 64, [5000, 64, 901]), (8, 4, 4, 128, [4096, 100, 2049, 1]), (5, 8, 2, 128, [9000, 5]), (63, 8, 1, 128, [6000, 2000]),
+    (40, 2, 2, 64, [3000, 3]), (7, 4, 1, 256, [2500]), (30, 4, 1, 256, [2500, 70]), (48, 1, 2, 96, [1900, 333])])
+@pytest.mark.parametrize("dt", [E.BF16, E.F16])
+def test_attention_takes_each_tokens_value(sampler, T, G, Hkv, D, lens, dt):
+    """Rows that ask for one token each, spread over every tile of the contexts."""
+    k, v, tabs, n, keys, values, rows = E.named_tokens(len(lens), T, G, Hkv, D, lens, 64, dt)
+    d = [dev(x) for x in (rows, rows, k, v, tabs, n)]
+    step = max(1, -(-max(lens) // (T * G)))  # (the rows of a call spread over the longest context)
+    for first in range(0, step, max(1, min(step // 3, 29))):
+        H.log(f"attention of named tokens T={T} G={G} D={D} lens={lens} first={first} {dt}")
+        q, at = E.queries(keys, n, T, G, first, step)
+        out = sampler.tree_attention(dev(q), *d, scale=2.0)
+        torch.cuda.synchronize()
+        E.check_named(out.cpu(), at, values)
+
+
+@pytest.mark.parametrize("B,T,Hq", [(130, 1, 1), (300, 5, 2), (70, 40, 1)])
+def test_attention_of_many_sequences(sampler, B, T, Hq):
+    lens = torch.randint(0, 90, (B,), generator=E.gen(B)).tolist()
+    lens[B - 4] = 1500
+    run_attn(sampler, attn_inputs(B, B, T, Hq, 1, 64, lens, 32, E.BF16))

@@ -8,7 +8,7 @@ import torch
 
 import kv_cases as C
 import kv_edges as E
-from test_kv_sim import BF16, F16, F32, check_attn, sim, write_inputs  # noqa: F401  (sim: a fixture)
+from test_kv_sim import BF16, F16, F32, attn_inputs, check_attn, sim, write_inputs  # noqa: F401  (sim: a fixture)
 
 
 # ------------------------------------------------------------------ beams
@@ -131,3 +131,22 @@ def test_append_of_few_of_many_rows(sim):  # noqa: F811
     rc, k1, v1, l1 = C.sim_append(sim, kn.expand(1, 2, T, 1, 8), vn.expand(1, 2, T, 1, 8), k, v, tabs, lens, counts)
     k2, v2, l2 = C.append(*(x.expand(1, 2, 21, 1, 8) for x in (kn, vn)), k, v, tabs, lens, counts)
     assert rc == 0 and torch.equal(k1, k2) and torch.equal(v1, v2) and torch.equal(l1, l2)
+
+
+# ------------------------------------------------------------------ every token's value, many sequences
+
+@pytest.mark.parametrize("T,G,D,lens", [(4, 2, 64, [300, 77]), (11, 3, 64, [290, 64])])
+def test_attention_takes_each_tokens_value(sim, T, G, D, lens):  # noqa: F811
+    k, v, tabs, n, keys, values, rows = E.named_tokens(2, T, G, 1, D, lens, 16, F16)
+    for first, step in ((0, 9), (5, 31)):
+        q, at = E.queries(keys, n, T, G, first, step)
+        rc, out, _ = C.sim_attention(sim, q, rows, rows, k, v, tabs, n, None, 2.0, num_cu=3)
+        assert rc == 0
+        E.check_named(out, at, values)
+
+
+def test_attention_of_many_sequences(sim):  # noqa: F811
+    """More sequences than a wave has lanes, in shares that start anywhere among them."""
+    lens = torch.randint(0, 60, (70,), generator=E.gen(2)).tolist()
+    lens[66] = 290
+    run_attn(sim, attn_inputs(70, 70, 1, 1, 1, 64, lens, 32, BF16), num_cu=9)
