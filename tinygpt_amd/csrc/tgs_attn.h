@@ -539,7 +539,12 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
   if (a.lse && sub == 0) a.lse[out] = row_lse(m, l);
 }
 
-// Few rows: one a workgroup, so that their parts are read by many.
+// Few rows: one a workgroup, so that their parts are read by many.  The whole
+// call, one row a workgroup against 16, 8 key heads of 128 (us): one sequence of
+// 131,000 tokens and 160 rows 103 : 135; of 2,000 to 4,000 tokens 8 with 1,024
+// rows 26.6 : 29.7, 16 with 2,048 50.3 : 49.5, 16 with 4,096 59.5 : 52.8.  The wide
+// kernel's rows, which lie apart in fewer parts, gain from 16 earlier (one
+// sequence of 30,000, 1,280 rows 65.7 : 54.6), which this rule leaves.
 template <typename DT, int TILE>
 hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
   if ((long long)a.B * a.Hkv * a.M <= 2048)
@@ -555,6 +560,6 @@ hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
 
 hipError_t launch_attn_narrow(const AttnArgs& a, int dtype, hipStream_t st);
 hipError_t launch_attn_wide(const AttnArgs& a, int dtype, hipStream_t st);
-hipError_t set_attn_narrow_lds(size_t bytes);
+hipError_t set_attn_narrow_lds();
 
 }  // namespace tgs

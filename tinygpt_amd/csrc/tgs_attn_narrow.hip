@@ -17,8 +17,7 @@
 namespace tgs {
 namespace attn {
 
-template <int D, int QT>
-constexpr int narrow_waves() { return 4; }
+constexpr int NARROW_WAVES = 4;
 
 template <typename DT, int D, int QT, int NW>
 struct Narrow {
@@ -374,7 +373,7 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void narrow_kernel(AttnA
 
 template <typename DT, int D, int QT>
 hipError_t narrow_run(const AttnArgs& a, hipStream_t st) {
-  constexpr int NW = narrow_waves<D, QT>();
+  constexpr int NW = NARROW_WAVES;
   typedef Narrow<DT, D, QT, NW> K;
   const int grid = a.nwg ? a.nwg : a.B * a.Hkv;
   hipLaunchKernelGGL((narrow_kernel<DT, D, QT, NW>), dim3(grid), dim3(NW * 64), sizeof(typename K::Shared), st, a);
@@ -384,7 +383,7 @@ hipError_t narrow_run(const AttnArgs& a, hipStream_t st) {
 }
 template <typename DT, int D, int QT>
 hipError_t narrow_lds() {
-  constexpr int NW = narrow_waves<D, QT>();
+  constexpr int NW = NARROW_WAVES;
   return hipFuncSetAttribute((const void*)narrow_kernel<DT, D, QT, NW>, hipFuncAttributeMaxDynamicSharedMemorySize,
                              (int)sizeof(typename Narrow<DT, D, QT, NW>::Shared));
 }
@@ -423,7 +422,7 @@ hipError_t narrow_lds_type() {
 hipError_t launch_attn_narrow(const AttnArgs& a, int dtype, hipStream_t st) {
   return dtype == TGS_BF16 ? attn::narrow_type<attn::BF16>(a, a.QB / 16, st) : attn::narrow_type<attn::F16>(a, a.QB / 16, st);
 }
-hipError_t set_attn_narrow_lds(size_t) {
+hipError_t set_attn_narrow_lds() {
   const hipError_t e = attn::narrow_lds_type<attn::BF16>(), f = attn::narrow_lds_type<attn::F16>();
   return e != hipSuccess ? e : f;
 }

@@ -530,8 +530,8 @@ hipError_t launch_attn(const AttnArgs& a, const AttnPlan& p, int dtype, hipStrea
   return p.wide ? launch_attn_wide(a, dtype, st) : launch_attn_narrow(a, dtype, st);
 }
 
-hipError_t set_attn_lds_limit(size_t bytes) {
-  const hipError_t e = set_attn_narrow_lds(bytes), f = attn::wide_lds_type<attn::BF16>(), g = attn::wide_lds_type<attn::F16>();
+hipError_t set_attn_lds() {
+  const hipError_t e = set_attn_narrow_lds(), f = attn::wide_lds_type<attn::BF16>(), g = attn::wide_lds_type<attn::F16>();
   return e != hipSuccess ? e : f != hipSuccess ? f : g;
 }
 

@@ -114,6 +114,6 @@ struct AttnPlan {
 };
 AttnPlan attn_plan(int M, int D);
 hipError_t launch_attn(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st);
-hipError_t set_attn_lds_limit(size_t bytes);
+hipError_t set_attn_lds();  // dynamic LDS of the attention kernels
 
 }  // namespace tgs

@@ -55,7 +55,7 @@ int raise_lds(tgs_ctx* h) {
   std::lock_guard<std::mutex> lock(mu);
   if (h->device < 64 && (ready & bit)) return TGS_OK;
   hipError_t e = tgs::set_kv_fork_lds_limit(h->lds_limit);
-  if (e == hipSuccess) e = tgs::set_attn_lds_limit(h->lds_limit);
+  if (e == hipSuccess) e = tgs::set_attn_lds();
   if (e != hipSuccess) return hip_fail(h, e, "LDS limit");
   if (h->device < 64) ready |= bit;
   return TGS_OK;
