@@ -229,28 +229,26 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
     const int2 x = LDS ? rows[r] : load_row(r);
     return fork_row(a, x.x, x.y);
   };
+  // whether rows are bad: few are, so that only those mark themselves
+  auto bad_row = [&](int r) -> int& {
+    if constexpr (LDS) return s.at[r];
+    else return a.copies[r].w;
+  };
   if (LDS && tid < a.R) rows[tid] = load_row(tid);
+  for (int r = tid; r < a.R; r += KV_PLAN_NT) bad_row(r) = 0;
   for (int i = tid; i < N; i += KV_PLAN_NT) owner[i] = OWNER_FREE;
   if (!LDS) __threadfence();
   __syncthreads();
   for (int r = tid >> 6; r < a.R; r += KV_PLAN_NT / 64) {
     const ForkRow w = row_of(r);
     const int* t = a.tables + (long long)(w.par < 0 ? 0 : w.par) * P;
-    bool bad = false;
     for (int i = lane_id(); i < w.end; i += 64) {
       const int p = t[i];
       if ((unsigned)p < (unsigned)N)
         atomicMin(&owner[p], i < w.full ? -1 : r * P + i);
-      else
-        bad |= (long long)i << a.page_shift < w.len;
+      else if ((long long)i << a.page_shift < w.len)
+        bad_row(r) = 1;
       if (out && i < w.full) a.tables_out[(long long)r * P + i] = p;
-    }
-    bad = __ballot(bad) != 0;
-    if (lane_id() == 0) {
-      if constexpr (LDS)
-        s.at[r] = bad;
-      else
-        a.copies[r].w = bad;
     }
   }
   if (!LDS) __threadfence();
@@ -271,7 +269,7 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
     const int r = r0 + tid;
     const ForkRow w = r < a.R ? row_of(r) : ForkRow{-1, 0, 0, 0};
     const int* t = a.tables + (long long)(w.par < 0 ? 0 : w.par) * P;
-    const bool bad = r < a.R && (LDS ? s.at[tid] : a.copies[r].w) != 0;
+    const bool bad = r < a.R && bad_row(r);
     int need = 0;
     for (int i = w.full; i < w.end && !bad; i++) {
       const int p = t[i];
