@@ -129,7 +129,8 @@ const char* tgs_status_string(int status);
 int tgs_hint_from_params(const tgs_row_params* host_params, int B, int V, tgs_batch_hint* out);
 
 /* Create a sampler on `device`.  max_batch, max_vocab and max_hist bound
- * every later call (workspace is sized once here; calls never allocate). */
+ * every later call (workspace is sized once here, on a GPU of 256 CUs to 68 MB
+ * at least, which tgs_tree_attention's parts take; calls never allocate). */
 int tgs_create(tgs_handle* out, int device, int max_batch, int max_vocab, int max_hist);
 void tgs_destroy(tgs_handle h);
 /* Message of the handle's last error; NULL: the calling thread's last
@@ -306,8 +307,9 @@ typedef struct {
 /* Selects from each of G requests with W beams the n_out best continuations
  *   scores[g W + w] + x[g W + w][v] - logsumexp(x[g W + w])
  * over beams w and ids v, in descending order, equal ones by the lower beam,
- * then the lower id.  Logits as in tgs_sample (NaN and -inf logits are not
- * selected).  Totals are compared in 64 bits.  A beam whose score is not
+ * then the lower id (inside a beam by its logits).  Logits as in tgs_sample
+ * (NaN and -inf logits are not selected; finite ones of any size count as they
+ * are).  Exponentials are 32-bit, totals are compared in 64 bits.  A beam whose score is not
  * finite (-inf: it has ended) or whose row holds +inf or nothing gives no
  * candidates; outputs past the last candidate are -inf, -1, -1 and an empty
  * history.

@@ -9,7 +9,7 @@
 // through LDS at the end of a (sequence, key head).
 //
 // 16-bit, D = 128, 8 key heads: one sequence of 131,000 tokens 96 us (537 MB,
-// 5.6 TB/s; a plain read reaches 6.2); 32 sequences of 100 to 4096 tokens 63 us
+// 5.6 TB/s; a plain read reaches 6.2); 32 sequences of 100 to 4096 tokens 62 us
 // (280 MB, 4.5 TB/s), where a worker starts and ends about 1.5 of the
 // (sequence, key head) pairs.
 #include "tgs_attn.h"

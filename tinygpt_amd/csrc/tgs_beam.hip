@@ -14,7 +14,7 @@
 // needs no arithmetic; join_kernel orders the candidates of different beams by
 // totals in 64 bits, so that no further rounding to 32 decides between them.
 //
-// 32 requests of 8 beams over 128,256 ids, bf16 (66 MB): chunks 27 us, 2.4 TB/s,
+// 32 requests of 8 beams over 128,256 ids, bf16 (66 MB): chunks 28 us, 2.4 TB/s,
 // in two rounds of four workgroups a CU that each load, sort and collect in
 // turn; join 10 us.  4 beams over 32,000 ids, fp32: 5.4 and 5.8 us, the latency
 // of dependent steps.  Joining in the last workgroup to finish, in one launch,
