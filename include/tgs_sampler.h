@@ -346,7 +346,8 @@ typedef struct {
  * are taken within [0, width page].  What the cache's pages hold past a sequence's end
  * is never used, and a drafted node's row, whatever it holds, reaches only the
  * nodes that see it.  Products and sums are 32-bit; softmax weights are rounded
- * to the cache's type before they multiply values.  Outputs must not overlap
+ * to the cache's type before they multiply values, and their rounded sum divides
+ * the result; lse is that of the unrounded ones.  Outputs must not overlap
  * inputs. */
 int tgs_tree_attention(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs,
                        const tgs_attn* attn, tgs_stream stream);

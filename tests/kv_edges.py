@@ -301,3 +301,23 @@ def check_named(out, at, values):
     for b in range(B):
         for h in range(Hkv):
             assert ((out[b, :, h].double() - values[b][h, at[b, :, h]].double()).abs() < 2**-7).all(), (b, h)
+
+
+def one_value(T, G, D, dt, n=160, page=32):
+    """Every value is one number of the type, just below 2: whatever the weights are, so is every result.  One token
+    comes late and lies up to 2^5.9 above the first, by a different factor in every row, and the others 2^30 below."""
+    N = n // page
+    c = 2 - 2 * torch.finfo(dt).eps
+    k = torch.zeros(N, 1, page, D, dtype=dt)
+    k[..., 1] = -30
+    k[0, 0, 1] = 0
+    k[N - 1, 0, 2] = 0
+    k[N - 1, 0, 2, 0] = 1
+    v = torch.full((N, 1, page // 8, D, 8), c).to(dt)
+    q = torch.zeros(1, T, G, D, dtype=dt)
+    q[..., 0] = (5.9 * (torch.arange(T * G) + 1) / (T * G)).view(1, T, G)
+    q[..., 1] = 1
+    kn, vn = torch.zeros(1, T, 1, D, dtype=dt), torch.full((1, T, 1, D), c).to(dt)
+    kn[..., 1] = -30
+    table = torch.arange(N, dtype=torch.int32)[None]
+    return (q, kn, vn, k, v, table, torch.tensor([n], dtype=torch.int32), None), math.log(2), c

@@ -164,3 +164,16 @@ def test_attention_of_many_sequences(sampler, B, T, Hq):
     lens = torch.randint(0, 90, (B,), generator=E.gen(B)).tolist()
     lens[B - 4] = 1500
     run_attn(sampler, attn_inputs(B, B, T, Hq, 1, 64, lens, 32, E.BF16))
+
+
+@pytest.mark.parametrize("T,G,D,n", [(2, 8, 64, 160), (4, 8, 128, 160), (8, 8, 64, 160), (4, 32, 96, 160), (4, 8, 256, 160), (16, 8, 256, 320)])
+@pytest.mark.parametrize("dt", [E.BF16, E.F16])
+def test_attention_of_one_value(sampler, T, G, D, n, dt):
+    args, scale, c = E.one_value(T, G, D, dt, n=n)
+    H.log(f"attention of one value T={T} G={G} D={D} n={n} {dt}")
+    lse = torch.empty(1, T, G, device=DEV)
+    out = sampler.tree_attention(*(dev(t) for t in args[:7]), scale=scale, lse=lse)
+    torch.cuda.synchronize()
+    assert (out.cpu().double() == c).all(), out.cpu().double().sub(c).abs().max()
+    want = E.attention(args, scale)[1]
+    assert ((lse.cpu().double() - want).abs() <= 2**-18 * (1 + want.abs())).all()

@@ -150,3 +150,16 @@ def test_attention_of_many_sequences(sim):  # noqa: F811
     lens = torch.randint(0, 60, (70,), generator=E.gen(2)).tolist()
     lens[66] = 290
     run_attn(sim, attn_inputs(70, 70, 1, 1, 1, 64, lens, 32, BF16), num_cu=9)
+
+
+@pytest.mark.parametrize("T,G,D,n", [(2, 8, 64, 160), (4, 8, 128, 160), (8, 8, 64, 160), (4, 32, 96, 160), (16, 4, 64, 320)])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_attention_of_one_value(sim, T, G, D, n, dt):  # noqa: F811
+    """Results are sums over the weights that the product has, so that their rounding does not show in equal values (a
+    result before its rounding is off by a few steps of 32 bits, and the value is a number of the type)."""
+    args, scale, c = E.one_value(T, G, D, dt, n=n)
+    rc, out, lse = C.sim_attention(sim, *args, scale=scale)
+    assert rc == 0
+    assert (out.double() == c).all(), out.double().sub(c).abs().max()
+    want = E.attention(args, scale)[1]
+    assert ((lse.double() - want).abs() <= 2**-18 * (1 + want.abs())).all()

@@ -13,7 +13,12 @@
 // consecutive tokens, which is also one 16-byte vector of the values' layout.
 // No score goes through LDS or another lane.  The running maximum and sum are
 // 32-bit; P is rounded to the inputs' 16 bits (half a step of each weight, the
-// precision of the values it multiplies), O accumulates in 32.
+// precision of the values it multiplies), O accumulates in 32.  O is divided by
+// the sum of the rounded weights, so that what they are off by together cancels
+// (fp16, 217 tokens: the error against 64 bits, over that of 32-bit weights, from
+// 1.21 to 1.11 in the mean and from 1.55 to 1.21 at worst); the logsumexp is
+// that of the unrounded ones.  The second sum costs nothing that shows below 32
+// rows and 1 to 2 % above.
 //
 // Work is cut by an even share of tiles per worker, not by sequence: worker w
 // of N takes tiles [w U / N, (w + 1) U / N) of the U tiles of all sequences
@@ -98,6 +103,22 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 #else
   (void)lo, (void)hi;
   return 0;
+#endif
+}
+
+// c plus the two 16-bit values of x, in 32 bits.
+template <typename DT>
+__device__ __forceinline__ float add2(uint32_t x, float c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (__is_same(DT, BF16))
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, 0x3F803F80u), c, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, 0x3C003C00u), c, false);
+#elif defined(TGS_HOST_MFMA)
+  return c + hipcpu_to_float((uint16_t)x, __is_same(DT, BF16)) + hipcpu_to_float((uint16_t)(x >> 16), __is_same(DT, BF16));
+#else
+  (void)x;
+  return c;
 #endif
 }
 

@@ -42,7 +42,7 @@ struct Narrow {
 
   struct State {
     f32x4 o[QT][DT16];
-    float m[QT], l[QT];  // (l: of the lane's tokens alone)
+    float m[QT], l[QT], r[QT];  // (l, r: of the lane's tokens alone; r: of the rounded weights)
   };
 
   // Page entries of cache tile i for the lane's key block and value block.
@@ -142,6 +142,7 @@ struct Narrow {
         const float f = s.m[t] == NEG ? 0.0f : exp2_hw(s.m[t] - now);
         s.m[t] = now;
         s.l[t] *= f;
+        s.r[t] *= f;
 #pragma unroll
         for (int d = 0; d < DT16; d++) s.o[t][d] *= f;
       }
@@ -153,6 +154,8 @@ struct Narrow {
         s.l[t] += w[j];
       }
       p[t] = vec16(pack2<DT>(w[0], w[1]), pack2<DT>(w[2], w[3]), pack2<DT>(w[4], w[5]), pack2<DT>(w[6], w[7]));
+#pragma unroll
+      for (int j = 0; j < 4; j++) s.r[t] = add2<DT>(p[t][j], s.r[t]);
     }
   }
 
@@ -209,6 +212,7 @@ struct Narrow {
     for (int t = 0; t < QT; t++) {
       st.m[t] = NEG;
       st.l[t] = 0.0f;
+      st.r[t] = 0.0f;
 #pragma unroll
       for (int d = 0; d < DT16; d++) st.o[t][d] = f32x4{0, 0, 0, 0};
     }
@@ -288,6 +292,9 @@ struct Narrow {
     for (int t = 0; t < QT; t++) {
       st.l[t] += xor_lane<16>(st.l[t]);
       st.l[t] += xor_lane<32>(st.l[t]);
+      st.r[t] += xor_lane<16>(st.r[t]);
+      st.r[t] += xor_lane<32>(st.r[t]);
+      st.r[t] = st.r[t] > 0.0f ? st.l[t] / st.r[t] : 1.0f;
       if (any_bad) st.l[t] = __builtin_nanf("");
       if (grp == 0) {
         s.ml[wave][t * 16 + col][0] = st.m[t];
@@ -305,7 +312,7 @@ struct Narrow {
         const float mw = s.ml[w][t * 16 + col][0];
         sum += s.ml[w][t * 16 + col][1] * (mw == NEG ? 1.0f : exp2_hw(mw - top));
       }
-      const float f = st.m[t] == NEG ? 0.0f : exp2_hw(st.m[t] - top);
+      const float f = st.m[t] == NEG ? 0.0f : exp2_hw(st.m[t] - top) * st.r[t];
 #pragma unroll
       for (int d = 0; d < DT16; d++) s.o[wave][d * QT + t][lane] = st.o[t][d] * f;
       if (wave == 0 && grp == 0) {

@@ -169,7 +169,7 @@ struct Wide {
 
   struct State {
     f32x16 o[DT32];
-    float m, l;
+    float m, l, r;  // r: the sum of the rounded weights
   };
 
   // S^T of the tile in buffer f: element j of half x is token 32 x + 16 (j / 8) + 8 half + j % 8.
@@ -215,6 +215,7 @@ struct Wide {
       const float g = st.m == NEG ? 0.0f : exp2_hw(st.m - now);
       st.m = now;
       st.l *= g;
+      st.r *= g;
 #pragma unroll
       for (int d = 0; d < DT32; d++) st.o[d] *= g;
     }
@@ -224,7 +225,9 @@ struct Wide {
       const float u = exp2_hw(__builtin_fmaf(sc[y >> 1][(y & 1) * 8 + 2 * i], a.scale_log2, -base));
       const float w = exp2_hw(__builtin_fmaf(sc[y >> 1][(y & 1) * 8 + 2 * i + 1], a.scale_log2, -base));
       st.l += u + w;
-      return pack2<DT>(u, w);
+      const uint32_t x = pack2<DT>(u, w);
+      st.r = add2<DT>(x, st.r);
+      return x;
     };
     // each product runs beside the weights and the operand of the next 16 tokens'
     Vec x[DT32];
@@ -276,7 +279,7 @@ struct Wide {
     }
     State st;
     st.m = NEG;
-    st.l = 0.0f;
+    st.l = st.r = 0.0f;
 #pragma unroll
     for (int d = 0; d < DT32; d++)
 #pragma unroll
@@ -377,14 +380,15 @@ struct Wide {
           }
       }
     }
-    float m = st.m, l = st.l;
+    float m = st.m, l = st.l, lr = st.r;
     const f32x16(&o)[DT32] = st.o;
     l += xor_lane<32>(l);
+    lr += xor_lane<32>(lr);
     if (__ballot(bad)) l = __builtin_nanf("");  // (every wave read every entry)
     if (i >= a.M) return;  // (a part's rows past M are not read)
     if (full) {
       const long long row = ((long long)b * a.T + node) * a.Hq + h * a.G + hg;
-      const float r = 1.0f / l;
+      const float r = (l > 0.0f ? 1.0f : l) / lr;
 #pragma unroll
       for (int d = 0; d < DT32; d++)
 #pragma unroll
@@ -395,11 +399,12 @@ struct Wide {
       if (a.lse && half == 0) a.lse[row] = row_lse(m, l);
     } else {
       float* to = a.part_o + part * D + wave * 32 * D + lane * 4;
+      const float r = lr > 0.0f ? l / lr : 1.0f;
 #pragma unroll
       for (int d = 0; d < DT32; d++)
 #pragma unroll
         for (int x = 0; x < 4; x++)
-          *(f32x4*)(to + (d * 4 + x) * 256) = f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+          *(f32x4*)(to + (d * 4 + x) * 256) = f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]} * r;
       if (half == 0) {
         const long long row = part + wave * 32 + col;
         a.part_ml[row * 2] = m;
