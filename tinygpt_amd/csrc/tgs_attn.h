@@ -106,20 +106,25 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 #endif
 }
 
-// c plus the two 16-bit values of x, in 32 bits.
+// c plus the products of the two 16-bit values of x and those of y, in 32 bits.
 template <typename DT>
-__device__ __forceinline__ float add2(uint32_t x, float c) {
+__device__ __forceinline__ float dot2(uint32_t x, uint32_t y, float c) {
 #if defined(__HIP_DEVICE_COMPILE__)
   if constexpr (__is_same(DT, BF16))
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, 0x3F803F80u), c, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, y), c, false);
   else
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, 0x3C003C00u), c, false);
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, y), c, false);
 #elif defined(TGS_HOST_MFMA)
-  return c + hipcpu_to_float((uint16_t)x, __is_same(DT, BF16)) + hipcpu_to_float((uint16_t)(x >> 16), __is_same(DT, BF16));
+  auto value = [](uint32_t u) { return hipcpu_to_float((uint16_t)u, __is_same(DT, BF16)); };
+  return c + value(x) * value(y) + value(x >> 16) * value(y >> 16);
 #else
-  (void)x;
+  (void)x, (void)y;
   return c;
 #endif
+}
+template <typename DT>
+__device__ __forceinline__ float add2(uint32_t x, float c) {
+  return dot2<DT>(x, __is_same(DT, BF16) ? 0x3F803F80u : 0x3C003C00u, c);
 }
 
 // 2^x by the hardware instruction: results below 2^-126 are 0, weights that
@@ -311,9 +316,13 @@ __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
   constexpr bool B = __is_same(DT, BF16);
   return ((w & (B ? 0x7F807F80u : 0x7C007C00u)) + (B ? 0x00800080u : 0x04000400u)) & 0x80008000u;
 }
+// c where all eight values are finite, else NaN (0 times each is added; code
+// that every launch meets cold, so that few instructions count).
 template <typename DT>
-__device__ __forceinline__ uint32_t odd_bits(Vec x) {
-  return odd_bits<DT>(x[0]) | odd_bits<DT>(x[1]) | odd_bits<DT>(x[2]) | odd_bits<DT>(x[3]);
+__device__ __forceinline__ float finite_or_nan(Vec x, float c) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) c = dot2<DT>(x[i], 0u, c);
+  return c;
 }
 // Those values, and 0 for the others.
 template <typename DT>
@@ -325,6 +334,10 @@ __device__ __forceinline__ Vec odd_of(Vec x) {
   }
   return x;
 }
+template <typename DT>
+__device__ __forceinline__ bool is_nan(uint32_t u) {
+  return odd_bits<DT>(u) != 0 && (u & (__is_same(DT, BF16) ? 0x7Fu : 0x3FFu)) != 0;
+}
 // Elements d .. d + 3 of (b, h)'s drafted values: the sum of what is not finite
 // in the nodes of `sees`, 0 where all is.
 template <typename DT>
@@ -335,8 +348,8 @@ __device__ __forceinline__ f32x4 odd_sum(const AttnArgs& a, int b, int h, u64 se
     if (!(sees >> j & 1)) continue;
 #pragma unroll
     for (int z = 0; z < 4; z++) {
-      const uint32_t u = p[z], rest = u & (__is_same(DT, BF16) ? 0x7Fu : 0x3FFu);
-      if (odd_bits<DT>(u)) s[z] += tg_u2f((u & 0x8000u) << 16 | 0x7F800000u | (rest ? 0x400000u : 0u));
+      const uint32_t u = p[z];
+      if (odd_bits<DT>(u)) s[z] += tg_u2f((u & 0x8000u) << 16 | 0x7F800000u | (is_nan<DT>(u) ? 0x400000u : 0u));
     }
   }
   return s;

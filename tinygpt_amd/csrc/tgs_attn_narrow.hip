@@ -265,12 +265,12 @@ struct Narrow {
       load_tree_values(x);
       load_tree_keys(k);
       const u64 anc = ancestors(a, par);  // of node `lane`
-      uint32_t odd = 0;
+      float odd = 0.0f;  // NaN: not all values are finite
       if (a.T > 1) {  // (one node: every row sees it)
 #pragma unroll
         for (int n = 0; n < GO; n++)
 #pragma unroll
-          for (int j = 0; j < 8; j++) odd |= odd_bits<DT>(x[n][j]);
+          for (int j = 0; j < 8; j++) odd = finite_or_nan<DT>(x[n][j], odd);
       }
       scores(k, q, sc);
       turn_tree((Vec*)s.o[wave], x, v);
@@ -283,7 +283,7 @@ struct Narrow {
         for (int j = 0; j < 8; j++) sc[t][j >> 2][j & 3] = seen(sc[t][j >> 2][j & 3], in, j);
       }
       weights(sc, st, p);
-      if (__ballot(odd != 0)) add_odd(v, p, anc, st);
+      if (__ballot(odd != 0.0f)) add_odd(v, p, anc, st);
       add(v, p, st);
     }
     // the waves' states

@@ -36,10 +36,11 @@ struct Wide {
   int b, h, qb, len, nc;
   const int* table;
   bool bad;
+  int odd;  // whether a drafted tile so far had values that are not finite
 
   __device__ __forceinline__ Wide(const AttnArgs& a_)
       : a(a_), tid((int)threadIdx.x), lane(lane_id()), wave((int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), col(lane & 31), half(lane >> 5), b(0), h(0), qb(0),
-        len(0), nc(0), table(nullptr), bad(false) {}
+        len(0), nc(0), table(nullptr), bad(false), odd(0) {}
 
   // Where chunk ch of row tok lies.
   static __device__ __forceinline__ int at_key(int tok, int ch) {
@@ -143,12 +144,12 @@ struct Wide {
     }
     int odd = 0;
     if (a.T > 1) {  // (one node: every row sees it)
-      uint32_t bits = 0;
+      float sum = 0.0f;
 #pragma unroll
       for (int n = 0; n < TURN; n++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) bits |= odd_bits<DT>(v[n][j]);
-      odd = __ballot(bits != 0) != 0;
+        for (int j = 0; j < 8; j++) sum = finite_or_nan<DT>(v[n][j], sum);
+      odd = __ballot(sum != 0.0f) != 0;
       if (odd) {
 #pragma unroll
         for (int n = 0; n < TURN; n++)
@@ -314,6 +315,10 @@ struct Wide {
     }
     lds_barrier();
     if (drafted) {
+      int any = 0;
+#pragma unroll
+      for (int w = 0; w < QW; w++) any |= s.odd[w];
+      odd |= uniform(any);
       if (work) {
         const u64 sees = lane_bits(ancestors(a, par), node);
         scores(s, 1, q, sc);
@@ -360,26 +365,6 @@ struct Wide {
       }
       if (t < tc) step(t, 0, k0, v0);
     }
-    if (drafted) {
-      // What is not finite takes the place of a sum: no weight or addend that is
-      // finite changes it.  (s.odd is written again behind the next segment's
-      // first barrier.  The check costs 1 us of 34 for 16 sequences of 1000 to
-      // 3000 tokens and 48 rows of 128; adding at the drafted tile spills.)
-      int odd = 0;
-#pragma unroll
-      for (int w = 0; w < QW; w++) odd |= s.odd[w];
-      if (uniform(odd)) {
-        const u64 sees = lane_bits(ancestors(a, parent_of(a, b)), node);
-#pragma unroll
-        for (int d = 0; d < DT32; d++)
-#pragma unroll
-          for (int x = 0; x < 4; x++) {
-            const f32x4 y = odd_sum<DT>(a, b, h, sees, d * 32 + x * 8 + half * 4);
-#pragma unroll
-            for (int z = 0; z < 4; z++) st.o[d][4 * x + z] = y[z] == 0.0f ? st.o[d][4 * x + z] : y[z];
-          }
-      }
-    }
     float m = st.m, l = st.l, lr = st.r;
     const f32x16(&o)[DT32] = st.o;
     l += xor_lane<32>(l);
@@ -412,6 +397,30 @@ struct Wide {
       }
     }
   }
+
+  // Puts the drafted values that are not finite (the product had 0 for them)
+  // where a row that sees them has its results: no weight or addend that is
+  // finite changes them.  A lane writes what it wrote before.
+  __device__ __forceinline__ void put_odd(bool full, long long part) const {
+    const int i = qb * a.QB + wave * 32 + col;
+    const int node = i < a.M ? i / a.G : 0, hg = i < a.M ? i - node * a.G : 0;
+    const u64 sees = lane_bits(ancestors(a, parent_of(a, b)), node);
+    if (i >= a.M) return;
+    __threadfence();  // (behind the stores of the segment, whose types are others)
+    uint16_t* out = (uint16_t*)a.out + (((long long)b * a.T + node) * a.Hq + h * a.G + hg) * D;
+#pragma nounroll
+    for (int d = half * 4; d < D; d += 8) {
+      const f32x4 y = odd_sum<DT>(a, b, h, sees, d);
+#pragma unroll
+      for (int z = 0; z < 4; z++) {
+        if (y[z] == 0.0f) continue;
+        if (!full)
+          a.part_o[part * D + part_at<WTILE>(D, wave * 32 + col, d + z)] = y[z];
+        else if (!is_nan<DT>(out[d + z]))  // (a row of NaN stays one)
+          out[d + z] = (uint16_t)pack2<DT>(y[z], 0.0f);
+      }
+    }
+  }
 };
 
 template <typename DT, int D, int QW>
@@ -427,6 +436,7 @@ __global__ __launch_bounds__(QW * 64, D == 256 ? 1 : 2) void wide_kernel(AttnArg
     n.b = seg / a.Hkv;
     n.h = seg % a.Hkv;
     n.segment(s, 0, cache_tiles<WTILE>(a, n.b) + tree, true, 0);
+    if (n.odd) n.put_odd(true, 0);
     return;
   }
   // the row groups that read the same tiles run at the same time on one XCD
@@ -436,22 +446,30 @@ __global__ __launch_bounds__(QW * 64, D == 256 ? 1 : 2) void wide_kernel(AttnArg
   n.qb = a.nwg % 8 == 0 ? x / 8 % a.nqb : x % a.nqb;
   const Place at0 = find_place<WTILE>(a, w);
   const long long u0 = at0.u0, u1 = at0.u1;
-  int b = at0.b, h = at0.h, at = at0.at, nt = at0.nt;
-  for (long long u = u0; u < u1;) {
-    const int end = nt - at < u1 - u ? nt : at + (int)(u1 - u);
-    const int real = nt - extra<WTILE>();
-    if (at < real) {
-      n.b = b;
-      n.h = h;
-      n.segment(s, at, end < real ? end : real, at == 0 && end >= real, ((long long)(n.qb * a.nwg + w) * 2 + (u != u0)) * a.QB);
+  auto walk = [&](auto f) {
+    int b = at0.b, h = at0.h, at = at0.at, nt = at0.nt;
+    for (long long u = u0; u < u1;) {
+      const int end = nt - at < u1 - u ? nt : at + (int)(u1 - u);
+      const int real = nt - extra<WTILE>();
+      if (at < real) {
+        n.b = b;
+        n.h = h;
+        f(at, end < real ? end : real, real, at == 0 && end >= real, ((long long)(n.qb * a.nwg + w) * 2 + (u != u0)) * a.QB);
+      }
+      u += end - at;
+      at = 0;
+      if (++h == a.Hkv) {
+        h = 0;
+        if (++b < a.B) nt = cache_tiles<WTILE>(a, b) + tree + extra<WTILE>();
+      }
     }
-    u += end - at;
-    at = 0;
-    if (++h == a.Hkv) {
-      h = 0;
-      if (++b < a.B) nt = cache_tiles<WTILE>(a, b) + tree + extra<WTILE>();
-    }
-  }
+  };
+  walk([&](int t0, int t1, int, bool full, long long part) { n.segment(s, t0, t1, full, part); });
+  // (Behind everything: code to jump over in a segment costs 1 us of 33, for 16
+  // sequences of 1000 to 3000 tokens and 48 rows of 128.)
+  if (n.odd) walk([&](int, int t1, int real, bool full, long long part) {
+    if (t1 == real) n.put_odd(full, part);
+  });
 }
 
 template <typename DT, int D, int QW>
