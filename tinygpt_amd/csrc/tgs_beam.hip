@@ -70,7 +70,7 @@ __device__ __forceinline__ double scaled(double x, float e) { return __builtin_l
 
 // The natural logarithm of a sum and its base as they are handed on.
 __device__ __forceinline__ double log_sum(double base, double sum) {
-  return sum < 0.0 ? base + log(-sum) : sum == 0.0 ? -__builtin_inf() : base * LN2 + log(sum);
+  return (sum < 0.0 ? base : base * LN2) + log(__builtin_fabs(sum));
 }
 
 // Workgroup (row, chunk): ids [c L, min(V, (c + 1) L)), NVT vectors a thread.
@@ -211,8 +211,13 @@ __global__ __launch_bounds__(BEAM_NT, 4) void chunk_kernel(BeamArgs a) {
       double at = (double)b, t = 0.0;
       if (far) {
         at = -__builtin_inf();
-        for (int i = 0; i < BEAM_NT / 64; i++) at = fmax(at, log_sum((double)s.base[i], s.sum[i]));
-        for (int i = 0; i < BEAM_NT / 64; i++) t -= exp(log_sum((double)s.base[i], s.sum[i]) - at);
+#pragma nounroll
+        for (int i = 0; i < BEAM_NT / 64; i++) {
+          s.sum[i] = log_sum((double)s.base[i], s.sum[i]);
+          at = fmax(at, s.sum[i]);
+        }
+#pragma nounroll
+        for (int i = 0; i < BEAM_NT / 64; i++) t -= exp(s.sum[i] - at);
       } else {
 #pragma unroll
         for (int i = 0; i < BEAM_NT / 64; i++) t += scaled(s.sum[i], s.base[i] - b);
