@@ -9,7 +9,7 @@
 // are neighbours already.
 //
 // 16 sequences of 2000 to 6000 tokens, 63 nodes, 4 key heads with 8 query heads
-// each, D = 128: 85 us for 66.6 GFLOP, 0.8 PFLOP/s (59 us at a large library
+// each, D = 128: 87 us for 66.6 GFLOP, 0.8 PFLOP/s (59 us at a large library
 // product's rate).  28 us of it are not in the tile loop.  In the loop a tile's
 // LDS reads, products and weights follow each other in both waves of a SIMD;
 // 64 rows a wave would halve the reads but need copies between the register
