@@ -296,6 +296,52 @@ typedef struct {
   int64_t v_layer, v_seq, v_tok, v_head;
 } tgs_kv_rows;
 
+/* The same cache held in 8 bits, in blocks of 16 tokens (all strides in bytes,
+ * multiples of 16, those of scales of 2; k and v 16-byte aligned):
+ *   k      [layers][n_pages][kv_heads][page][head_dim]           e4m3 codes
+ *   v      [layers][n_pages][kv_heads][page / 16][head_dim][16]  e4m3 codes
+ *   scales [layers][n_pages][kv_heads][page / 16][2]             e8m0: 2^(byte - 127)
+ * with one scale for the keys and one for the values of each block of a head: a
+ * number is its code times its block's scale.  A page of each is contiguous.
+ *
+ * Rows are written so: magnitudes past 1.875 2^127 (bf16 rows) or 61,440 (fp16
+ * rows) count as that, numbers that are not finite become NaN; the scale 2^e of a
+ * block is the smallest, e at least -100 (bf16) or -15 (fp16), with which the
+ * largest of its new rows stays within 448, and none below the one it has while
+ * it holds earlier tokens of the sequence; codes are rounded to the nearest, ties
+ * to even, those of the earlier tokens again where the scale grows.  So every
+ * number that the cache stands for is exact in the rows' type. */
+typedef struct {
+  void* k;
+  void* v;
+  void* scales;
+  int64_t k_layer, k_page, v_layer, v_page, s_layer, s_page;
+  int32_t layers, n_pages;
+  int32_t page;     /* tokens of a page: a power of two, 16 to 1024 */
+  int32_t kv_heads;
+  int32_t head_dim; /* a multiple of 16, at most 256; kv_heads * head_dim < 65536 */
+} tgs_kv8_cache;
+
+/* The position rotation: pair j of a row's first `dims` dimensions turns by the
+ * angle position * freq[j] (reduced in 64 bits): dimensions j and j + dims / 2, or
+ * with `pairs` the neighbours 2 j and 2 j + 1.  The others stay. */
+typedef struct {
+  const float* freq; /* [dims / 2], on the device */
+  int32_t dims;      /* a multiple of 16, 16 to 256, at most head_dim */
+  int32_t pairs;
+} tgs_rotary;
+
+/* Rows [B][T][heads][head_dim] and where they go, with any strides (in elements);
+ * head_dim is contiguous.  out is x with its strides (in place) or does not
+ * overlap it. */
+typedef struct {
+  const void* x;
+  void* out;
+  int64_t x_seq, x_tok, x_head;
+  int64_t out_seq, out_tok, out_head;
+  int32_t heads;
+} tgs_rotate_rows;
+
 /* The sequences of a call: page tables [B][width] and lengths [B] (tokens in
  * the cache). */
 typedef struct {
@@ -394,6 +440,43 @@ int tgs_tree_commit(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* 
  * Outputs must not overlap inputs. */
 int tgs_kv_fork(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_seqs* seqs, const int32_t* d_parents, int room,
                 int32_t* d_tables_out, int32_t* d_lens_out, tgs_stream stream);
+
+/* tgs_tree_attention over a cache held in 8 bits (one layer): queries, the nodes'
+ * own rows and out are of the type dt (TGS_BF16 or TGS_F16), the one of the rows
+ * that the cache was written from; head_dim 64, 96, 128 or 256.  Everything else
+ * as there.  A block whose scale is NaN (255) gives NaN. */
+int tgs_kv8_attention(tgs_handle h, const tgs_kv8_cache* cache, tgs_dtype dt, const tgs_kv_rows* rows,
+                      const tgs_kv_seqs* seqs, const tgs_attn* attn, tgs_stream stream);
+
+/* tgs_kv_append with the keys turned by their positions lens[b] + i on the way
+ * (in 32 bits, then rounded once); values move as they are. */
+int tgs_kv_append_rotated(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs,
+                          int T, const int32_t* d_counts, const tgs_rotary* rotary, int32_t* d_lens_out,
+                          tgs_stream stream);
+
+/* tgs_kv_append of rows of the type dt (TGS_BF16 or TGS_F16) to a cache held in 8
+ * bits, the keys turned by their positions where rotary is given (nullable). */
+int tgs_kv8_append(tgs_handle h, const tgs_kv8_cache* cache, tgs_dtype dt, const tgs_kv_rows* rows,
+                   const tgs_kv_seqs* seqs, int T, const int32_t* d_counts, const tgs_rotary* rotary,
+                   int32_t* d_lens_out, tgs_stream stream);
+
+/* tgs_tree_commit with rows of the type dt to a cache held in 8 bits. */
+int tgs_kv8_commit(tgs_handle h, const tgs_kv8_cache* cache, tgs_dtype dt, const tgs_kv_rows* rows,
+                   const tgs_kv_seqs* seqs, int T, const int32_t* d_parents, const int32_t* d_draft,
+                   const int32_t* d_sampled, int32_t* d_n_acc, int32_t* d_tokens, int32_t* d_path, int32_t* d_lens_out,
+                   tgs_stream stream);
+
+/* tgs_kv_fork of a cache held in 8 bits: copies are whole blocks of 16 tokens,
+ * with their scales. */
+int tgs_kv8_fork(tgs_handle h, const tgs_kv8_cache* cache, const tgs_kv_seqs* seqs, const int32_t* d_parents, int room,
+                 int32_t* d_tables_out, int32_t* d_lens_out, tgs_stream stream);
+
+/* Turns the queries and keys of T new nodes per sequence by their positions, lens[b]
+ * and the node's depth in its tree (d_parents as in tgs_attn, T <= 64 then; NULL: a
+ * chain of any T), in 32 bits, then rounded once to dt (TGS_BF16 or TGS_F16).  A
+ * length below 0 counts as 0.  k is nullable. */
+int tgs_rotate(tgs_handle h, tgs_dtype dt, const tgs_rotate_rows* q, const tgs_rotate_rows* k, int B, int T, int head_dim,
+               const int32_t* d_lens, const int32_t* d_parents, const tgs_rotary* rotary, tgs_stream stream);
 
 #ifdef __cplusplus
 }

@@ -10,6 +10,7 @@
 struct alignas(16) int4 {
   int x, y, z, w;
 };
+static inline uint2 make_uint2(uint32_t a, uint32_t b) { return {a, b}; }
 static inline int4 make_int4(int a, int b, int c, int d) { return {a, b, c, d}; }
 inline void __threadfence() { __atomic_thread_fence(__ATOMIC_SEQ_CST); }
 
@@ -64,4 +65,28 @@ inline V hipcpu_mfma(const A& a, const A& b, V c) {
   }
   hipcpu::wave().bar->arrive_and_wait();
   return c;
+}
+
+// ---- e4m3 codes (4 bits of exponent, 3 of significand, no infinity), and the
+// power of two that the scaled conversions take from a float's exponent.
+inline float hipcpu_from_e4m3(uint8_t x) {
+  const int e = (x >> 3) & 15, m = x & 7;
+  const float s = x & 0x80 ? -1.0f : 1.0f;
+  if (e == 15 && m == 7) return NAN;
+  return s * (e ? std::ldexp((float)(8 + m), e - 10) : std::ldexp((float)m, -9));
+}
+inline uint8_t hipcpu_to_e4m3(float f) {
+  const uint8_t s = std::signbit(f) ? 0x80 : 0;
+  const float a = std::fabs(f);
+  if (!(a <= 464.0f)) return s | 0x7F;
+  int e;
+  std::frexp(a, &e);  // a in [2^(e-1), 2^e)
+  if (a == 0.0f) return s;
+  const int q = e - 4 < -9 ? -9 : e - 4;  // exponent of a step
+  const uint32_t n = (uint32_t)std::nearbyint(std::ldexp(a, -q));
+  return s | (uint8_t)(q == -9 ? n : ((uint32_t)(q + 9) << 3) + n);
+}
+inline float hipcpu_scale(float s) {
+  const int e = (int)(__float_as_uint(s) >> 23 & 255);
+  return e == 255 ? NAN : std::ldexp(1.0f, e - 127);
 }

@@ -79,9 +79,34 @@ int main(int argc, char** argv) {
                          i32("o_tokens"), i32("o_path"), i32("o_lens"), nullptr);
   else if (op == "fork")
     rc = tgs_kv_fork(&h, &c, &s, i32("parents"), I("room"), i32("o_tables"), i32("o_lens"), nullptr);
+  // the same over an 8-bit cache, and the rotation
+  tgs_kv8_cache c8 = {in("k"), in("v"), in("scales"), L("k_layer"), L("k_page"), L("v_layer"), L("v_page"), L("s_layer"),
+                      L("s_page"), I("layers"), I("pages"), I("page"), I("kv_heads"), I("D")};
+  const tgs_dtype dt = (tgs_dtype)I("dtype");
+  tgs_rotary rot = {f32("freq"), I("dims"), I("pairs")};
+  const tgs_rotary* turns = rot.freq ? &rot : nullptr;
+  if (op == "attn8") {
+    tgs_attn a = {in("q"), L("qs"), L("qt"), L("qh"), i32("parents"), in("o_out"), f32("o_lse"), I("T"), I("Hq"),
+                  I("max_len"), (float)meta["scale"]};
+    rc = tgs_kv8_attention(&h, &c8, dt, &r, &s, &a, nullptr);
+  } else if (op == "append8")
+    rc = tgs_kv8_append(&h, &c8, dt, &r, &s, I("T"), i32("counts"), turns, i32("o_lens"), nullptr);
+  else if (op == "append_rotated")
+    rc = tgs_kv_append_rotated(&h, &c, &r, &s, I("T"), i32("counts"), turns, i32("o_lens"), nullptr);
+  else if (op == "commit8")
+    rc = tgs_kv8_commit(&h, &c8, dt, &r, &s, I("T"), i32("parents"), i32("draft"), i32("sampled"), i32("o_n_acc"),
+                        i32("o_tokens"), i32("o_path"), i32("o_lens"), nullptr);
+  else if (op == "fork8")
+    rc = tgs_kv8_fork(&h, &c8, &s, i32("parents"), I("room"), i32("o_tables"), i32("o_lens"), nullptr);
+  else if (op == "rotate") {
+    const bool here = I("here");
+    tgs_rotate_rows q = {here ? in("o_q") : in("q"), in("o_q"), L("qs"), L("qt"), L("qh"), L("oqs"), L("oqt"), L("oqh"), I("Hq")};
+    tgs_rotate_rows k = {here ? in("o_k") : in("k_new"), in("o_k"), L("ks"), L("kt"), L("kh"), L("oks"), L("okt"), L("okh"), I("Hk")};
+    rc = tgs_rotate(&h, dt, &q, I("Hk") ? &k : nullptr, I("B"), I("T"), I("D"), i32("lens"), i32("parents"), turns, nullptr);
+  }
   std::printf("rc %d %s\n", rc, h.err.c_str());
   for (auto& [name, a] : arrays)
-    if (name.rfind("o_", 0) == 0 || name == "k" || name == "v") {
+    if (name.rfind("o_", 0) == 0 || name == "k" || name == "v" || name == "scales") {
       FILE* f = std::fopen((dir + "/" + name + ".out").c_str(), "wb");
       std::fwrite(a.first, 1, a.second, f);
       std::fclose(f);

@@ -49,6 +49,12 @@ EXPORTS = (
     "tgs_kv_append",
     "tgs_tree_commit",
     "tgs_kv_fork",
+    "tgs_kv_append_rotated",
+    "tgs_kv8_attention",
+    "tgs_kv8_append",
+    "tgs_kv8_commit",
+    "tgs_kv8_fork",
+    "tgs_rotate",
 )
 
 ROW_PARAMS_DTYPE = np.dtype(
@@ -149,6 +155,18 @@ def load() -> C.CDLL:
     L.tgs_tree_commit.argtypes = [P, P, P, P, I, P, P, P, P, P, P, P, P]
     L.tgs_kv_fork.restype = I
     L.tgs_kv_fork.argtypes = [P, P, P, P, I, P, P, P]
+    L.tgs_kv_append_rotated.restype = I
+    L.tgs_kv_append_rotated.argtypes = [P, P, P, P, I, P, P, P, P]
+    L.tgs_kv8_attention.restype = I
+    L.tgs_kv8_attention.argtypes = [P, P, I, P, P, P, P]
+    L.tgs_kv8_append.restype = I
+    L.tgs_kv8_append.argtypes = [P, P, I, P, P, I, P, P, P, P]
+    L.tgs_kv8_commit.restype = I
+    L.tgs_kv8_commit.argtypes = [P, P, I, P, P, I, P, P, P, P, P, P, P, P]
+    L.tgs_kv8_fork.restype = I
+    L.tgs_kv8_fork.argtypes = [P, P, P, P, I, P, P, P]
+    L.tgs_rotate.restype = I
+    L.tgs_rotate.argtypes = [P, I, P, P, I, I, I, P, P, P, P]
     _lib = L
     return L
 

@@ -19,8 +19,8 @@ OUT = os.path.join(HERE, "libtgs_sampler.so")
 # its own library: not part of the sampler's C ABI)
 FLOOR_SRC = "tgs_floor.hip"
 FLOOR_OUT = os.path.join(HERE, "libtgs_floor.so")
-SOURCES = ["tgs_attn_wide.hip", "tgs_attn_narrow.hip", "tgs_kernels.hip", "tgs_k64.hip", "tgs_spec.hip", "tgs_topp.hip", "tgs_topp_split.hip", "tgs_topk.hip", "tgs_logprob.hip",
-           "tgs_mask.hip", "tgs_kv.hip", "tgs_beam.hip", "tgs_kv_api.hip", "tgs_api.hip"]
+SOURCES = ["tgs_attn_wide.hip", "tgs_attn_wide8.hip", "tgs_attn_narrow.hip", "tgs_attn_narrow8.hip", "tgs_kernels.hip", "tgs_k64.hip", "tgs_spec.hip", "tgs_topp.hip", "tgs_topp_split.hip", "tgs_topk.hip", "tgs_logprob.hip",
+           "tgs_mask.hip", "tgs_kv.hip", "tgs_kv8.hip", "tgs_rotate.hip", "tgs_beam.hip", "tgs_kv_api.hip", "tgs_api.hip"]
 # the Python side's checks of the cache calls (host code against torch's headers)
 PY_SRC = "tgs_cache_py.cpp"
 PY_OUT = os.path.join(HERE, "_cache_calls.so")

@@ -28,6 +28,7 @@
 #pragma once
 
 #include "tgs_device.h"
+#include "tgs_e8.h"
 #include "tgs_kv.h"
 #include "tgs_row.h"
 
@@ -44,13 +45,12 @@ __device__ __forceinline__ Vec load16(const uint16_t* p) {
   return *(const Vec2*)p;
 }
 
-struct BF16 {};
-struct F16 {};
+using e8::BF16;
+using e8::F16;
 
 #if defined(__HIP_DEVICE_COMPILE__)
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 #endif
@@ -89,22 +89,7 @@ __device__ __forceinline__ f32x16 mfma32(Vec a, Vec b, f32x16 c) {
 #endif
 }
 
-// Two floats to 16 bits, to the nearest, ties to even: the first in the low half.
-template <typename DT>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  const f32x2v x = {lo, hi};
-  if constexpr (__is_same(DT, BF16))
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
-#elif defined(TGS_HOST_MFMA)
-  return hipcpu_pack2<__is_same(DT, BF16)>(lo, hi);
-#else
-  (void)lo, (void)hi;
-  return 0;
-#endif
-}
+using e8::to16;
 
 // c plus the products of the two 16-bit values of x and those of y, in 32 bits.
 template <typename DT>
@@ -125,6 +110,13 @@ __device__ __forceinline__ float dot2(uint32_t x, uint32_t y, float c) {
 template <typename DT>
 __device__ __forceinline__ float add2(uint32_t x, float c) {
   return dot2<DT>(x, __is_same(DT, BF16) ? 0x3F803F80u : 0x3C003C00u, c);
+}
+
+// Eight e4m3 codes times the scale s, in 16 bits.
+template <typename DT>
+__device__ __forceinline__ Vec decode8(uint32_t lo, uint32_t hi, float s) {
+  constexpr bool B = __is_same(DT, BF16);
+  return vec16(e8::decode16<B, false>(lo, s), e8::decode16<B, true>(lo, s), e8::decode16<B, false>(hi, s), e8::decode16<B, true>(hi, s));
 }
 
 // 2^x by the hardware instruction: results below 2^-126 are 0, weights that
@@ -156,7 +148,24 @@ __device__ __forceinline__ void lds_barrier() {
 #endif
 }
 
-constexpr int NTILE = 32, WTILE = 64;  // tokens of a tile of the narrow and of the wide kernel
+// A kernel's tiles: their tokens, what a (sequence, key head) costs beyond its tiles
+// (queries, the first tile's latency, the result), counted in tiles when shares are
+// cut, and whether a part's sums lie row by row.  Without the extra a worker whose
+// share lies in short sequences would end last (32 sequences of 100 to 4096 tokens,
+// 8 key heads of 128: 86 us without, 63 with 4 or more).
+struct Narrow16 {
+  static constexpr int TILE = 32, EXTRA = 8;
+  static constexpr bool ROWS = true;
+};
+struct Narrow8 {  // (of an 8-bit cache: as many bytes a tile)
+  static constexpr int TILE = 64, EXTRA = 8;
+  static constexpr bool ROWS = true;
+};
+struct WideGeo {
+  static constexpr int TILE = 64, EXTRA = 4;
+  static constexpr bool ROWS = false;
+};
+constexpr int NTILE = 32, WTILE = 64;  // drafted nodes that the narrow and the wide kernel take at most
 constexpr float NEG = -__builtin_inff();
 
 // The length by which an append, a commit or a fork reports that rows did not
@@ -186,29 +195,22 @@ __device__ __forceinline__ int clamp_len(const AttnArgs& a, int n) {
   const long long cap = (long long)a.P << a.page_shift;
   return n < 0 ? 0 : n > cap ? (int)cap : n;
 }
-template <int TILE>
+template <class GEO>
 __device__ __forceinline__ int cache_tiles(const AttnArgs& a, int b) {
-  return (uniform(clamp_len(a, a.lens[b])) + TILE - 1) / TILE;
+  return (uniform(clamp_len(a, a.lens[b])) + GEO::TILE - 1) / GEO::TILE;
 }
-template <int TILE>  // (a sequence per lane)
+template <class GEO>  // (a sequence per lane)
 __device__ __forceinline__ int lane_tiles(const AttnArgs& a, int b) {
-  return (clamp_len(a, a.lens[b]) + TILE - 1) / TILE;
+  return (clamp_len(a, a.lens[b]) + GEO::TILE - 1) / GEO::TILE;
 }
-
-// What a (sequence, key head) costs beyond its tiles (queries, the first
-// tile's latency, the result), counted in tiles when shares are cut: a worker
-// whose share lies in short sequences would else end last (32 sequences of 100
-// to 4096 tokens, 8 key heads of 128: 86 us without, 63 with 4 or more).
-template <int TILE>
-constexpr int extra() { return TILE == NTILE ? 8 : 4; }
 
 // Tiles of sequences before b (of one key head), and of all: by one wave.
-template <int TILE>
+template <class GEO>
 __device__ __forceinline__ void tiles_before(const AttnArgs& a, int b, int& before, int& all) {
-  const int tree = (a.T + TILE - 1) / TILE + extra<TILE>();
+  const int tree = (a.T + GEO::TILE - 1) / GEO::TILE + GEO::EXTRA;
   int x = 0, y = 0;
   for (int i = lane_id(); i < a.B; i += 64) {
-    const int n = lane_tiles<TILE>(a, i) + tree;
+    const int n = lane_tiles<GEO>(a, i) + tree;
     y += n;
     if (i < b) x += n;
   }
@@ -231,18 +233,18 @@ struct Place {
   long long u0, u1;
   int b, h, at, nt;
 };
-template <int TILE>
+template <class GEO>
 __device__ __forceinline__ Place find_place(const AttnArgs& a, int w) {
-  const int tree = (a.T + TILE - 1) / TILE + extra<TILE>(), lane = lane_id();
-  const int mine = lane < a.B ? lane_tiles<TILE>(a, lane) + tree : 0;  // (of the first 64 sequences)
+  const int tree = (a.T + GEO::TILE - 1) / GEO::TILE + GEO::EXTRA, lane = lane_id();
+  const int mine = lane < a.B ? lane_tiles<GEO>(a, lane) + tree : 0;  // (of the first 64 sequences)
   int y = mine;
-  for (int i = lane + 64; i < a.B; i += 64) y += lane_tiles<TILE>(a, i) + tree;
+  for (int i = lane + 64; i < a.B; i += 64) y += lane_tiles<GEO>(a, i) + tree;
   const long long U = (long long)uniform(wave_sum(y)) * a.Hkv;
   Place p{share_start(U, a.nwg, w), share_start(U, a.nwg, w + 1), 0, 0, 0, 0};
   if (p.u0 == p.u1) return p;
   long long before = 0;
   for (int b0 = 0;; b0 += 64) {
-    const int n = b0 == 0 ? mine : b0 + lane < a.B ? lane_tiles<TILE>(a, b0 + lane) + tree : 0;
+    const int n = b0 == 0 ? mine : b0 + lane < a.B ? lane_tiles<GEO>(a, b0 + lane) + tree : 0;
     const int incl = wave_incl_scan(n);
     const u64 ends = __ballot(b0 + lane < a.B && before + (long long)incl * a.Hkv > p.u0);
     if (ends) {
@@ -271,9 +273,8 @@ __device__ __forceinline__ int parent_of(const AttnArgs& a, int b) {
 
 // Ancestors of each node, itself among them, as bits, from its parent: by one
 // wave, node in lane.
-__device__ __forceinline__ u64 ancestors(const AttnArgs& a, int par) {
+__device__ __forceinline__ u64 ancestors_of(int par) {
   const int lane = lane_id();
-  if (!a.parents) return lane == 63 ? ~0ull : (2ull << lane) - 1;
   u64 m = 1ull << lane;
 #pragma unroll
   for (int i = 0; i < 6; i++) {  // paths double
@@ -287,16 +288,23 @@ __device__ __forceinline__ u64 ancestors(const AttnArgs& a, int par) {
   }
   return m;
 }
+__device__ __forceinline__ u64 ancestors(const AttnArgs& a, int par) {
+  const int lane = lane_id();
+  if (!a.parents) return lane == 63 ? ~0ull : (2ull << lane) - 1;
+  return ancestors_of(par);
+}
 
 // Lane `from`'s 64 bits.
 __device__ __forceinline__ u64 lane_bits(u64 m, int from) {
   return ((u64)(uint32_t)__shfl((int)(m >> 32), from, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)m, from, 64);
 }
 
-// A mask of the first n of eight 16-bit values (n <= 0: none).
+// A mask of the first n of a vector's values of BITS bits (n <= 0: none).
+template <int BITS>
 __device__ __forceinline__ Vec first_of(int n) {
-  const u64 lo = n >= 4 ? ~0ull : n <= 0 ? 0ull : (1ull << (16 * n)) - 1;
-  const u64 hi = n >= 8 ? ~0ull : n <= 4 ? 0ull : (1ull << (16 * n - 64)) - 1;
+  constexpr int HALF = 64 / BITS;
+  const u64 lo = n >= HALF ? ~0ull : n <= 0 ? 0ull : (1ull << (BITS * n)) - 1;
+  const u64 hi = n >= 2 * HALF ? ~0ull : n <= HALF ? 0ull : (1ull << (BITS * n - 64)) - 1;
   return vec16((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
@@ -382,8 +390,8 @@ __device__ __forceinline__ void transpose8(Vec (&x)[8]) {
 template <typename DT>
 __device__ __forceinline__ void store4(uint16_t* p, f32x4 x) {
   uint2 w;
-  w.x = pack2<DT>(x[0], x[1]);
-  w.y = pack2<DT>(x[2], x[3]);
+  w.x = to16<DT>(x[0], x[1]);
+  w.y = to16<DT>(x[2], x[3]);
   *(uint2*)p = w;
 }
 
@@ -412,9 +420,9 @@ __device__ __forceinline__ float wave_sumf(float x) {
 // the wide kernel's by 32 rows, [D / 8][half][row][4], a lane's four next to the
 // neighbouring rows' (its stores are 1 KB each; 64-byte pieces took 5 us more
 // of 16 sequences' 63 nodes).
-template <int TILE>
+template <class GEO>
 __device__ __forceinline__ int part_at(int D, int row, int d) {
-  if (TILE == NTILE) return row * D + d;
+  if (GEO::ROWS) return row * D + d;
   return (row >> 5) * 32 * D + ((d >> 3) * 64 + ((d >> 2) & 1) * 32 + (row & 31)) * 4 + (d & 3);
 }
 
@@ -434,12 +442,12 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, int b, int h, int i
   const float rl = 1.0f / l;
 #pragma unroll
   for (int z = 0; z < 4; z++)
-    if (z * 64 + lane < a.D) ((uint16_t*)a.out)[out * a.D + z * 64 + lane] = (uint16_t)pack2<DT>(o[z] * rl, 0.0f);
+    if (z * 64 + lane < a.D) ((uint16_t*)a.out)[out * a.D + z * 64 + lane] = (uint16_t)to16<DT>(o[z] * rl, 0.0f);
   if (a.lse && lane == 0) a.lse[out] = row_lse(m, l);
 }
 
 // Row i of (b, h) from n parts, a quarter of them a wave.
-template <typename DT, int TILE>
+template <typename DT, class GEO>
 __device__ __forceinline__ void join_one(const AttnArgs& a, JoinShared& s, int b, int h, int i, int n) {
   const int r = i % a.QB, part = a.QB * a.D;
   const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
@@ -464,7 +472,7 @@ __device__ __forceinline__ void join_one(const AttnArgs& a, JoinShared& s, int b
         const long long at = (long long)s.part[j + y < cn ? c + j + y : c + cn - 1] * part;
 #pragma unroll
         for (int z = 0; z < 4; z++)
-          x[y][z] = z * 64 + lane < a.D ? a.part_o[at + part_at<TILE>(a.D, r, z * 64 + lane)] : 0.0f;
+          x[y][z] = z * 64 + lane < a.D ? a.part_o[at + part_at<GEO>(a.D, r, z * 64 + lane)] : 0.0f;
       }
 #pragma unroll
       for (int y = 0; y < 8; y++) {
@@ -498,15 +506,15 @@ __device__ __forceinline__ void join_one(const AttnArgs& a, JoinShared& s, int b
   write_row<DT>(a, b, h, i, o, top, l);
 }
 
-template <typename DT, int TILE, int R>
+template <typename DT, class GEO, int R>
 __global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
   TGS_STATIC_SMEM(JoinShared, s);
   const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
   const int g = blockIdx.x % groups, bh = blockIdx.x / groups, h = bh % a.Hkv, b = bh / a.Hkv;
   int before, all;
-  tiles_before<TILE>(a, b, before, all);
-  const int nt = cache_tiles<TILE>(a, b) + (a.T + TILE - 1) / TILE;
-  const long long U = (long long)all * a.Hkv, s0 = (long long)before * a.Hkv + (long long)h * (nt + extra<TILE>()), s1 = s0 + nt;
+  tiles_before<GEO>(a, b, before, all);
+  const int nt = cache_tiles<GEO>(a, b) + (a.T + GEO::TILE - 1) / GEO::TILE;
+  const long long U = (long long)all * a.Hkv, s0 = (long long)before * a.Hkv + (long long)h * (nt + GEO::EXTRA), s1 = s0 + nt;
   const int N = a.nwg;
   const int w0 = (int)(((s0 + 1) * N - 1) / U), w1 = (int)((s1 * N - 1) / U);
   if (w0 == w1) return;
@@ -532,7 +540,7 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
   __syncthreads();
   const int n = s.n;
   if constexpr (R == 1) {
-    join_one<DT, TILE>(a, s, b, h, i0, n);
+    join_one<DT, GEO>(a, s, b, h, i0, n);
     return;
   }
   // A lane takes one row and, of the row's D / 4 fours, every sixteenth.
@@ -551,7 +559,7 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
       const float pm = a.part_ml[2ll * (p * a.QB + r)], pl = a.part_ml[2ll * (p * a.QB + r) + 1];
 #pragma unroll
       for (int z = 0; z < 4; z++)
-        if ((sub + 16 * z) * 4 < a.D) x[k][z] = *(const f32x4*)(a.part_o + p * part + part_at<TILE>(a.D, r, (sub + 16 * z) * 4));
+        if ((sub + 16 * z) * 4 < a.D) x[k][z] = *(const f32x4*)(a.part_o + p * part + part_at<GEO>(a.D, r, (sub + 16 * z) * 4));
       f[k] = j + k >= n || pm == NEG ? 0.0f : exp2_hw(pm - m);
       if (j + k < n) l += pm == NEG ? pl : f[k] * pl;  // (a part without weights has the sum 0, or NaN)
     }
@@ -579,13 +587,13 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
 // rows 26.6 : 29.7, 16 with 2,048 50.3 : 49.5, 16 with 4,096 59.5 : 52.8.  The wide
 // kernel's rows, which lie apart in fewer parts, gain from 16 earlier (one
 // sequence of 30,000, 1,280 rows 65.7 : 54.6), which this rule leaves.
-template <typename DT, int TILE>
+template <typename DT, class GEO>
 hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
   if ((long long)a.B * a.Hkv * a.M <= 2048)
-    hipLaunchKernelGGL((join_kernel<DT, TILE, 1>), dim3(a.B * a.Hkv * a.M), dim3(JOIN_NT), 0, st, a, a.M);
+    hipLaunchKernelGGL((join_kernel<DT, GEO, 1>), dim3(a.B * a.Hkv * a.M), dim3(JOIN_NT), 0, st, a, a.M);
   else {
     const int groups = (a.M + 15) / 16;
-    hipLaunchKernelGGL((join_kernel<DT, TILE, 16>), dim3(a.B * a.Hkv * groups), dim3(JOIN_NT), 0, st, a, groups);
+    hipLaunchKernelGGL((join_kernel<DT, GEO, 16>), dim3(a.B * a.Hkv * groups), dim3(JOIN_NT), 0, st, a, groups);
   }
   return hipGetLastError();
 }
@@ -593,7 +601,12 @@ hipError_t launch_join(const AttnArgs& a, hipStream_t st) {
 }  // namespace attn
 
 hipError_t launch_attn_narrow(const AttnArgs& a, int dtype, hipStream_t st);
+hipError_t launch_attn_narrow8(const AttnArgs& a, int dtype, hipStream_t st);
 hipError_t launch_attn_wide(const AttnArgs& a, int dtype, hipStream_t st);
+hipError_t launch_attn_wide8(const AttnArgs& a, int dtype, hipStream_t st);
 hipError_t set_attn_narrow_lds();
+hipError_t set_attn_narrow8_lds();
+hipError_t set_attn_wide_lds();
+hipError_t set_attn_wide8_lds();
 
 }  // namespace tgs

@@ -7,6 +7,7 @@
 // tensors that do not fit, and returns the C ABI's status.
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -24,6 +25,12 @@ decltype(&tgs_tree_attention) p_attention = nullptr;
 decltype(&tgs_kv_append) p_append = nullptr;
 decltype(&tgs_tree_commit) p_commit = nullptr;
 decltype(&tgs_kv_fork) p_fork = nullptr;
+decltype(&tgs_kv_append_rotated) p_append_rotated = nullptr;
+decltype(&tgs_kv8_attention) p_attention8 = nullptr;
+decltype(&tgs_kv8_append) p_append8 = nullptr;
+decltype(&tgs_kv8_commit) p_commit8 = nullptr;
+decltype(&tgs_kv8_fork) p_fork8 = nullptr;
+decltype(&tgs_rotate) p_rotate = nullptr;
 
 struct Raised {};  // a Python error is set
 
@@ -98,42 +105,96 @@ struct Call {
       if (out && p == out) bad_tensor(fn, name, "no input");
   }
 
-  // The cache: keys [layers,] pages, kv_heads, page, D; values [..., page / 8, D, 8].
-  at::ScalarType cache(PyObject* ko, PyObject* vo, bool layered, tgs_kv_cache& c) const {
+  // The cache: keys [layers,] pages, kv_heads, page, D; values [..., page / 8, D, 8], in 16 bits (so: None).  In 8
+  // bits: values [..., page / 16, D, 16] and scales [..., page / 16, 2].
+  struct Cache {
+    tgs_kv_cache c;       // 16 bits
+    tgs_kv8_cache e;      // 8 bits
+    bool eight;
+    at::ScalarType rows;  // of new rows and queries (8 bits: not known here)
+    int32_t layers, kv_heads, page, head_dim;
+  };
+  Cache cache(PyObject* ko, PyObject* vo, PyObject* so, bool layered) const {
+    Cache x;
     const at::Tensor &k = tensor(ko, "k"), &v = tensor(vo, "v");
+    const at::Tensor* sc = maybe(so, "scales");
+    x.eight = sc != nullptr;
+    if (!sc && k.scalar_type() == at::kFloat8_e4m3fn) {
+      PyErr_Format(PyExc_TypeError, "%s: a cache in 8 bits needs its scales", fn);
+      throw Raised{};
+    }
+    const int64_t per = x.eight ? 16 : 8;
     const int f = layered ? 1 : 0;
-    if (k.dim() != 4 + f || v.dim() != 5 + f)
+    if (k.dim() != 4 + f || v.dim() != 5 + f) {
+      if (x.eight)
+        bad(fn, layered ? "k must be [layers, pages, kv_heads, page, D], v [layers, pages, kv_heads, page / 16, D, 16]"
+                        : "k must be [pages, kv_heads, page, D], v [pages, kv_heads, page / 16, D, 16]");
       bad(fn, layered ? "k must be [layers, pages, kv_heads, page, D], v [layers, pages, kv_heads, page / 8, D, 8]"
                       : "k must be [pages, kv_heads, page, D], v [pages, kv_heads, page / 8, D, 8]");
+    }
     const auto ks = k.sizes(), vs = v.sizes(), kt = k.strides(), vt = v.strides();
     if (layered && ks[0] != vs[0]) bad(fn, "k and v differ in layers");
     const int64_t N = ks[f], H = ks[f + 1], page = ks[f + 2], D = ks[f + 3];
-    if (page % 8 || vs[f] != N || vs[f + 1] != H || vs[f + 2] != page / 8 || vs[f + 3] != D || vs[f + 4] != 8)
-      bad(fn, "v must be [..., pages, kv_heads, page / 8, D, 8] for k [..., pages, kv_heads, page, D]");
-    if (kt[f + 1] != page * D || kt[f + 2] != D || kt[f + 3] != 1 || vt[f + 1] != page * D || vt[f + 2] != 8 * D ||
-        vt[f + 3] != 8 || vt[f + 4] != 1)
+    if (page % per || vs[f] != N || vs[f + 1] != H || vs[f + 2] != page / per || vs[f + 3] != D || vs[f + 4] != per)
+      bad(fn, x.eight ? "v must be [..., pages, kv_heads, page / 16, D, 16] for k [..., pages, kv_heads, page, D]"
+                      : "v must be [..., pages, kv_heads, page / 8, D, 8] for k [..., pages, kv_heads, page, D]");
+    if (kt[f + 1] != page * D || kt[f + 2] != D || kt[f + 3] != 1 || vt[f + 1] != page * D || vt[f + 2] != per * D ||
+        vt[f + 3] != per || vt[f + 4] != 1)
       bad(fn, "a page of the cache must be contiguous");
     const at::ScalarType dt = k.scalar_type();
-    if ((dt != at::kBFloat16 && dt != at::kHalf) || v.scalar_type() != dt) {
-      PyErr_Format(PyExc_TypeError, "%s: the cache must be bfloat16 or float16", fn);
+    if (x.eight ? dt != at::kFloat8_e4m3fn || v.scalar_type() != dt || sc->scalar_type() != at::kFloat8_e8m0fnu
+                : (dt != at::kBFloat16 && dt != at::kHalf) || v.scalar_type() != dt) {
+      PyErr_Format(PyExc_TypeError, x.eight ? "%s: a cache with scales must be float8_e4m3fn, its scales float8_e8m0fnu"
+                                            : "%s: the cache must be bfloat16 or float16 (float8_e4m3fn with scales)", fn);
       throw Raised{};
     }
-    if (!here(k) || !here(v)) bad(fn, "the cache must be on the handle's device");
+    if (!here(k) || !here(v) || (sc && !here(*sc))) bad(fn, "the cache must be on the handle's device");
     if ((layered && ks[0] > INT32_MAX) || N > INT32_MAX || H > INT32_MAX || page > INT32_MAX || D > INT32_MAX)
       bad(fn, "a cache dimension beyond 32 bits");
-    c.k = k.data_ptr();
-    c.v = v.data_ptr();
-    c.layers = layered ? (int)ks[0] : 1;
-    c.k_layer = c.layers > 1 ? kt[0] : 0;
-    c.v_layer = c.layers > 1 ? vt[0] : 0;
-    c.k_page = kt[f];
-    c.v_page = vt[f];
-    c.n_pages = (int)N;
-    c.kv_heads = (int)H;
-    c.page = (int)page;
-    c.head_dim = (int)D;
-    c.dtype = dt == at::kHalf ? TGS_F16 : TGS_BF16;
+    x.rows = dt;
+    x.layers = layered ? (int)ks[0] : 1;
+    x.kv_heads = (int)H;
+    x.page = (int)page;
+    x.head_dim = (int)D;
+    const int64_t kl = x.layers > 1 ? kt[0] : 0, vl = x.layers > 1 ? vt[0] : 0;
+    if (!x.eight) {
+      x.c = tgs_kv_cache{k.data_ptr(), v.data_ptr(), kl, kt[f], vl, vt[f], x.layers, (int)N, x.page, x.kv_heads, x.head_dim,
+                         dt == at::kHalf ? TGS_F16 : TGS_BF16};
+      return x;
+    }
+    const auto ss = sc->sizes(), st = sc->strides();
+    if (sc->dim() != 4 + f || (layered && ss[0] != ks[0]) || ss[f] != N || ss[f + 1] != H || ss[f + 2] != page / 16 || ss[f + 3] != 2 ||
+        st[f + 1] != page / 8 || st[f + 2] != 2 || st[f + 3] != 1)
+      bad(fn, "scales must be [..., pages, kv_heads, page / 16, 2] for k [..., pages, kv_heads, page, D], a page of them contiguous");
+    x.e = tgs_kv8_cache{k.data_ptr(), v.data_ptr(), sc->data_ptr(), kl, kt[f], vl, vt[f], x.layers > 1 ? st[0] : 0, st[f],
+                        x.layers, (int)N, x.page, x.kv_heads, x.head_dim};
+    return x;
+  }
+  // The type of new rows: the cache's, or of an 8-bit cache their own.
+  at::ScalarType rows_type(const Cache& x, const at::Tensor& t, const char* name) const {
+    if (!x.eight) return x.rows;
+    const at::ScalarType dt = t.scalar_type();
+    if (dt != at::kBFloat16 && dt != at::kHalf) {
+      PyErr_Format(PyExc_TypeError, "%s: %s must be bfloat16 or float16", fn, name);
+      throw Raised{};
+    }
     return dt;
+  }
+  static tgs_dtype code(at::ScalarType dt) { return dt == at::kHalf ? TGS_F16 : TGS_BF16; }
+  bool flag(PyObject* o) const {
+    const int x = PyObject_IsTrue(o);
+    if (x < 0) throw Raised{};
+    return x != 0;
+  }
+  // The rotation's frequencies (None: none).
+  bool rotary(PyObject* fo, PyObject* po, tgs_rotary& r) const {
+    const at::Tensor* t = maybe(fo, "rotary");
+    r.pairs = flag(po);
+    if (!t) return false;
+    if (t->dim() != 1 || t->size(0) > 65535) bad(fn, "rotary must be float32 [dims / 2]");
+    r.freq = (const float*)exact(*t, "rotary", at::kFloat, {t->size(0)});
+    r.dims = 2 * (int)t->size(0);
+    return true;
   }
   void seqs(PyObject* to, PyObject* lo, tgs_kv_seqs& s) const {
     const at::Tensor& t = tensor(to, "tables");
@@ -226,16 +287,17 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// handle, device, stream, q, k_new, v_new, k, v, tables, lens, parents, max_len (-1: the tables'), scale (None: 1 / sqrt(D)), out, lse
+// handle, device, stream, q, k_new, v_new, k, v, tables, lens, parents, max_len (-1: the tables'), scale (None: 1 / sqrt(D)), out, lse,
+// scales
 PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
-    Call c("tree_attention", a, n, 15);
-    tgs_kv_cache cache;
+    Call c("tree_attention", a, n, 16);
     tgs_kv_rows rows;
     tgs_kv_seqs seqs;
     tgs_attn t;
     const at::Tensor& q = c.tensor(a[3], "q");
-    const at::ScalarType dt = c.cache(a[6], a[7], false, cache);
+    const Call::Cache cache = c.cache(a[6], a[7], a[15], false);
+    const at::ScalarType dt = c.rows_type(cache, q, "q");
     c.seqs(a[8], a[9], seqs);
     if (q.dim() != 4 || q.size(1) > INT32_MAX || q.size(2) > INT32_MAX) bad(c.fn, "q must be [B, T, q_heads, D]");
     const int64_t B = seqs.B, T = q.size(1), Hq = q.size(2), H = cache.kv_heads, D = cache.head_dim;
@@ -255,37 +317,44 @@ PyObject* tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor* lse = c.maybe(a[14], "lse");
     t.lse = lse ? (float*)c.exact(*lse, "lse", at::kFloat, {B, T, Hq}) : nullptr;
     c.apart(t.out, "out", {t.q, rows.k, rows.v});
-    return p_attention(c.h, &cache, &rows, &seqs, &t, c.stream);
+    if (cache.eight) return p_attention8(c.h, &cache.e, Call::code(dt), &rows, &seqs, &t, c.stream);
+    return p_attention(c.h, &cache.c, &rows, &seqs, &t, c.stream);
   });
 }
 
-// handle, device, stream, k_new, v_new, k, v, tables, lens, counts, lens_out
+// handle, device, stream, k_new, v_new, k, v, tables, lens, counts, lens_out, scales, rotary, pairs
 PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
-    Call c("kv_append", a, n, 11);
-    tgs_kv_cache cache;
+    Call c("kv_append", a, n, 14);
     tgs_kv_rows rows;
     tgs_kv_seqs seqs;
-    const at::ScalarType dt = c.cache(a[5], a[6], true, cache);
-    c.seqs(a[7], a[8], seqs);
+    tgs_rotary rot;
+    const Call::Cache cache = c.cache(a[5], a[6], a[11], true);
     const int64_t T = c.nodes(a[3]);
+    const at::ScalarType dt = c.rows_type(cache, c.tensor(a[3], "k_new"), "k_new");
+    c.seqs(a[7], a[8], seqs);
+    const bool turns = c.rotary(a[12], a[13], rot);
     c.new_rows(a[3], a[4], dt, {cache.layers, seqs.B, T, cache.kv_heads, cache.head_dim}, rows);
     int32_t *counts = c.ints_or_null(a[9], "counts", {seqs.B}), *out = c.ints(a[10], "lens_out", {seqs.B});
     c.apart(out, "lens_out", {seqs.lens, seqs.tables, counts});
-    return p_append(c.h, &cache, &rows, &seqs, (int)T, counts, out, c.stream);
+    if (cache.eight)
+      return p_append8(c.h, &cache.e, Call::code(dt), &rows, &seqs, (int)T, counts, turns ? &rot : nullptr, out, c.stream);
+    if (turns) return p_append_rotated(c.h, &cache.c, &rows, &seqs, (int)T, counts, &rot, out, c.stream);
+    return p_append(c.h, &cache.c, &rows, &seqs, (int)T, counts, out, c.stream);
   });
 }
 
-// handle, device, stream, k_new, v_new, k, v, tables, lens, parents, draft, sampled, out n_acc, tokens, path, lens
+// handle, device, stream, k_new, v_new, k, v, tables, lens, parents, draft, sampled, out n_acc, tokens, path, lens, scales
 PyObject* tree_commit(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
-    Call c("tree_commit", a, n, 16);
-    tgs_kv_cache cache;
+    Call c("tree_commit", a, n, 17);
     tgs_kv_rows rows;
     tgs_kv_seqs seqs;
-    const at::ScalarType dt = c.cache(a[5], a[6], true, cache);
+    const Call::Cache cache = c.cache(a[5], a[6], a[16], true);
+    const int64_t T = c.nodes(a[3]);
+    const at::ScalarType dt = c.rows_type(cache, c.tensor(a[3], "k_new"), "k_new");
     c.seqs(a[7], a[8], seqs);
-    const int64_t B = seqs.B, T = c.nodes(a[3]);
+    const int64_t B = seqs.B;
     c.new_rows(a[3], a[4], dt, {cache.layers, B, T, cache.kv_heads, cache.head_dim}, rows);
     int32_t *par = c.ints(a[9], "parents", {B, T}), *draft = c.ints(a[10], "draft", {B, T}),
             *smp = c.ints(a[11], "sampled", {B, T});
@@ -294,23 +363,72 @@ PyObject* tree_commit(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const char* names[] = {"out n_acc", "out tokens", "out path", "out lens"};
     int32_t* outs[] = {acc, tok, path, lens};
     for (int i = 0; i < 4; i++) c.apart(outs[i], names[i], {seqs.lens, seqs.tables, par, draft, smp});
-    return p_commit(c.h, &cache, &rows, &seqs, (int)T, par, draft, smp, acc, tok, path, lens, c.stream);
+    if (cache.eight)
+      return p_commit8(c.h, &cache.e, Call::code(dt), &rows, &seqs, (int)T, par, draft, smp, acc, tok, path, lens, c.stream);
+    return p_commit(c.h, &cache.c, &rows, &seqs, (int)T, par, draft, smp, acc, tok, path, lens, c.stream);
   });
 }
 
-// handle, device, stream, k, v, tables, lens, parents, room, tables_out, lens_out
+// handle, device, stream, k, v, tables, lens, parents, room, tables_out, lens_out, scales
 PyObject* kv_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&] {
-    Call c("kv_fork", a, n, 11);
-    tgs_kv_cache cache;
+    Call c("kv_fork", a, n, 12);
     tgs_kv_seqs seqs;
-    c.cache(a[3], a[4], true, cache);
+    const Call::Cache cache = c.cache(a[3], a[4], a[11], true);
     c.seqs(a[5], a[6], seqs);
     int32_t* par = c.ints(a[7], "parents", {seqs.B});
     int32_t *tab = c.ints(a[9], "tables_out", {seqs.B, seqs.width}), *lens = c.ints(a[10], "lens_out", {seqs.B});
     c.apart(tab, "tables_out", {seqs.lens, seqs.tables, par});
     c.apart(lens, "lens_out", {seqs.lens, seqs.tables, par});
-    return p_fork(c.h, &cache, &seqs, par, (int)c.number(a[8]), tab, lens, c.stream);
+    const int room = (int)c.number(a[8]);
+    if (cache.eight) return p_fork8(c.h, &cache.e, &seqs, par, room, tab, lens, c.stream);
+    return p_fork(c.h, &cache.c, &seqs, par, room, tab, lens, c.stream);
+  });
+}
+
+// handle, device, stream, q, k (None: none), lens, rotary, pairs, parents, q_out, k_out
+PyObject* rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    Call c("rotate", a, n, 11);
+    const at::Tensor& q = c.tensor(a[3], "q");
+    const at::Tensor* k = c.maybe(a[4], "k_new");
+    if (q.dim() != 4 || q.size(0) > INT32_MAX || q.size(1) > INT32_MAX || q.size(2) > INT32_MAX || q.size(3) > INT32_MAX)
+      bad(c.fn, "q must be [B, T, q_heads, D]");
+    const at::ScalarType dt = q.scalar_type();
+    if (dt != at::kBFloat16 && dt != at::kHalf) {
+      PyErr_SetString(PyExc_TypeError, "rotate: q must be bfloat16 or float16");
+      throw Raised{};
+    }
+    const int64_t B = q.size(0), T = q.size(1), D = q.size(3);
+    tgs_rotary rot;
+    if (!c.rotary(a[6], a[7], rot)) bad(c.fn, "rotary must be a tensor");
+    const int32_t *lens = c.ints(a[5], "lens", {B}), *parents = c.ints_or_null(a[8], "parents", {B, T});
+    auto fill = [&](const at::Tensor& x, const char* name, PyObject* oo, const char* oname, tgs_rotate_rows& r) -> const at::Tensor& {
+      if (x.dim() != 4 || x.size(2) > INT32_MAX) bad_tensor(c.fn, name, "[B, T, heads, D]");
+      const at::Tensor& o = c.tensor(oo, oname);
+      for (const at::Tensor* t : {&x, &o})
+        if (t->scalar_type() != dt || t->sizes() != at::IntArrayRef({B, T, x.size(2), D}) || t->stride(3) != 1 || !c.here(*t))
+          bad_tensor(c.fn, t == &x ? name : oname, "of q's type and device and of the shape [B, T, heads, D], its last dimension contiguous");
+      if (at::has_internal_overlap(o) == at::MemOverlap::Yes) bad_tensor(c.fn, oname, "rows of their own (no expanded dimension)");
+      r = tgs_rotate_rows{x.data_ptr(), o.data_ptr(), x.stride(0), x.stride(1), x.stride(2), o.stride(0), o.stride(1), o.stride(2), (int)x.size(2)};
+      return o;
+    };
+    auto apart = [&](const at::Tensor& o, const char* oname, const at::Tensor& x) {
+      const auto st = at::get_overlap_status(o, x);
+      if (o.numel() && (o.data_ptr() == x.data_ptr() || st == at::MemOverlapStatus::Partial || st == at::MemOverlapStatus::Full))
+        bad_tensor(c.fn, oname, "apart from the other tensors (or its input itself)");
+    };
+    tgs_rotate_rows rq, rk;
+    const at::Tensor& qo = fill(q, "q", a[9], "q_out", rq);
+    if (rq.x != rq.out) apart(qo, "q_out", q);
+    if (k) {
+      const at::Tensor& ko = fill(*k, "k_new", a[10], "k_out", rk);
+      if (rk.x != rk.out) apart(ko, "k_out", *k);
+      apart(qo, "q_out", *k);
+      apart(qo, "q_out", ko);
+      apart(ko, "k_out", q);
+    }
+    return p_rotate(c.h, Call::code(dt), &rq, k ? &rk : nullptr, (int)B, (int)T, (int)D, lens, parents, &rot, c.stream);
   });
 }
 
@@ -328,7 +446,14 @@ PyObject* bind(PyObject*, PyObject* path) {
   p_append = (decltype(p_append))dlsym(lib, "tgs_kv_append");
   p_commit = (decltype(p_commit))dlsym(lib, "tgs_tree_commit");
   p_fork = (decltype(p_fork))dlsym(lib, "tgs_kv_fork");
-  if (!p_beam || !p_attention || !p_append || !p_commit || !p_fork) {
+  p_append_rotated = (decltype(p_append_rotated))dlsym(lib, "tgs_kv_append_rotated");
+  p_attention8 = (decltype(p_attention8))dlsym(lib, "tgs_kv8_attention");
+  p_append8 = (decltype(p_append8))dlsym(lib, "tgs_kv8_append");
+  p_commit8 = (decltype(p_commit8))dlsym(lib, "tgs_kv8_commit");
+  p_fork8 = (decltype(p_fork8))dlsym(lib, "tgs_kv8_fork");
+  p_rotate = (decltype(p_rotate))dlsym(lib, "tgs_rotate");
+  if (!p_beam || !p_attention || !p_append || !p_commit || !p_fork || !p_append_rotated || !p_attention8 || !p_append8 ||
+      !p_commit8 || !p_fork8 || !p_rotate) {
     PyErr_Format(PyExc_RuntimeError, "%s lacks an entry point: build it again", p);
     return nullptr;
   }
@@ -342,6 +467,7 @@ PyMethodDef methods[] = {
     {"kv_append", (PyCFunction)(void (*)(void))kv_append, METH_FASTCALL, nullptr},
     {"tree_commit", (PyCFunction)(void (*)(void))tree_commit, METH_FASTCALL, nullptr},
     {"kv_fork", (PyCFunction)(void (*)(void))kv_fork, METH_FASTCALL, nullptr},
+    {"rotate", (PyCFunction)(void (*)(void))rotate, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_cache_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -38,9 +38,31 @@ struct KvWriteArgs {
   int* path;    // [B][T]
   int* lens_out;  // [B]
   FastDiv half_d, chunks, heads;  // head_dim / 2, head_dim / 8, kv_heads
+  FastDiv units;                  // 16 dimensions each, the last one perhaps 8
+  // 8-bit caches (c's strides in bytes, c.dtype: that of the rows)
+  uint8_t* scales;
+  long long s_layer, s_page;
+  tgs_rotary rot;  // of the keys; freq nullptr: none
 };
 hipError_t launch_kv_append(const KvWriteArgs& a, hipStream_t st);
 hipError_t launch_tree_commit(const KvWriteArgs& a, hipStream_t st);
+hipError_t launch_kv_append_rotated(const KvWriteArgs& a, hipStream_t st);
+hipError_t launch_kv8_append(const KvWriteArgs& a, hipStream_t st);
+hipError_t launch_kv8_commit(const KvWriteArgs& a, hipStream_t st);
+
+// Queries and keys of drafted nodes turned by their positions.
+constexpr int ROTARY_MAX = 256;  // dimensions that turn, at most
+constexpr int ROTATE_TOKENS = 4;  // of a workgroup, where there are many
+struct RotateArgs {
+  tgs_rotate_rows q, k;
+  const int* lens;     // [B]
+  const int* parents;  // [B][T] or nullptr (a chain)
+  tgs_rotary rot;
+  int B, T, D, dtype;
+  int tokens;  // of a workgroup: 1 or ROTATE_TOKENS
+  FastDiv units, heads;  // of a row; of queries and keys together
+};
+hipError_t launch_rotate(const RotateArgs& a, hipStream_t st);
 
 struct KvForkArgs {
   tgs_kv_cache c;
@@ -52,7 +74,9 @@ struct KvForkArgs {
   int R, P, room, page_shift;
   int* owner;          // [n_pages] workspace, for pools beyond the planning kernel's LDS
   int* fresh;          // [n_pages] workspace, likewise: the free pages, in order
-  int4* copies;        // [R] workspace: source page, new page, 8-token blocks, -
+  int4* copies;        // [R] workspace: source page, new page, blocks, -
+  uint8_t* scales;     // 8-bit caches (c's strides in bytes): blocks of 16 tokens, else of 8
+  long long s_layer, s_page;
 };
 size_t kv_fork_lds(int n_pages, int rows);  // dynamic LDS of the planning kernel (0: its lists lie in the workspace)
 hipError_t launch_kv_fork(const KvForkArgs& a, int num_cu, hipStream_t st);
@@ -104,15 +128,18 @@ struct AttnArgs {
   int nwg;             // workers per row group: each takes an even share of the tiles; 0: one workgroup per (sequence, head)
   float* part_o;       // [nqb * nwg][2][QB][D]
   float* part_ml;      // [nqb * nwg][2][QB][2]
+  const uint8_t* scales;  // 8-bit caches: of the layer (k, v and k_page, v_page in bytes); nullptr: a 16-bit cache
+  long long s_page;
 };
 struct AttnPlan {
   int wide;   // 0: a wave owns its tiles; 1: tiles shared through LDS
+  int e8;     // whether the cache holds 8 bits
   int tile;   // tokens of a unit of work
   int QB, nqb;
   int per_cu;  // workgroups that a CU holds
   int least;   // tiles worth a worker of their own
 };
-AttnPlan attn_plan(int M, int D);
+AttnPlan attn_plan(int M, int D, bool e8);
 hipError_t launch_attn(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st);
 hipError_t set_attn_lds();  // dynamic LDS of the attention kernels
 

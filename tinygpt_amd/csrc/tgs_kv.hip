@@ -8,37 +8,24 @@
 // tokens, 16 layers, 176 us (923 MB, 5.2 TB/s read and written); pages of 128
 // forked beams 94 us (403 MB, 4.3 TB/s).
 #include "tgs_device.h"
+#include "tgs_e8.h"
 #include "tgs_kv.h"
+#include "tgs_kv_write.h"
 #include "tgs_row.h"
 
 namespace tgs {
 namespace kv {
 
-__device__ __forceinline__ unsigned div_by(unsigned x, FastDiv f) { return f.d == 1 ? x : __umulhi(x, f.m); }
-
+// ROT: void, or the type of the keys that are turned.
+template <class ROT>
 struct WriteShared {
-  int path[KV_MAX_NODES];
-  int n;
+  WriteHead head;
+  e8::Turn cs[8][ROTARY_MAX / 2];
 };
-
-// The accepted path of a tree by one wave, node j in lane j: from the root on,
-// the lowest child whose drafted token is the one sampled at its parent.
-// Children come after their parents, so each step moves to a higher node and
-// the walk ends.  Returns the nodes taken, the root among them.
-__device__ __forceinline__ int accept_walk(const int* parents, const int* draft, const int* sampled, int T, int* path) {
-  const int lane = lane_id();
-  const bool in = lane < T;
-  const int par = in ? parents[lane] : -2, tok = in ? draft[lane] : 0, smp = in ? sampled[lane] : 0;
-  int cur = 0, n = 0;
-  while (true) {
-    if (lane == n) path[n] = cur;
-    n++;
-    const int want = (int)readlane_u32((uint32_t)smp, cur);
-    const u64 fits = __ballot(in && lane > cur && par == cur && tok == want);
-    if (fits == 0) return n;
-    cur = __ffsll((long long)fits) - 1;
-  }
-}
+template <>
+struct WriteShared<void> {
+  WriteHead head;
+};
 
 // Workgroup (x, sequence b, layer l) over the 8-token blocks x, x + nblk, ...
 // of the positions that b's new rows take.  Keys move as 16-byte vectors.  A
@@ -48,47 +35,17 @@ __device__ __forceinline__ int accept_walk(const int* parents, const int* draft,
 // A block that the rows cover in part is read, filled in and written whole: 16
 // bytes a d instead of 2-byte stores 16 bytes apart, of which every one costs
 // the cache a line (64 trees of 63 nodes, 32 layers: 45 us, was 59).
-template <bool COMMIT>
+// Keys that turn (ROT) go by units of two chunks, with the cosines and sines of the
+// block's positions in LDS.
+template <bool COMMIT, class ROT>
 __global__ __launch_bounds__(KV_NT) void write_kernel(KvWriteArgs a) {
-  TGS_STATIC_SMEM(WriteShared, s);
+  TGS_STATIC_SMEM(WriteShared<ROT>, sh);
+  WriteHead& s = sh.head;
   const int x = blockIdx.x % a.nblk, bl = blockIdx.x / a.nblk, b = bl % a.B, l = bl / a.B;
   const int tid = threadIdx.x;
-  const int len = a.lens[b];
-  int n;
-  if constexpr (COMMIT) {
-    if (tid < 64) {
-      const int cnt = accept_walk(a.parents + (long long)b * a.T, a.draft + (long long)b * a.T,
-                                  a.sampled + (long long)b * a.T, a.T, s.path);
-      if (tid == 0) s.n = cnt;
-    }
-    __syncthreads();
-    n = s.n;
-  } else {
-    n = a.counts ? a.counts[b] : a.T;
-  }
-  // what does not fit is not written: a count outside [0, T], positions past
-  // the table, pages outside the pool
-  int bad = n < 0 || n > a.T || len < 0 || (long long)len + n > ((long long)a.P << a.page_shift);
+  int len, n;
+  if (!write_head<COMMIT>(a, s, b, l == 0 && x == 0, len, n)) return;
   const int* table = a.tables + (long long)b * a.P;
-  if (!bad && n > 0)
-    for (int i = (len >> a.page_shift) + tid; i <= (len + n - 1) >> a.page_shift; i += KV_NT)
-      bad |= (unsigned)table[i] >= (unsigned)a.c.n_pages;
-  bad = __syncthreads_or(bad);
-  if (l == 0 && x == 0) {
-    if (tid == 0) {
-      a.lens_out[b] = bad ? -1 : len + n;
-      if (COMMIT) a.n_acc[b] = n - 1;
-    }
-    if (COMMIT && tid < a.T) {
-      const long long o = (long long)b * a.T;
-      a.path[o + tid] = tid < n ? s.path[tid] : -1;
-      int t = -1;  // the accepted nodes' tokens, then the one sampled at the last
-      if (tid < n - 1) t = a.draft[o + s.path[tid + 1]];
-      if (tid == n - 1) t = a.sampled[o + s.path[tid]];
-      a.tokens[o + tid] = t;
-    }
-  }
-  if (bad || n == 0) return;
   const int D = a.c.head_dim, H = a.c.kv_heads, page = 1 << a.page_shift;
   const uint16_t* kn = (const uint16_t*)a.r.k + l * a.r.k_layer + b * a.r.k_seq;
   const uint16_t* vn = (const uint16_t*)a.r.v + l * a.r.v_layer + b * a.r.v_seq;
@@ -101,6 +58,34 @@ __global__ __launch_bounds__(KV_NT) void write_kernel(KvWriteArgs a) {
     uint16_t* kp = (uint16_t*)a.c.k + l * a.c.k_layer + pg * a.c.k_page + (long long)(t0 & (page - 1)) * D;
     uint16_t* vp = (uint16_t*)a.c.v + l * a.c.v_layer + pg * a.c.v_page + (long long)(pos0 & (page - 1)) * D;
     const int C = D >> 3;
+    if constexpr (!__is_same(ROT, void)) {
+      const int half = a.rot.dims >> 1, U = e8::units(D);
+      __syncthreads();  // (the block before is done with the table)
+      for (int e = tid; e < nt * half; e += KV_NT) {
+        const int i = e / half, j = e - i * half;
+        sh.cs[i][j] = e8::turn((uint32_t)(t0 + i), a.rot.freq[j]);
+      }
+      __syncthreads();
+      for (int e = tid; e < nt * H * U; e += KV_NT) {  // (token, head, unit)
+        const unsigned row = div_by((unsigned)e, a.units), u = (unsigned)e - row * U;
+        const int i = div_by(row, a.heads), h = row - i * H;
+        const uint16_t* from = kn + (t0 - len + i) * a.r.k_tok + h * a.r.k_head;
+        uint16_t* to = kp + ((long long)h * page + i) * D;
+        const e8::Unit w = e8::unit_of((int)u, D, a.rot.dims, a.rot.pairs);
+        const uint4 lo = load_row16<false>(from + w.a), hi = w.b >= 0 ? load_row16<false>(from + w.b) : lo;
+        if (w.angle < 0) {
+          *(uint4*)(to + w.a) = lo;
+          if (w.b >= 0) *(uint4*)(to + w.b) = hi;
+          continue;
+        }
+        float y[16];
+        e8::widen<ROT>(lo, y);
+        e8::widen<ROT>(hi, y + 8);
+        e8::turn_unit(y, sh.cs[i] + w.angle, a.rot.pairs);
+        *(uint4*)(to + w.a) = e8::narrow<ROT>(y);
+        *(uint4*)(to + w.b) = e8::narrow<ROT>(y + 8);
+      }
+    } else
     for (int e = tid; e < nt * H * C; e += KV_NT) {  // 16-byte vectors of keys: (token, head, chunk)
       const unsigned row = div_by((unsigned)e, a.chunks), ch = (unsigned)e - row * C;
       const int i = div_by(row, a.heads), h = row - i * H;
@@ -304,7 +289,7 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
       if (!((unsigned)p < (unsigned)N && owner_get<LDS>(owner, p) == r * P + i)) {
         to = fits ? fresh[next++] : -1;
         const int held = w.len - (i << a.page_shift);
-        if (held > 0 && fits) copy = make_int4(p, to, (held + 7) >> 3, 0);
+        if (held > 0 && fits) copy = make_int4(p, to, a.scales ? (held + e8::BLOCK - 1) / e8::BLOCK : (held + 7) >> 3, 0);
       }
       if (out) to_row[i] = to;
     }
@@ -322,20 +307,32 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
 }
 
 // The blocks of row r's page that are in use lie contiguous per head: copies
-// those of layer y / 2, keys or values.
+// those of layer y / 2, keys or values (and with them their scales).  A block's
+// vectors of 16 bytes are as many as a head has dimensions, of 8 tokens in 16
+// bits or of 16 in 8.
 __device__ __forceinline__ void copy_page(const KvForkArgs& a, const int4& c, int y) {
   if (c.z == 0) return;
   const int l = y >> 1, D = a.c.head_dim, H = a.c.kv_heads;
   const bool val = y & 1;
-  uint16_t* pool = (uint16_t*)(val ? a.c.v : a.c.k) + l * (val ? a.c.v_layer : a.c.k_layer);
-  const long long ps = val ? a.c.v_page : a.c.k_page;
+  const int bytes = a.scales ? 1 : 2, per = a.scales ? e8::BLOCK : 8;
+  unsigned char* pool = (unsigned char*)(val ? a.c.v : a.c.k) + l * (val ? a.c.v_layer : a.c.k_layer) * bytes;
+  const long long ps = (val ? a.c.v_page : a.c.k_page) * bytes;
   const uint4* from = (const uint4*)(pool + c.x * ps);
   uint4* to = (uint4*)(pool + c.y * ps);
-  const int n = c.z * D;  // 16-byte vectors of a head's blocks
-  const int hs = D << a.page_shift >> 3;  // and of its page
+  const int n = c.z * D;  // vectors of a head's blocks
+  const int blocks = (1 << a.page_shift) / per;
   // a wave a head, so that every thread has work where a head's blocks are few
-  for (int h = threadIdx.x >> 6; h < H; h += blockDim.x >> 6)
-    for (int i = lane_id(); i < n; i += 64) to[(long long)h * hs + i] = from[(long long)h * hs + i];
+  for (int h = threadIdx.x >> 6; h < H; h += blockDim.x >> 6) {
+    for (int i = lane_id(); i < n; i += 64) to[((long long)h * blocks) * D + i] = from[((long long)h * blocks) * D + i];
+    if (a.scales) {
+      const uint8_t* sc = a.scales + l * a.s_layer;
+      uint8_t* st = a.scales + l * a.s_layer;
+      for (int i = lane_id(); i < c.z; i += 64) {
+        const long long at = ((long long)h * blocks + i) * 2 + val;
+        st[c.y * a.s_page + at] = sc[c.x * a.s_page + at];
+      }
+    }
+  }
 }
 
 template <bool LDS>
@@ -362,12 +359,21 @@ __global__ __launch_bounds__(KV_PLAN_NT) void fork_kernel(KvForkArgs a) {
 }  // namespace kv
 
 hipError_t launch_kv_append(const KvWriteArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(kv::write_kernel<false>, dim3(a.nblk * a.B * a.c.layers), dim3(KV_NT), 0, st, a);
+  hipLaunchKernelGGL((kv::write_kernel<false, void>), dim3(a.nblk * a.B * a.c.layers), dim3(KV_NT), 0, st, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_append_rotated(const KvWriteArgs& a, hipStream_t st) {
+  const dim3 grid(a.nblk * a.B * a.c.layers);
+  if (a.c.dtype == TGS_BF16)
+    hipLaunchKernelGGL((kv::write_kernel<false, e8::BF16>), grid, dim3(KV_NT), 0, st, a);
+  else
+    hipLaunchKernelGGL((kv::write_kernel<false, e8::F16>), grid, dim3(KV_NT), 0, st, a);
   return hipGetLastError();
 }
 
 hipError_t launch_tree_commit(const KvWriteArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(kv::write_kernel<true>, dim3(a.nblk * a.B * a.c.layers), dim3(KV_NT), 0, st, a);
+  hipLaunchKernelGGL((kv::write_kernel<true, void>), dim3(a.nblk * a.B * a.c.layers), dim3(KV_NT), 0, st, a);
   return hipGetLastError();
 }
 

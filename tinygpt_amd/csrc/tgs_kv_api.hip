@@ -1,4 +1,4 @@
-// tgs_kv_api.hip -- host side of the beam, tree-attention and paged-cache
+// tgs_kv_api.hip -- host side of the beam, tree-attention, paged-cache and rotation
 // entry points of include/tgs_sampler.h: argument checks, the split of the
 // work and the launches.  Nothing here allocates or synchronises.
 #include <hip/hip_runtime.h>
@@ -40,6 +40,33 @@ int check_cache(tgs_ctx* h, const tgs_kv_cache* c) {
   return TGS_OK;
 }
 
+// The same of a cache held in 8 bits, as a block of the 16-bit form's kind with
+// strides in bytes (dtype: that of the rows).
+int check_cache8(tgs_ctx* h, const tgs_kv8_cache* c, tgs_dtype dt, tgs_kv_cache& out) {
+  if (!c || !c->k || !c->v || !c->scales) return fail(h, TGS_EINVAL, "cache: null buffer");
+  if (dt != TGS_BF16 && dt != TGS_F16) return fail(h, TGS_EINVAL, "rows: dtype (bf16 or fp16)");
+  if (c->page < 16 || c->page > 1024 || (c->page & (c->page - 1)))
+    return fail(h, TGS_EINVAL, "8-bit cache: a page holds a power of two of tokens, 16 to 1024");
+  if (c->layers < 1 || c->n_pages < 1 || c->kv_heads < 1 || c->head_dim < 16 || c->head_dim % 16 || c->head_dim > 256 ||
+      (int64_t)c->kv_heads * c->head_dim > 65535)
+    return fail(h, TGS_EINVAL, "8-bit cache: shape");
+  const int64_t whole = (int64_t)c->kv_heads * c->page * c->head_dim, scales = (int64_t)c->kv_heads * c->page / 8;
+  if (c->k_page < whole || c->v_page < whole || c->k_page % 16 || c->v_page % 16 || c->k_layer % 16 || c->v_layer % 16 ||
+      c->k_layer < 0 || c->v_layer < 0 || !aligned16(c->k) || !aligned16(c->v) || c->s_page < scales || c->s_page % 2 ||
+      c->s_layer < 0 || c->s_layer % 2 || (uintptr_t)c->scales % 2)
+    return fail(h, TGS_EINVAL, "8-bit cache: strides and alignment");
+  out = tgs_kv_cache{c->k, c->v, c->k_layer, c->k_page, c->v_layer, c->v_page, c->layers, c->n_pages,
+                     c->page, c->kv_heads, c->head_dim, (int32_t)dt};
+  return TGS_OK;
+}
+
+int check_rotary(tgs_ctx* h, const tgs_rotary* r, int head_dim) {
+  if (!r || !r->freq) return fail(h, TGS_EINVAL, "rotation: null buffer");
+  if (r->dims < 16 || r->dims % 16 || r->dims > tgs::ROTARY_MAX || r->dims > head_dim)
+    return fail(h, TGS_EINVAL, "rotation: dims a multiple of 16, 16 to 256, at most head_dim");
+  return TGS_OK;
+}
+
 int check_seqs(tgs_ctx* h, const tgs_kv_cache* c, const tgs_kv_seqs* s) {
   if (!s || s->B < 0 || s->width < 1 || (int64_t)s->width * c->page > INT32_MAX)
     return fail(h, TGS_EINVAL, "sequences: shape");
@@ -63,7 +90,6 @@ int raise_lds(tgs_ctx* h) {
 
 int write_args(tgs_ctx* h, const tgs_kv_cache* c, const tgs_kv_rows* r, const tgs_kv_seqs* s, int T, int32_t* lens_out,
                tgs::KvWriteArgs& a) {
-  if (int rc = check_cache(h, c)) return rc;
   if (int rc = check_seqs(h, c, s)) return rc;
   if (T < 1) return fail(h, TGS_EINVAL, "rows: at least one per sequence");
   std::memset(&a, 0, sizeof(a));
@@ -82,6 +108,161 @@ int write_args(tgs_ctx* h, const tgs_kv_cache* c, const tgs_kv_rows* r, const tg
   a.half_d = tgs::fast_div(c->head_dim / 2);
   a.chunks = tgs::fast_div(c->head_dim / 8);
   a.heads = tgs::fast_div(c->kv_heads);
+  a.units = tgs::fast_div((c->head_dim + 15) / 16);
+  return TGS_OK;
+}
+
+// Rows of new tokens: workgroups per (sequence, layer) and the launch.
+template <class F>
+int append(tgs_ctx* h, tgs::KvWriteArgs& a, const int32_t* d_counts, int block, F launch) {
+  a.counts = d_counts;
+  // blocks that T rows, or as many as a table holds, lie in at most
+  a.nblk = a.T == 1 ? 1 : (int)((std::min<int64_t>(a.T, (int64_t)a.P * a.c.page) + block - 1) / block + 1);
+  if ((int64_t)a.nblk * a.B * a.c.layers > INT32_MAX) return fail(h, TGS_ETOOBIG, "rows");
+  DeviceGuard g(h->device);
+  if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
+  hipError_t e = launch(a);
+  if (e != hipSuccess) return hip_fail(h, e, "append kernel launch");
+  return TGS_OK;
+}
+
+template <class F>
+int commit(tgs_ctx* h, tgs::KvWriteArgs& a, const int32_t* d_parents, const int32_t* d_draft, const int32_t* d_sampled,
+           int32_t* d_n_acc, int32_t* d_tokens, int32_t* d_path, F launch) {
+  if (!d_parents || !d_draft || !d_sampled || !d_n_acc || !d_tokens || !d_path)
+    return fail(h, TGS_EINVAL, "null buffer");
+  a.parents = d_parents;
+  a.draft = d_draft;
+  a.sampled = d_sampled;
+  a.n_acc = d_n_acc;
+  a.tokens = d_tokens;
+  a.path = d_path;
+  a.nblk = a.T < 3 ? 1 : 2;  // (a path is seldom longer than two blocks)
+  if ((int64_t)a.nblk * a.B * a.c.layers > INT32_MAX) return fail(h, TGS_ETOOBIG, "rows");
+  DeviceGuard g(h->device);
+  if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
+  hipError_t e = launch(a);
+  if (e != hipSuccess) return hip_fail(h, e, "commit kernel launch");
+  return TGS_OK;
+}
+
+void set_scales(tgs::KvWriteArgs& a, const tgs_kv8_cache* c) {
+  a.scales = (uint8_t*)c->scales;
+  a.s_layer = c->s_layer;
+  a.s_page = c->s_page;
+}
+
+// scales: of a cache held in 8 bits (cache's strides in bytes), else nullptr.
+int attention(tgs_ctx* h, const tgs_kv_cache& cache, const uint8_t* scales, int64_t s_page, const tgs_kv_rows* rows,
+              const tgs_kv_seqs* seqs, const tgs_attn* attn, tgs_stream stream) {
+  if (int rc = check_seqs(h, &cache, seqs)) return rc;
+  if (!attn || !rows) return fail(h, TGS_EINVAL, "null argument");
+  const int D = cache.head_dim, T = attn->T, B = seqs->B;
+  if (cache.layers != 1) return fail(h, TGS_EINVAL, "attention: one layer of the cache");
+  if (D != 64 && D != 96 && D != 128 && D != 256) return fail(h, TGS_EINVAL, "attention: head_dim 64, 96, 128 or 256");
+  if (T < 1 || T > tgs::KV_MAX_NODES) return fail(h, TGS_EINVAL, "attention: 1 to 64 nodes");
+  if (attn->q_heads < 1 || attn->q_heads % cache.kv_heads)
+    return fail(h, TGS_EINVAL, "attention: query heads a multiple of key heads");
+  if (!(attn->scale > 0.0f) || !(attn->scale < 1e30f) || attn->max_len < 0)
+    return fail(h, TGS_EINVAL, "attention: scale and max_len");
+  if (B == 0) return TGS_OK;
+  if (!attn->q || !attn->out || !rows->k || !rows->v) return fail(h, TGS_EINVAL, "null buffer");
+  if (!aligned16(attn->out)) return fail(h, TGS_EINVAL, "attention: out must be 16-byte aligned");
+  if ((int64_t)B * cache.kv_heads * T * (attn->q_heads / cache.kv_heads) > INT32_MAX)
+    return fail(h, TGS_ETOOBIG, "attention: rows");
+  DeviceGuard g(h->device);
+  if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
+  if (int rc = raise_lds(h)) return rc;
+  tgs::AttnArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.q = attn->q;
+  a.k_new = rows->k;
+  a.v_new = rows->v;
+  a.q_b = attn->q_seq, a.q_t = attn->q_tok, a.q_h = attn->q_head;
+  a.kn_b = rows->k_seq, a.kn_t = rows->k_tok, a.kn_h = rows->k_head;
+  a.vn_b = rows->v_seq, a.vn_t = rows->v_tok, a.vn_h = rows->v_head;
+  a.k = cache.k;
+  a.v = cache.v;
+  a.k_page = cache.k_page;
+  a.v_page = cache.v_page;
+  a.tables = seqs->tables;
+  a.lens = seqs->lens;
+  a.parents = attn->parents;
+  a.out = attn->out;
+  a.lse = attn->lse;
+  a.B = B;
+  a.T = T;
+  a.Hq = attn->q_heads;
+  a.Hkv = cache.kv_heads;
+  a.G = a.Hq / a.Hkv;
+  a.D = D;
+  a.P = seqs->width;
+  a.n_pages = cache.n_pages;
+  a.page_shift = shift_of(cache.page);
+  a.scale_log2 = attn->scale * 1.4426950408889634f;
+  a.M = T * a.G;
+  a.scales = scales;
+  a.s_page = s_page;
+  const tgs::AttnPlan p = tgs::attn_plan(a.M, D, scales != nullptr);
+  a.QB = p.QB;
+  a.nqb = p.nqb;
+  // Workers: as many as the chip holds at once, of at least p.least tiles, as
+  // far as the workspace has room for their parts.  Where every (sequence,
+  // key head) is short, one workgroup each and no join.
+  const int64_t len = std::min<int64_t>(attn->max_len, (int64_t)a.P * cache.page);
+  const int64_t per = (len + p.tile - 1) / p.tile + (T + p.tile - 1) / p.tile;
+  int64_t n = 0;
+  if (per > 2 * p.least) {
+    n = std::min<int64_t>((int64_t)h->num_cu * p.per_cu / p.nqb, (per * B * a.Hkv + p.least - 1) / p.least);
+    const int64_t part = (int64_t)2 * p.QB * (D + 2) * p.nqb;  // floats
+    n = std::min(n, (int64_t)h->ws_words * 2 / part);
+    if (p.nqb > 1 && n >= 8) n = n / 8 * 8;  // (row groups of a worker on one XCD)
+  }
+  a.nwg = (int)n;
+  a.part_o = (float*)h->ws;
+  a.part_ml = a.part_o + n * p.nqb * 2 * p.QB * D;
+  hipError_t e = tgs::launch_attn(a, p, cache.dtype, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(h, e, "attention kernel launch");
+  return TGS_OK;
+}
+
+int fork(tgs_ctx* h, const tgs_kv_cache& cache, uint8_t* scales, int64_t s_layer, int64_t s_page, const tgs_kv_seqs* seqs,
+         const int32_t* d_parents, int room, int32_t* d_tables_out, int32_t* d_lens_out, tgs_stream stream) {
+  if (int rc = check_seqs(h, &cache, seqs)) return rc;
+  if (room < 0) return fail(h, TGS_EINVAL, "fork: room");
+  const int R = seqs->B, P = seqs->width;
+  if (R == 0) return TGS_OK;
+  if (!d_parents || !d_tables_out || !d_lens_out) return fail(h, TGS_EINVAL, "null buffer");
+  if (d_tables_out == seqs->tables || d_lens_out == seqs->lens)
+    return fail(h, TGS_EINVAL, "fork: outputs must not be inputs");
+  if ((int64_t)R * P >= INT32_MAX || cache.layers > 32767) return fail(h, TGS_ETOOBIG, "fork: rows");
+  // workspace: copies, and for pools beyond the planning kernel's LDS owners and free pages
+  const size_t pages = tgs::kv_fork_lds(cache.n_pages, R) ? 0 : (size_t)cache.n_pages;
+  if ((size_t)R * 2 + pages > h->ws_words)
+    return fail(h, TGS_ETOOBIG, "fork: pages beyond the handle's workspace");
+  DeviceGuard g(h->device);
+  if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
+  if (int rc = raise_lds(h)) return rc;
+  tgs::KvForkArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.c = cache;
+  a.scales = scales;
+  a.s_layer = s_layer;
+  a.s_page = s_page;
+  a.tables = seqs->tables;
+  a.lens = seqs->lens;
+  a.parents = d_parents;
+  a.tables_out = d_tables_out;
+  a.lens_out = d_lens_out;
+  a.R = R;
+  a.P = P;
+  a.room = room;
+  a.page_shift = shift_of(cache.page);
+  a.copies = (int4*)h->ws;
+  a.owner = (int*)(a.copies + R);
+  a.fresh = a.owner + pages;
+  hipError_t e = tgs::launch_kv_fork(a, h->num_cu, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(h, e, "fork kernel launch");
   return TGS_OK;
 }
 
@@ -146,90 +327,55 @@ int tgs_tree_attention(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_row
                        const tgs_attn* attn, tgs_stream stream) {
   if (!h) return TGS_EINVAL;
   if (int rc = check_cache(h, cache)) return rc;
-  if (int rc = check_seqs(h, cache, seqs)) return rc;
-  if (!attn || !rows) return fail(h, TGS_EINVAL, "null argument");
-  const int D = cache->head_dim, T = attn->T, B = seqs->B;
-  if (cache->layers != 1) return fail(h, TGS_EINVAL, "attention: one layer of the cache");
-  if (D != 64 && D != 96 && D != 128 && D != 256) return fail(h, TGS_EINVAL, "attention: head_dim 64, 96, 128 or 256");
-  if (T < 1 || T > tgs::KV_MAX_NODES) return fail(h, TGS_EINVAL, "attention: 1 to 64 nodes");
-  if (attn->q_heads < 1 || attn->q_heads % cache->kv_heads)
-    return fail(h, TGS_EINVAL, "attention: query heads a multiple of key heads");
-  if (!(attn->scale > 0.0f) || !(attn->scale < 1e30f) || attn->max_len < 0)
-    return fail(h, TGS_EINVAL, "attention: scale and max_len");
-  if (B == 0) return TGS_OK;
-  if (!attn->q || !attn->out || !rows->k || !rows->v) return fail(h, TGS_EINVAL, "null buffer");
-  if (!aligned16(attn->out)) return fail(h, TGS_EINVAL, "attention: out must be 16-byte aligned");
-  if ((int64_t)B * cache->kv_heads * T * (attn->q_heads / cache->kv_heads) > INT32_MAX)
-    return fail(h, TGS_ETOOBIG, "attention: rows");
-  DeviceGuard g(h->device);
-  if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
-  if (int rc = raise_lds(h)) return rc;
-  tgs::AttnArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.q = attn->q;
-  a.k_new = rows->k;
-  a.v_new = rows->v;
-  a.q_b = attn->q_seq, a.q_t = attn->q_tok, a.q_h = attn->q_head;
-  a.kn_b = rows->k_seq, a.kn_t = rows->k_tok, a.kn_h = rows->k_head;
-  a.vn_b = rows->v_seq, a.vn_t = rows->v_tok, a.vn_h = rows->v_head;
-  a.k = cache->k;
-  a.v = cache->v;
-  a.k_page = cache->k_page;
-  a.v_page = cache->v_page;
-  a.tables = seqs->tables;
-  a.lens = seqs->lens;
-  a.parents = attn->parents;
-  a.out = attn->out;
-  a.lse = attn->lse;
-  a.B = B;
-  a.T = T;
-  a.Hq = attn->q_heads;
-  a.Hkv = cache->kv_heads;
-  a.G = a.Hq / a.Hkv;
-  a.D = D;
-  a.P = seqs->width;
-  a.n_pages = cache->n_pages;
-  a.page_shift = shift_of(cache->page);
-  a.scale_log2 = attn->scale * 1.4426950408889634f;
-  a.M = T * a.G;
-  const tgs::AttnPlan p = tgs::attn_plan(a.M, D);
-  a.QB = p.QB;
-  a.nqb = p.nqb;
-  // Workers: as many as the chip holds at once, of at least p.least tiles, as
-  // far as the workspace has room for their parts.  Where every (sequence,
-  // key head) is short, one workgroup each and no join.
-  const int64_t len = std::min<int64_t>(attn->max_len, (int64_t)a.P * cache->page);
-  const int64_t per = (len + p.tile - 1) / p.tile + (T + p.tile - 1) / p.tile;
-  int64_t n = 0;
-  if (per > 2 * p.least) {
-    n = std::min<int64_t>((int64_t)h->num_cu * p.per_cu / p.nqb, (per * B * a.Hkv + p.least - 1) / p.least);
-    const int64_t part = (int64_t)2 * p.QB * (D + 2) * p.nqb;  // floats
-    n = std::min(n, (int64_t)h->ws_words * 2 / part);
-    if (p.nqb > 1 && n >= 8) n = n / 8 * 8;  // (row groups of a worker on one XCD)
-  }
-  a.nwg = (int)n;
-  a.part_o = (float*)h->ws;
-  a.part_ml = a.part_o + n * p.nqb * 2 * p.QB * D;
-  hipError_t e = tgs::launch_attn(a, p, cache->dtype, (hipStream_t)stream);
-  if (e != hipSuccess) return hip_fail(h, e, "attention kernel launch");
-  return TGS_OK;
+  return attention(h, *cache, nullptr, 0, rows, seqs, attn, stream);
+}
+
+int tgs_kv8_attention(tgs_handle h, const tgs_kv8_cache* cache, tgs_dtype dt, const tgs_kv_rows* rows,
+                      const tgs_kv_seqs* seqs, const tgs_attn* attn, tgs_stream stream) {
+  if (!h) return TGS_EINVAL;
+  tgs_kv_cache c;
+  if (int rc = check_cache8(h, cache, dt, c)) return rc;
+  return attention(h, c, (const uint8_t*)cache->scales, cache->s_page, rows, seqs, attn, stream);
 }
 
 int tgs_kv_append(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs, int T,
                   const int32_t* d_counts, int32_t* d_lens_out, tgs_stream stream) {
   if (!h) return TGS_EINVAL;
   tgs::KvWriteArgs a;
+  if (int rc = check_cache(h, cache)) return rc;
   if (int rc = write_args(h, cache, rows, seqs, T, d_lens_out, a)) return rc;
   if (a.B == 0) return TGS_OK;
-  a.counts = d_counts;
-  // blocks that T rows, or as many as a table holds, lie in at most
-  a.nblk = T == 1 ? 1 : (int)((std::min<int64_t>(T, (int64_t)a.P * cache->page) + 7) / 8 + 1);
-  if ((int64_t)a.nblk * a.B * cache->layers > INT32_MAX) return fail(h, TGS_ETOOBIG, "rows");
-  DeviceGuard g(h->device);
-  if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
-  hipError_t e = tgs::launch_kv_append(a, (hipStream_t)stream);
-  if (e != hipSuccess) return hip_fail(h, e, "append kernel launch");
-  return TGS_OK;
+  return append(h, a, d_counts, 8, [&](const tgs::KvWriteArgs& x) { return tgs::launch_kv_append(x, (hipStream_t)stream); });
+}
+
+int tgs_kv_append_rotated(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs,
+                          int T, const int32_t* d_counts, const tgs_rotary* rotary, int32_t* d_lens_out,
+                          tgs_stream stream) {
+  if (!h) return TGS_EINVAL;
+  tgs::KvWriteArgs a;
+  if (int rc = check_cache(h, cache)) return rc;
+  if (int rc = check_rotary(h, rotary, cache->head_dim)) return rc;
+  if (int rc = write_args(h, cache, rows, seqs, T, d_lens_out, a)) return rc;
+  if (a.B == 0) return TGS_OK;
+  a.rot = *rotary;
+  return append(h, a, d_counts, 8,
+                [&](const tgs::KvWriteArgs& x) { return tgs::launch_kv_append_rotated(x, (hipStream_t)stream); });
+}
+
+int tgs_kv8_append(tgs_handle h, const tgs_kv8_cache* cache, tgs_dtype dt, const tgs_kv_rows* rows,
+                   const tgs_kv_seqs* seqs, int T, const int32_t* d_counts, const tgs_rotary* rotary,
+                   int32_t* d_lens_out, tgs_stream stream) {
+  if (!h) return TGS_EINVAL;
+  tgs_kv_cache c;
+  tgs::KvWriteArgs a;
+  if (int rc = check_cache8(h, cache, dt, c)) return rc;
+  if (rotary)
+    if (int rc = check_rotary(h, rotary, c.head_dim)) return rc;
+  if (int rc = write_args(h, &c, rows, seqs, T, d_lens_out, a)) return rc;
+  if (a.B == 0) return TGS_OK;
+  set_scales(a, cache);
+  if (rotary) a.rot = *rotary;
+  return append(h, a, d_counts, 16, [&](const tgs::KvWriteArgs& x) { return tgs::launch_kv8_append(x, (hipStream_t)stream); });
 }
 
 int tgs_tree_commit(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs, int T,
@@ -238,61 +384,86 @@ int tgs_tree_commit(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* 
   if (!h) return TGS_EINVAL;
   if (T > tgs::KV_MAX_NODES) return fail(h, TGS_EINVAL, "commit: at most 64 nodes");
   tgs::KvWriteArgs a;
+  if (int rc = check_cache(h, cache)) return rc;
   if (int rc = write_args(h, cache, rows, seqs, T, d_lens_out, a)) return rc;
   if (a.B == 0) return TGS_OK;
-  if (!d_parents || !d_draft || !d_sampled || !d_n_acc || !d_tokens || !d_path)
-    return fail(h, TGS_EINVAL, "null buffer");
-  a.parents = d_parents;
-  a.draft = d_draft;
-  a.sampled = d_sampled;
-  a.n_acc = d_n_acc;
-  a.tokens = d_tokens;
-  a.path = d_path;
-  a.nblk = T < 3 ? 1 : 2;  // (a path is seldom longer than two blocks)
-  if ((int64_t)a.nblk * a.B * cache->layers > INT32_MAX) return fail(h, TGS_ETOOBIG, "rows");
-  DeviceGuard g(h->device);
-  if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
-  hipError_t e = tgs::launch_tree_commit(a, (hipStream_t)stream);
-  if (e != hipSuccess) return hip_fail(h, e, "commit kernel launch");
-  return TGS_OK;
+  return commit(h, a, d_parents, d_draft, d_sampled, d_n_acc, d_tokens, d_path,
+                [&](const tgs::KvWriteArgs& x) { return tgs::launch_tree_commit(x, (hipStream_t)stream); });
+}
+
+int tgs_kv8_commit(tgs_handle h, const tgs_kv8_cache* cache, tgs_dtype dt, const tgs_kv_rows* rows,
+                   const tgs_kv_seqs* seqs, int T, const int32_t* d_parents, const int32_t* d_draft,
+                   const int32_t* d_sampled, int32_t* d_n_acc, int32_t* d_tokens, int32_t* d_path, int32_t* d_lens_out,
+                   tgs_stream stream) {
+  if (!h) return TGS_EINVAL;
+  if (T > tgs::KV_MAX_NODES) return fail(h, TGS_EINVAL, "commit: at most 64 nodes");
+  tgs_kv_cache c;
+  tgs::KvWriteArgs a;
+  if (int rc = check_cache8(h, cache, dt, c)) return rc;
+  if (int rc = write_args(h, &c, rows, seqs, T, d_lens_out, a)) return rc;
+  if (a.B == 0) return TGS_OK;
+  set_scales(a, cache);
+  return commit(h, a, d_parents, d_draft, d_sampled, d_n_acc, d_tokens, d_path,
+                [&](const tgs::KvWriteArgs& x) { return tgs::launch_kv8_commit(x, (hipStream_t)stream); });
 }
 
 int tgs_kv_fork(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_seqs* seqs, const int32_t* d_parents, int room,
                 int32_t* d_tables_out, int32_t* d_lens_out, tgs_stream stream) {
   if (!h) return TGS_EINVAL;
   if (int rc = check_cache(h, cache)) return rc;
-  if (int rc = check_seqs(h, cache, seqs)) return rc;
-  if (room < 0) return fail(h, TGS_EINVAL, "fork: room");
-  const int R = seqs->B, P = seqs->width;
-  if (R == 0) return TGS_OK;
-  if (!d_parents || !d_tables_out || !d_lens_out) return fail(h, TGS_EINVAL, "null buffer");
-  if (d_tables_out == seqs->tables || d_lens_out == seqs->lens)
-    return fail(h, TGS_EINVAL, "fork: outputs must not be inputs");
-  if ((int64_t)R * P >= INT32_MAX || cache->layers > 32767) return fail(h, TGS_ETOOBIG, "fork: rows");
-  // workspace: copies, and for pools beyond the planning kernel's LDS owners and free pages
-  const size_t pages = tgs::kv_fork_lds(cache->n_pages, R) ? 0 : (size_t)cache->n_pages;
-  if ((size_t)R * 2 + pages > h->ws_words)
-    return fail(h, TGS_ETOOBIG, "fork: pages beyond the handle's workspace");
+  return fork(h, *cache, nullptr, 0, 0, seqs, d_parents, room, d_tables_out, d_lens_out, stream);
+}
+
+int tgs_kv8_fork(tgs_handle h, const tgs_kv8_cache* cache, const tgs_kv_seqs* seqs, const int32_t* d_parents, int room,
+                 int32_t* d_tables_out, int32_t* d_lens_out, tgs_stream stream) {
+  if (!h) return TGS_EINVAL;
+  tgs_kv_cache c;
+  if (int rc = check_cache8(h, cache, TGS_BF16, c)) return rc;  // (a fork rounds nothing)
+  return fork(h, c, (uint8_t*)cache->scales, cache->s_layer, cache->s_page, seqs, d_parents, room, d_tables_out, d_lens_out,
+              stream);
+}
+
+int tgs_rotate(tgs_handle h, tgs_dtype dt, const tgs_rotate_rows* q, const tgs_rotate_rows* k, int B, int T, int head_dim,
+               const int32_t* d_lens, const int32_t* d_parents, const tgs_rotary* rotary, tgs_stream stream) {
+  if (!h) return TGS_EINVAL;
+  if (dt != TGS_BF16 && dt != TGS_F16) return fail(h, TGS_EINVAL, "rotation: dtype (bf16 or fp16)");
+  if (B < 0 || T < 1 || head_dim < 16 || head_dim % 8) return fail(h, TGS_EINVAL, "rotation: shape");
+  if (int rc = check_rotary(h, rotary, head_dim)) return rc;
+  if (d_parents && T > tgs::KV_MAX_NODES) return fail(h, TGS_EINVAL, "rotation: trees of at most 64 nodes");
+  if (!q) return fail(h, TGS_EINVAL, "rotation: null argument");
+  tgs::RotateArgs a;
+  std::memset(&a, 0, sizeof(a));
+  for (const tgs_rotate_rows* r : {q, k}) {
+    if (!r) continue;
+    if (r->heads < 1) return fail(h, TGS_EINVAL, "rotation: heads");
+    if (B == 0) continue;
+    if (!r->x || !r->out) return fail(h, TGS_EINVAL, "null buffer");
+    if (r->x == r->out && ((B > 1 && (r->x_seq != r->out_seq || r->out_seq == 0)) || (T > 1 && (r->x_tok != r->out_tok || r->out_tok == 0)) ||
+                           (r->heads > 1 && (r->x_head != r->out_head || r->out_head == 0))))
+      return fail(h, TGS_EINVAL, "rotation: in place only with the same strides, none of them 0");
+  }
+  const int units = (head_dim + 15) / 16;
+  const int64_t heads = (int64_t)q->heads + (k ? k->heads : 0);
+  if (heads * units > 65535) return fail(h, TGS_ETOOBIG, "rotation: heads of a token");
+  if ((int64_t)B * T > INT32_MAX) return fail(h, TGS_ETOOBIG, "rotation: tokens");
+  if (B == 0) return TGS_OK;
+  if (!d_lens) return fail(h, TGS_EINVAL, "null buffer");
+  a.q = *q;
+  if (k) a.k = *k;
+  a.lens = d_lens;
+  a.parents = d_parents;
+  a.rot = *rotary;
+  a.B = B;
+  a.T = T;
+  a.D = head_dim;
+  a.dtype = dt;
+  a.tokens = (int64_t)B * T >= 4 * h->num_cu && heads * units * tgs::ROTATE_TOKENS <= 65535 ? tgs::ROTATE_TOKENS : 1;
+  a.units = tgs::fast_div(units);
+  a.heads = tgs::fast_div((unsigned)heads);
   DeviceGuard g(h->device);
   if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
-  if (int rc = raise_lds(h)) return rc;
-  tgs::KvForkArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.c = *cache;
-  a.tables = seqs->tables;
-  a.lens = seqs->lens;
-  a.parents = d_parents;
-  a.tables_out = d_tables_out;
-  a.lens_out = d_lens_out;
-  a.R = R;
-  a.P = P;
-  a.room = room;
-  a.page_shift = shift_of(cache->page);
-  a.copies = (int4*)h->ws;
-  a.owner = (int*)(a.copies + R);
-  a.fresh = a.owner + pages;
-  hipError_t e = tgs::launch_kv_fork(a, h->num_cu, (hipStream_t)stream);
-  if (e != hipSuccess) return hip_fail(h, e, "fork kernel launch");
+  hipError_t e = tgs::launch_rotate(a, (hipStream_t)stream);
+  if (e != hipSuccess) return hip_fail(h, e, "rotation kernel launch");
   return TGS_OK;
 }
 
