@@ -12,6 +12,12 @@ struct alignas(16) int4 {
 };
 static inline uint2 make_uint2(uint32_t a, uint32_t b) { return {a, b}; }
 static inline int4 make_int4(int a, int b, int c, int d) { return {a, b, c, d}; }
+inline uint32_t atomicMax(uint32_t* p, uint32_t v) {
+  uint32_t was = __atomic_load_n(p, __ATOMIC_RELAXED);
+  while (was < v && !__atomic_compare_exchange_n(p, &was, v, false, __ATOMIC_SEQ_CST, __ATOMIC_RELAXED)) {
+  }
+  return was;
+}
 inline void __threadfence() { __atomic_thread_fence(__ATOMIC_SEQ_CST); }
 
 // ---- matrix instructions: the operands of a wave's lanes lie in one buffer

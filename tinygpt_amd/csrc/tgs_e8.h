@@ -26,6 +26,8 @@ struct F16 {};
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 #endif
 
 // The 16-bit number in the low half of u.
@@ -89,16 +91,84 @@ __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
   x[0] = x[1] = x[2] = x[3] = 0.0f;
 #endif
 }
-// Four numbers of at most 448 (or NaN) to codes, to the nearest, ties to even.
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+// Codes of four numbers over the scale s, whose magnitudes are at most 448 then (or
+// NaN), to the nearest, ties to even.
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float s) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+  const s16x2 none = {0, 0};
+  const s16x2 w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(none, a, b, s, false);
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, c, d, s, true));
 #elif defined(TGS_HOST_MFMA)
-  return hipcpu_to_e4m3(a) | (uint32_t)hipcpu_to_e4m3(b) << 8 | (uint32_t)hipcpu_to_e4m3(c) << 16 | (uint32_t)hipcpu_to_e4m3(d) << 24;
+  s = hipcpu_scale(s);
+  return hipcpu_to_e4m3(a / s) | (uint32_t)hipcpu_to_e4m3(b / s) << 8 | (uint32_t)hipcpu_to_e4m3(c / s) << 16 | (uint32_t)hipcpu_to_e4m3(d / s) << 24;
 #else
-  (void)a, (void)b, (void)c, (void)d;
+  (void)a, (void)b, (void)c, (void)d, (void)s;
   return 0;
+#endif
+}
+
+// Codes of the four 16-bit numbers of two words over the scale s; four codes whose
+// numbers are multiplied by 1 / s (a power of two; they stay where it is 1).
+template <typename DT>
+__device__ __forceinline__ uint32_t encode4(uint32_t lo, uint32_t hi, float s) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  s16x2 w = {0, 0};
+  if constexpr (__is_same(DT, BF16)) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2, lo), s, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(bf16x2, hi), s, true);
+  } else {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2, lo), s, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(f16x2, hi), s, true);
+  }
+  return __builtin_bit_cast(uint32_t, w);
+#elif defined(TGS_HOST_MFMA)
+  s = hipcpu_scale(s);
+  auto one = [&](uint32_t u, int i) { return (uint32_t)hipcpu_to_e4m3(from16<DT>(u & 0xFFFFu) / s) << i; };
+  return one(lo, 0) | one(lo >> 16, 8) | one(hi, 16) | one(hi >> 16, 24);
+#else
+  (void)lo, (void)hi, (void)s;
+  return 0;
+#endif
+}
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float s) {  // (a code is exact in bf16)
+  return encode4<BF16>(decode16<true, false>(w, 1.0f), decode16<true, true>(w, 1.0f), s);
+}
+
+#if defined(__HIP_DEVICE_COMPILE__)
+#define TGS_HALVES(op, x, y) __builtin_bit_cast(uint32_t, op(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)))
+// Of each half of two words the larger one, and the smaller one.
+__device__ __forceinline__ uint32_t max2(uint32_t x, uint32_t y) { return TGS_HALVES(__builtin_elementwise_max, x, y); }
+__device__ __forceinline__ uint32_t min2(uint32_t x, uint32_t y) { return TGS_HALVES(__builtin_elementwise_min, x, y); }
+#undef TGS_HALVES
+#else
+template <class F>
+__device__ inline uint32_t halves(uint32_t x, uint32_t y, F f) { return f(x & 0xFFFFu, y & 0xFFFFu) | f(x >> 16, y >> 16) << 16; }
+__device__ inline uint32_t max2(uint32_t x, uint32_t y) { return halves(x, y, [](uint32_t a, uint32_t b) { return a > b ? a : b; }); }
+__device__ inline uint32_t min2(uint32_t x, uint32_t y) { return halves(x, y, [](uint32_t a, uint32_t b) { return a < b ? a : b; }); }
+#endif
+// The low (high with HIGH) halves of x and y, in this order.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t halves_of(uint32_t x, uint32_t y) {
+  return HIGH ? x >> 16 | (y & 0xFFFF0000u) : (x & 0xFFFFu) | y << 16;
+}
+// Bytes 0, 1 (2, 3 with HIGH) of x between those of y: x0 y0 x1 y1.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t mixed(uint32_t x, uint32_t y) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_perm(y, x, HIGH ? 0x07030602u : 0x05010400u);
+#else
+  if (HIGH) x >>= 16, y >>= 16;
+  return (x & 0xFFu) | (y & 0xFFu) << 8 | (x >> 8 & 0xFFu) << 16 | (y >> 8 & 0xFFu) << 24;
+#endif
+}
+// Bytes 0, 2 of x and 0, 2 of y (1, 3 with ODD), in this order.
+template <bool ODD>
+__device__ __forceinline__ uint32_t every_second(uint32_t x, uint32_t y) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_perm(y, x, ODD ? 0x07050301u : 0x06040200u);
+#else
+  if (ODD) x >>= 8, y >>= 8;
+  return (x & 0xFFu) | (x >> 8 & 0xFF00u) | (y & 0xFFu) << 16 | (y << 8 & 0xFF000000u);
 #endif
 }
 
@@ -111,16 +181,29 @@ constexpr float cap() { return __is_same(DT, BF16) ? 0x1.Ep127f : 61440.0f; }
 template <typename DT>
 constexpr int floor_byte() { return __is_same(DT, BF16) ? 27 : 112; }
 
-__device__ __forceinline__ bool finite(float x) { return (tg_f2u(x) & 0x7F800000u) != 0x7F800000u; }
+// The bits of the cap in its type, and of infinity.
+template <typename DT>
+constexpr uint32_t cap_bits() { return __is_same(DT, BF16) ? 0x7F70u : 0x7B80u; }
+template <typename DT>
+constexpr uint32_t inf_bits() { return __is_same(DT, BF16) ? 0x7F80u : 0x7C00u; }
 
 // A number as a block takes it: within the cap, NaN where it is not finite.
 template <typename DT>
 __device__ __forceinline__ float taken(float x) {
   const float y = fminf(fmaxf(x, -cap<DT>()), cap<DT>());
-  return finite(x) ? y : __builtin_nanf("");
+  return (tg_f2u(x) & 0x7F800000u) == 0x7F800000u ? __builtin_nanf("") : y;
 }
-// The larger of m and a taken number's magnitude (NaN: m).
-__device__ __forceinline__ float most(float m, float x) { return fmaxf(m, fabsf(x)); }
+// The same of the two 16-bit numbers of a word; and the largest magnitudes' bits with
+// theirs (NaN counts as 0).
+template <typename DT>
+__device__ __forceinline__ uint32_t taken2(uint32_t w, uint32_t& most) {
+  const uint32_t m = w & 0x7FFF7FFFu;
+  const uint32_t over = (m + (0x8000u - inf_bits<DT>()) * 0x10001u) & 0x80008000u;  // (no carry between the halves)
+  const uint32_t odd = over - (over >> 15);
+  const uint32_t y = min2(m, cap_bits<DT>() * 0x10001u);
+  most = max2(most, y & ~odd);
+  return (w & 0x80008000u) | y | odd;
+}
 
 // Byte of the smallest scale for the largest magnitude m: 448 = 1.75 2^8, so it
 // is m's exponent - 8, one more where m's significand passes 1.75 (the addition
@@ -130,12 +213,8 @@ __device__ __forceinline__ int need_byte(float m) {
   const int e = (int)((tg_f2u(m) + 0x1FFFFFu) >> 23) - 8;
   return e > floor_byte<DT>() ? e : floor_byte<DT>();
 }
-// 2^-e of a byte.
-__device__ __forceinline__ float inverse_of(int byte) {
-  return tg_u2f(byte < 254 ? (uint32_t)(254 - byte) << 23 : byte == 254 ? 0x400000u : 0x7FC00000u);
-}
-// 2^(from - to) of bytes from <= to (below 2^-126, which leaves nothing of a code: 0).
-__device__ __forceinline__ float shrink(int from, int to) { return to - from < 127 ? tg_u2f((uint32_t)(127 + from - to) << 23) : 0.0f; }
+// 2^(to - from) of bytes from <= to (beyond 2^127, which leaves nothing of a code: that).
+__device__ __forceinline__ float growth(int from, int to) { return tg_u2f((uint32_t)(127 + (to - from < 127 ? to - from : 127)) << 23); }
 
 // ------------------------------------------------------------------ rotation
 
@@ -143,7 +222,7 @@ __device__ __forceinline__ float shrink(int from, int to) { return to - from < 1
 // bits (a position near 2^17 leaves a 32-bit product 2^-7 off), what is left of
 // it, at most pi / 4, by the Taylor polynomials of degree 9 and 10, whose first
 // left out terms are below 2^-29.
-struct Turn {
+struct alignas(8) Turn {
   float c, s;
 };
 __device__ __forceinline__ Turn turn(uint32_t position, float freq) {
@@ -183,36 +262,76 @@ __device__ __forceinline__ Unit unit_of(int u, int D, int R, bool pairs) {
 }
 __device__ __forceinline__ int units(int D) { return (D + 15) >> 4; }
 
-// Turns the unit's sixteen numbers x (two chunks of eight); cs: its eight cosines
-// and sines.
-__device__ __forceinline__ void turn_unit(float (&x)[16], const Turn* cs, bool pairs) {
-  auto two = [](float& a, float& b, Turn t) {
-    const float lo = a, hi = b;
-    a = __builtin_fmaf(lo, t.c, -(hi * t.s));
-    b = __builtin_fmaf(hi, t.c, lo * t.s);
-  };
-  if (pairs) {
+// Turns the unit's pairs (x[i], x[i + 8]); cs: its eight cosines and sines.
+__device__ __forceinline__ void turn_unit(float (&x)[16], const Turn* cs) {
+  typedef float Two __attribute__((vector_size(16)));  // two of them
 #pragma unroll
-    for (int i = 0; i < 8; i++) two(x[2 * i], x[2 * i + 1], cs[i]);
-  } else {
+  for (int i = 0; i < 8; i += 2) {
+    const Two t = *(const Two*)(cs + i);
 #pragma unroll
-    for (int i = 0; i < 8; i++) two(x[i], x[i + 8], cs[i]);
+    for (int j = 0; j < 2; j++) {
+      const float lo = x[i + j], hi = x[i + j + 8];
+      x[i + j] = __builtin_fmaf(lo, t[2 * j], -(hi * t[2 * j + 1]));
+      x[i + j + 8] = __builtin_fmaf(hi, t[2 * j], lo * t[2 * j + 1]);
+    }
   }
 }
 
-// A chunk's eight 16-bit numbers as floats, and back.
-template <typename DT>
-__device__ __forceinline__ void widen(uint4 w, float* x) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// A unit's sixteen 16-bit numbers in eight words; neighbours' pairs are taken apart
+// (numbers 2 i to place i, 2 i + 1 to place i + 8), and put together again.
+template <typename W>
+__device__ __forceinline__ void take_apart(W& w) {
+  uint32_t x[8];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    x[2 * i] = from16<DT>(u[i] & 0xFFFFu);
-    x[2 * i + 1] = from16<DT>(u[i] >> 16);
+    x[i] = halves_of<false>(w[2 * i], w[2 * i + 1]);
+    x[i + 4] = halves_of<true>(w[2 * i], w[2 * i + 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i++) w[i] = x[i];
+}
+template <typename W>
+__device__ __forceinline__ void put_together(W& w) {
+  uint32_t x[8];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    x[2 * i] = halves_of<false>(w[i], w[i + 4]);
+    x[2 * i + 1] = halves_of<true>(w[i], w[i + 4]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; i++) w[i] = x[i];
+}
+// The same of sixteen codes in four words.
+__device__ __forceinline__ void put_together(uint32_t (&c)[4]) {
+  const uint32_t x[4] = {mixed<false>(c[0], c[2]), mixed<true>(c[0], c[2]), mixed<false>(c[1], c[3]), mixed<true>(c[1], c[3])};
+#pragma unroll
+  for (int i = 0; i < 4; i++) c[i] = x[i];
+}
+
+// The words' numbers as floats, and back.
+template <typename DT>
+__device__ __forceinline__ void widen(const uint32_t (&w)[8], float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    x[2 * i] = from16<DT>(w[i] & 0xFFFFu);
+    x[2 * i + 1] = from16<DT>(w[i] >> 16);
   }
 }
 template <typename DT>
-__device__ __forceinline__ uint4 narrow(const float* x) {
-  return make_uint4(to16<DT>(x[0], x[1]), to16<DT>(x[2], x[3]), to16<DT>(x[4], x[5]), to16<DT>(x[6], x[7]));
+__device__ __forceinline__ void narrow(const float (&x)[16], uint32_t (&w)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) w[i] = to16<DT>(x[2 * i], x[2 * i + 1]);
+}
+
+// A unit of a 16-bit row, turned.
+template <typename DT>
+__device__ __forceinline__ void turn_words(uint32_t (&w)[8], const Turn* cs, bool pairs) {
+  float x[16];
+  if (pairs) take_apart(w);
+  widen<DT>(w, x);
+  turn_unit(x, cs);
+  narrow<DT>(x, w);
+  if (pairs) put_together(w);
 }
 
 }  // namespace e8

@@ -43,12 +43,13 @@ struct KvWriteArgs {
   uint8_t* scales;
   long long s_layer, s_page;
   tgs_rotary rot;  // of the keys; freq nullptr: none
+  FastDiv turns;   // rot.dims / 2
 };
 hipError_t launch_kv_append(const KvWriteArgs& a, hipStream_t st);
 hipError_t launch_tree_commit(const KvWriteArgs& a, hipStream_t st);
 hipError_t launch_kv_append_rotated(const KvWriteArgs& a, hipStream_t st);
-hipError_t launch_kv8_append(const KvWriteArgs& a, hipStream_t st);
-hipError_t launch_kv8_commit(const KvWriteArgs& a, hipStream_t st);
+hipError_t launch_kv8_append(const KvWriteArgs& a, int num_cu, hipStream_t st);
+hipError_t launch_kv8_commit(const KvWriteArgs& a, int num_cu, hipStream_t st);
 
 // Queries and keys of drafted nodes turned by their positions.
 constexpr int ROTARY_MAX = 256;  // dimensions that turn, at most
@@ -60,7 +61,7 @@ struct RotateArgs {
   tgs_rotary rot;
   int B, T, D, dtype;
   int tokens;  // of a workgroup: 1 or ROTATE_TOKENS
-  FastDiv units, heads;  // of a row; of queries and keys together
+  FastDiv units, heads, turns;  // of a row; of queries and keys together; rot.dims / 2
 };
 hipError_t launch_rotate(const RotateArgs& a, hipStream_t st);
 

@@ -19,8 +19,8 @@ namespace kv {
 // ROT: void, or the type of the keys that are turned.
 template <class ROT>
 struct WriteShared {
+  alignas(16) e8::Turn cs[8][ROTARY_MAX / 2];
   WriteHead head;
-  e8::Turn cs[8][ROTARY_MAX / 2];
 };
 template <>
 struct WriteShared<void> {
@@ -43,9 +43,13 @@ __global__ __launch_bounds__(KV_NT) void write_kernel(KvWriteArgs a) {
   WriteHead& s = sh.head;
   const int x = blockIdx.x % a.nblk, bl = blockIdx.x / a.nblk, b = bl % a.B, l = bl / a.B;
   const int tid = threadIdx.x;
-  int len, n;
-  if (!write_head<COMMIT>(a, s, b, l == 0 && x == 0, len, n)) return;
+  const int len = a.lens[b], n = rows_of<COMMIT>(a, s, b);
   const int* table = a.tables + (long long)b * a.P;
+  int bad = past_table(a, len, n);
+  if (!bad) bad = outside_pool(a, table, len, n);
+  bad = __syncthreads_or(bad);
+  if (l == 0 && x == 0) report<COMMIT>(a, s, b, len, n, bad);
+  if (bad || n == 0) return;
   const int D = a.c.head_dim, H = a.c.kv_heads, page = 1 << a.page_shift;
   const uint16_t* kn = (const uint16_t*)a.r.k + l * a.r.k_layer + b * a.r.k_seq;
   const uint16_t* vn = (const uint16_t*)a.r.v + l * a.r.v_layer + b * a.r.v_seq;
@@ -62,7 +66,7 @@ __global__ __launch_bounds__(KV_NT) void write_kernel(KvWriteArgs a) {
       const int half = a.rot.dims >> 1, U = e8::units(D);
       __syncthreads();  // (the block before is done with the table)
       for (int e = tid; e < nt * half; e += KV_NT) {
-        const int i = e / half, j = e - i * half;
+        const int i = div_by((unsigned)e, a.turns), j = e - i * half;
         sh.cs[i][j] = e8::turn((uint32_t)(t0 + i), a.rot.freq[j]);
       }
       __syncthreads();
@@ -73,17 +77,10 @@ __global__ __launch_bounds__(KV_NT) void write_kernel(KvWriteArgs a) {
         uint16_t* to = kp + ((long long)h * page + i) * D;
         const e8::Unit w = e8::unit_of((int)u, D, a.rot.dims, a.rot.pairs);
         const uint4 lo = load_row16<false>(from + w.a), hi = w.b >= 0 ? load_row16<false>(from + w.b) : lo;
-        if (w.angle < 0) {
-          *(uint4*)(to + w.a) = lo;
-          if (w.b >= 0) *(uint4*)(to + w.b) = hi;
-          continue;
-        }
-        float y[16];
-        e8::widen<ROT>(lo, y);
-        e8::widen<ROT>(hi, y + 8);
-        e8::turn_unit(y, sh.cs[i] + w.angle, a.rot.pairs);
-        *(uint4*)(to + w.a) = e8::narrow<ROT>(y);
-        *(uint4*)(to + w.b) = e8::narrow<ROT>(y + 8);
+        uint32_t y[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (w.angle >= 0) e8::turn_words<ROT>(y, sh.cs[i] + w.angle, a.rot.pairs);
+        *(uint4*)(to + w.a) = make_uint4(y[0], y[1], y[2], y[3]);
+        if (w.b >= 0) *(uint4*)(to + w.b) = make_uint4(y[4], y[5], y[6], y[7]);
       }
     } else
     for (int e = tid; e < nt * H * C; e += KV_NT) {  // 16-byte vectors of keys: (token, head, chunk)

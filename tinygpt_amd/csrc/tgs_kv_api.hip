@@ -146,6 +146,11 @@ int commit(tgs_ctx* h, tgs::KvWriteArgs& a, const int32_t* d_parents, const int3
   return TGS_OK;
 }
 
+void set_rotary(tgs::KvWriteArgs& a, const tgs_rotary* r) {
+  a.rot = *r;
+  a.turns = tgs::fast_div(r->dims / 2);
+}
+
 void set_scales(tgs::KvWriteArgs& a, const tgs_kv8_cache* c) {
   a.scales = (uint8_t*)c->scales;
   a.s_layer = c->s_layer;
@@ -357,7 +362,7 @@ int tgs_kv_append_rotated(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_
   if (int rc = check_rotary(h, rotary, cache->head_dim)) return rc;
   if (int rc = write_args(h, cache, rows, seqs, T, d_lens_out, a)) return rc;
   if (a.B == 0) return TGS_OK;
-  a.rot = *rotary;
+  set_rotary(a, rotary);
   return append(h, a, d_counts, 8,
                 [&](const tgs::KvWriteArgs& x) { return tgs::launch_kv_append_rotated(x, (hipStream_t)stream); });
 }
@@ -374,8 +379,8 @@ int tgs_kv8_append(tgs_handle h, const tgs_kv8_cache* cache, tgs_dtype dt, const
   if (int rc = write_args(h, &c, rows, seqs, T, d_lens_out, a)) return rc;
   if (a.B == 0) return TGS_OK;
   set_scales(a, cache);
-  if (rotary) a.rot = *rotary;
-  return append(h, a, d_counts, 16, [&](const tgs::KvWriteArgs& x) { return tgs::launch_kv8_append(x, (hipStream_t)stream); });
+  if (rotary) set_rotary(a, rotary);
+  return append(h, a, d_counts, 16, [&](const tgs::KvWriteArgs& x) { return tgs::launch_kv8_append(x, h->num_cu, (hipStream_t)stream); });
 }
 
 int tgs_tree_commit(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_rows* rows, const tgs_kv_seqs* seqs, int T,
@@ -404,7 +409,7 @@ int tgs_kv8_commit(tgs_handle h, const tgs_kv8_cache* cache, tgs_dtype dt, const
   if (a.B == 0) return TGS_OK;
   set_scales(a, cache);
   return commit(h, a, d_parents, d_draft, d_sampled, d_n_acc, d_tokens, d_path,
-                [&](const tgs::KvWriteArgs& x) { return tgs::launch_kv8_commit(x, (hipStream_t)stream); });
+                [&](const tgs::KvWriteArgs& x) { return tgs::launch_kv8_commit(x, h->num_cu, (hipStream_t)stream); });
 }
 
 int tgs_kv_fork(tgs_handle h, const tgs_kv_cache* cache, const tgs_kv_seqs* seqs, const int32_t* d_parents, int room,
@@ -460,6 +465,7 @@ int tgs_rotate(tgs_handle h, tgs_dtype dt, const tgs_rotate_rows* q, const tgs_r
   a.tokens = (int64_t)B * T >= 4 * h->num_cu && heads * units * tgs::ROTATE_TOKENS <= 65535 ? tgs::ROTATE_TOKENS : 1;
   a.units = tgs::fast_div(units);
   a.heads = tgs::fast_div((unsigned)heads);
+  a.turns = tgs::fast_div(rotary->dims / 2);
   DeviceGuard g(h->device);
   if (!g.ok) return fail(h, TGS_EHIP, "hipSetDevice");
   hipError_t e = tgs::launch_rotate(a, (hipStream_t)stream);

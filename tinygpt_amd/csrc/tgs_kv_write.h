@@ -34,49 +34,49 @@ __device__ __forceinline__ int accept_walk(const int* parents, const int* draft,
   }
 }
 
-// The n rows of sequence b that follow its len tokens (COMMIT: s.path, found here),
-// by the whole workgroup; `first`: this workgroup reports.  False: nothing is written.
+// How many rows follow sequence b's len tokens (COMMIT: those of s.path, found here by
+// the whole workgroup).
 template <bool COMMIT>
-__device__ __forceinline__ bool write_head(const KvWriteArgs& a, WriteHead& s, int b, bool first, int& len_out, int& n_out) {
-  const int tid = threadIdx.x;
-  const int len = a.lens[b];
-  int n;
-  if constexpr (COMMIT) {
-    if (tid < 64) {
-      const int cnt = accept_walk(a.parents + (long long)b * a.T, a.draft + (long long)b * a.T,
-                                  a.sampled + (long long)b * a.T, a.T, s.path);
-      if (tid == 0) s.n = cnt;
-    }
-    __syncthreads();
-    n = s.n;
-  } else {
-    n = a.counts ? a.counts[b] : a.T;
+__device__ __forceinline__ int rows_of(const KvWriteArgs& a, WriteHead& s, int b) {
+  if constexpr (!COMMIT) return a.counts ? a.counts[b] : a.T;
+  const long long o = (long long)b * a.T;
+  if (threadIdx.x < 64) {
+    const int cnt = accept_walk(a.parents + o, a.draft + o, a.sampled + o, a.T, s.path);
+    if (threadIdx.x == 0) s.n = cnt;
   }
-  // what does not fit is not written: a count outside [0, T], positions past
-  // the table, pages outside the pool
-  int bad = n < 0 || n > a.T || len < 0 || (long long)len + n > ((long long)a.P << a.page_shift);
-  const int* table = a.tables + (long long)b * a.P;
-  if (!bad && n > 0)
-    for (int i = (len >> a.page_shift) + tid; i <= (len + n - 1) >> a.page_shift; i += (int)blockDim.x)
+  __syncthreads();
+  return s.n;
+}
+
+// What does not fit is not written: a count outside [0, T], positions past the
+// table, pages outside the pool (a thread looks at its share of them).
+__device__ __forceinline__ bool past_table(const KvWriteArgs& a, int len, int n) {
+  return n < 0 || n > a.T || len < 0 || (long long)len + n > ((long long)a.P << a.page_shift);
+}
+__device__ __forceinline__ bool outside_pool(const KvWriteArgs& a, const int* table, int len, int n) {
+  int bad = 0;
+  if (n > 0)
+    for (int i = (len >> a.page_shift) + (int)threadIdx.x; i <= (len + n - 1) >> a.page_shift; i += (int)blockDim.x)
       bad |= (unsigned)table[i] >= (unsigned)a.c.n_pages;
-  bad = __syncthreads_or(bad);
-  if (first) {
-    if (tid == 0) {
-      a.lens_out[b] = bad ? -1 : len + n;
-      if (COMMIT) a.n_acc[b] = n - 1;
-    }
-    if (COMMIT && tid < a.T) {
-      const long long o = (long long)b * a.T;
-      a.path[o + tid] = tid < n ? s.path[tid] : -1;
-      int t = -1;  // the accepted nodes' tokens, then the one sampled at the last
-      if (tid < n - 1) t = a.draft[o + s.path[tid + 1]];
-      if (tid == n - 1) t = a.sampled[o + s.path[tid]];
-      a.tokens[o + tid] = t;
-    }
+  return bad;
+}
+
+// The outputs but the cache, by one workgroup.
+template <bool COMMIT>
+__device__ __forceinline__ void report(const KvWriteArgs& a, const WriteHead& s, int b, int len, int n, bool bad) {
+  const int tid = threadIdx.x;
+  if (tid == 0) {
+    a.lens_out[b] = bad ? -1 : len + n;
+    if (COMMIT) a.n_acc[b] = n - 1;
   }
-  len_out = len;
-  n_out = n;
-  return !bad && n > 0;
+  if (COMMIT && tid < a.T) {
+    const long long o = (long long)b * a.T;
+    a.path[o + tid] = tid < n ? s.path[tid] : -1;
+    int t = -1;  // the accepted nodes' tokens, then the one sampled at the last
+    if (tid < n - 1) t = a.draft[o + s.path[tid + 1]];
+    if (tid == n - 1) t = a.sampled[o + s.path[tid]];
+    a.tokens[o + tid] = t;
+  }
 }
 
 }  // namespace kv

@@ -13,7 +13,7 @@ using kv::div_by;
 constexpr int NT = 256;  // (a wave a token finds its depth: ROTATE_TOKENS of them at most)
 
 struct Shared {
-  e8::Turn cs[ROTATE_TOKENS][ROTARY_MAX / 2];
+  alignas(16) e8::Turn cs[ROTATE_TOKENS][ROTARY_MAX / 2];
   uint32_t position[ROTATE_TOKENS];
 };
 
@@ -51,7 +51,7 @@ __global__ __launch_bounds__(NT) void rotate_kernel(RotateArgs a) {
   __syncthreads();
   const int half = a.rot.dims >> 1;
   for (int e = tid; e < n * half; e += NT) {
-    const int i = e / half, j = e - i * half;
+    const int i = div_by((unsigned)e, a.turns), j = e - i * half;
     s.cs[i][j] = e8::turn(s.position[i], a.rot.freq[j]);
   }
   __syncthreads();
@@ -70,17 +70,10 @@ __global__ __launch_bounds__(NT) void rotate_kernel(RotateArgs a) {
     const e8::Unit w = e8::unit_of((int)u, a.D, a.rot.dims, a.rot.pairs);
     if (w.angle < 0 && from == to) continue;
     const uint4 lo = load_row16<false>(from + w.a), hi = w.b >= 0 ? load_row16<false>(from + w.b) : lo;
-    if (w.angle < 0) {
-      store_row16(to + w.a, lo);
-      if (w.b >= 0) store_row16(to + w.b, hi);
-      continue;
-    }
-    float x[16];
-    e8::widen<DT>(lo, x);
-    e8::widen<DT>(hi, x + 8);
-    e8::turn_unit(x, s.cs[i] + w.angle, a.rot.pairs);
-    store_row16(to + w.a, e8::narrow<DT>(x));
-    store_row16(to + w.b, e8::narrow<DT>(x + 8));
+    uint32_t x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (w.angle >= 0) e8::turn_words<DT>(x, s.cs[i] + w.angle, a.rot.pairs);
+    store_row16(to + w.a, make_uint4(x[0], x[1], x[2], x[3]));
+    if (w.b >= 0) store_row16(to + w.b, make_uint4(x[4], x[5], x[6], x[7]));
   }
 }
 
