@@ -92,7 +92,7 @@ struct Part {
   const KvWriteArgs& a;
   const Block k;
   uint32_t w[NU][8];
-  uint4 was[WHOLE ? 1 : (NU + 1) / 2][2];  // of values: what a block that is filled in holds
+  uint2 was[WHOLE ? 1 : NU][2];  // of values: what a unit's two dimensions hold
   int D, U;
 
   __device__ __forceinline__ Part(const KvWriteArgs& args, const Block& b) : a(args), k(b), D(args.c.head_dim), U(args.c.head_dim >> 4) {}
@@ -140,11 +140,15 @@ struct Part {
     const ValueUnit x = value_unit(0);
     const uint16_t* p = from + (base + near(x.first)) * tok;
 #pragma unroll
-    for (int i = 0; i < 8 * H; i++) {
+    for (int h = 0; h < H; h++) {
+      if (!any_new(h)) continue;
 #pragma unroll
-      for (int n = 0; n < NU; n += H) __builtin_memcpy(&w[n + (i >> 3)][i & 7], p + value_unit(n).d, 4);
-      const int t = x.first + i;
-      p += WHOLE || (t >= k.lo && t < k.hi - 1) ? tok : 0;
+      for (int i = 0; i < 8; i++) {
+#pragma unroll
+        for (int n = 0; n < NU; n += H) __builtin_memcpy(&w[n + h][i], p + value_unit(n).d, 4);
+        const int t = x.first + 8 * h + i;
+        p += WHOLE || (t >= k.lo && t < k.hi - 1) ? tok : 0;
+      }
     }
   }
   // The same where path gives the rows' numbers.
@@ -156,30 +160,31 @@ struct Part {
     } else {
       const int mine = path[base + near(lane_id() & 15)];
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const uint16_t* p = from + (int)readlane_u32((uint32_t)mine, i) * tok;
+      for (int h = 0; h < 2; h++) {
+        if (!any_new(h)) continue;
 #pragma unroll
-        for (int n = 0; n < NU; n += 2) __builtin_memcpy(&w[n + (i >> 3)][i & 7], p + value_unit(n).d, 4);
+        for (int i = 0; i < 8; i++) {
+          const uint16_t* p = from + (int)readlane_u32((uint32_t)mine, 8 * h + i) * tok;
+#pragma unroll
+          for (int n = 0; n < NU; n += 2) __builtin_memcpy(&w[n + h][i], p + value_unit(n).d, 4);
+        }
       }
     }
   }
-  // What a lane's dimensions of a block of values hold.
+  // Whether unit n of the values has new tokens: of a block that is filled in, often
+  // only one half does (a lane has units of both where it has one alone).
+  __device__ __forceinline__ bool any_new(int n) const { return WHOLE || NU == 1 || (k.lo < (n & 1) * 8 + 8 && k.hi > (n & 1) * 8); }
+  __device__ __forceinline__ bool any_held(int n) const { return NU == 1 || k.lo > (n & 1) * 8; }
+  __device__ __forceinline__ void load_held(const uint8_t* from, int n) {
+    const ValueUnit x = value_unit(n);
+#pragma unroll
+    for (int d = 0; d < 2; d++) was[n][d] = *(const uint2*)(from + (x.d + d) * e8::BLOCK + x.first);
+  }
   __device__ __forceinline__ void load_held(const uint8_t* from) {
     if constexpr (!WHOLE) {
 #pragma unroll
-      for (int n = 0; n < NU; n += H) {
-        const ValueUnit x = value_unit(n);
-#pragma unroll
-        for (int d = 0; d < 2; d++) {
-          const uint8_t* p = from + (x.d + d) * e8::BLOCK + x.first;
-          if constexpr (H == 1) {
-            const uint2 y = *(const uint2*)p;
-            was[0][d] = make_uint4(y.x, y.y, 0, 0);
-          } else {
-            was[n / 2][d] = *(const uint4*)p;
-          }
-        }
-      }
+      for (int n = 0; n < NU; n++)
+        if (any_new(n)) load_held(from, n);
     }
   }
 
@@ -196,13 +201,14 @@ struct Part {
   }
 
   static __device__ __forceinline__ uint32_t both(uint32_t m) { return wave_max(m >> 16 > (m & 0xFFFFu) ? m >> 16 : m & 0xFFFFu); }
-  // The largest magnitude of all lanes (of the first `count` units); where it passes the
+  // The largest magnitude of all lanes, of the units that count; where it passes the
   // cap, the numbers are capped, and NaN where they are not finite.
-  __device__ __forceinline__ float largest(int count) {
+  template <class F>
+  __device__ __forceinline__ float largest(F counts) {
     uint32_t m = 0;
 #pragma unroll
     for (int n = 0; n < NU; n++) {
-      if (!WHOLE && n >= count) break;
+      if (!counts(n)) continue;
 #pragma unroll
       for (int i = 0; i < 8; i++) m = e8::max2(m, w[n][i] & 0x7FFF7FFFu);
     }
@@ -211,7 +217,7 @@ struct Part {
       m = 0;
 #pragma unroll
       for (int n = 0; n < NU; n++) {
-        if (!WHOLE && n >= count) break;
+        if (!counts(n)) continue;
 #pragma unroll
         for (int i = 0; i < 8; i++) w[n][i] = e8::taken2<DT>(w[n][i], m);
       }
@@ -240,10 +246,7 @@ struct Part {
   static __device__ __forceinline__ uint32_t code(uint32_t c, int byte) { return !WHOLE && byte == 255 ? 0x7F7F7F7Fu : c; }
 
   __device__ __forceinline__ void put_keys(uint8_t* to, int old, uint8_t* scale) {
-    int count = 0;
-#pragma unroll
-    for (int n = 0; n < NU; n++) count += live(n);
-    const Scale s = rescale<DT>(k, largest(count), old, scale);
+    const Scale s = rescale<DT>(k, largest([&](int n) { return live(n); }), old, scale);
 #pragma unroll
     for (int n = 0; n < NU; n++) {
       if (!live(n)) break;
@@ -304,36 +307,54 @@ struct Part {
     put();
   }
 
+  // The codes of unit n's two dimensions, eight tokens each.
+  __device__ __forceinline__ void codes(int n, const Scale& s, uint2 (&c)[2]) const {
+    uint32_t p[4];  // two tokens' two codes
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = code(e8::encode4<DT>(w[n][2 * i], w[n][2 * i + 1], s.of), s.byte);
+    c[0] = make_uint2(e8::every_second<false>(p[0], p[1]), e8::every_second<false>(p[2], p[3]));
+    c[1] = make_uint2(e8::every_second<true>(p[0], p[1]), e8::every_second<true>(p[2], p[3]));
+  }
+
   __device__ __forceinline__ void put_values(uint8_t* to, int old, uint8_t* scale) {
     select_values();
-    const Scale s = rescale<DT>(k, largest(NU), old, scale);
+    const Scale s = rescale<DT>(k, largest([&](int n) { return any_new(n); }), old, scale);
+    if constexpr (WHOLE) {
 #pragma unroll
-    for (int n = 0; n < NU; n += H) {
-      uint2 c[H][2];  // of each half, the two dimensions' eight codes
+      for (int n = 0; n < NU; n += H) {
+        uint2 c[H][2];
 #pragma unroll
-      for (int h = 0; h < H; h++) {
-        uint32_t p[4];  // two tokens' two codes
+        for (int h = 0; h < H; h++) codes(n + h, s, c[h]);
+        const ValueUnit x = value_unit(n);
+        if (!x.in) continue;
+        uint8_t* p = to + x.d * e8::BLOCK + x.first;
 #pragma unroll
-        for (int i = 0; i < 4; i++) p[i] = code(e8::encode4<DT>(w[n + h][2 * i], w[n + h][2 * i + 1], s.of), s.byte);
-        c[h][0] = make_uint2(e8::every_second<false>(p[0], p[1]), e8::every_second<false>(p[2], p[3]));
-        c[h][1] = make_uint2(e8::every_second<true>(p[0], p[1]), e8::every_second<true>(p[2], p[3]));
-      }
-      const ValueUnit x = value_unit(n);
-      if constexpr (!WHOLE) {
-#pragma unroll
-        for (int d = 0; d < 2; d++) {
-          const uint4 o = was[n / 2][d];
-          c[0][d] = merged(c[0][d], make_uint2(o.x, o.y), bytes_of(k.lo - x.first, k.hi - x.first), bytes_of(0, k.lo - x.first), s.grown);
-          if constexpr (H == 2) c[1][d] = merged(c[1][d], make_uint2(o.z, o.w), bytes_of(k.lo - 8, k.hi - 8), bytes_of(0, k.lo - 8), s.grown);
+        for (int d = 0; d < 2; d++, p += e8::BLOCK) {
+          if constexpr (H == 2) *(uint4*)p = make_uint4(c[0][d].x, c[0][d].y, c[1][d].x, c[1][d].y);
+          else *(uint2*)p = c[0][d];
         }
       }
-      if (!x.in) continue;
-      uint8_t* p = to + x.d * e8::BLOCK + x.first;
+      return;
+    }
 #pragma unroll
-      for (int d = 0; d < 2; d++, p += e8::BLOCK) {
-        if constexpr (H == 2) *(uint4*)p = make_uint4(c[0][d].x, c[0][d].y, c[1][d].x, c[1][d].y);
-        else *(uint2*)p = c[0][d];
+    for (int n = 0; n < NU; n++) {
+      const ValueUnit x = value_unit(n);
+      uint8_t* p = to + x.d * e8::BLOCK + x.first;
+      uint2 c[2];
+      if (any_new(n)) {
+        codes(n, s, c);
+#pragma unroll
+        for (int d = 0; d < 2; d++) c[d] = merged(c[d], was[n][d], bytes_of(k.lo - x.first, k.hi - x.first), bytes_of(0, k.lo - x.first), s.grown);
+      } else if (s.grown != 1.0f && any_held(n)) {
+        load_held(to, n);
+#pragma unroll
+        for (int d = 0; d < 2; d++) c[d] = merged(c[d], was[n][d], 0, ~0ull, s.grown);
+      } else {
+        continue;
       }
+      if (!x.in) continue;
+#pragma unroll
+      for (int d = 0; d < 2; d++) *(uint2*)(p + d * e8::BLOCK) = c[d];
     }
   }
 };
@@ -536,9 +557,10 @@ __global__ __launch_bounds__(STEP_NT) void step_kernel(KvWriteArgs a, int round)
 
 template <typename DT, bool COMMIT, bool ROT>
 hipError_t run(const KvWriteArgs& a, int num_cu, hipStream_t st) {
-  // Layers to a workgroup: as many as leave four workgroups a CU.
+  // Layers to a workgroup: as many as leave eight workgroups a CU (half of them for
+  // blocks that are not there, as a rule).
   const long long all = 2ll * a.nblk * a.B * a.c.layers;
-  int per = (int)(all / (4ll * num_cu));
+  int per = (int)(all / (8ll * num_cu));
   per = per < 1 ? 1 : per > 8 ? 8 : per;
   per = per < a.c.layers ? per : a.c.layers;
   const int groups = (a.c.layers + per - 1) / per, tasks = a.c.kv_heads * per;
