@@ -195,13 +195,9 @@ __device__ __forceinline__ int clamp_len(const AttnArgs& a, int n) {
   const long long cap = (long long)a.P << a.page_shift;
   return n < 0 ? 0 : n > cap ? (int)cap : n;
 }
-template <class GEO>
-__device__ __forceinline__ int cache_tiles(const AttnArgs& a, int b) {
-  return (uniform(clamp_len(a, a.lens[b])) + GEO::TILE - 1) / GEO::TILE;
-}
-template <class GEO>  // (a sequence per lane)
-__device__ __forceinline__ int lane_tiles(const AttnArgs& a, int b) {
-  return (clamp_len(a, a.lens[b]) + GEO::TILE - 1) / GEO::TILE;
+template <class GEO>  // of the length `given`
+__device__ __forceinline__ int cache_tiles(const AttnArgs& a, int given) {
+  return (clamp_len(a, given) + GEO::TILE - 1) / GEO::TILE;
 }
 
 // Tiles of sequences before b (of one key head), and of all: by one wave.
@@ -210,7 +206,7 @@ __device__ __forceinline__ void tiles_before(const AttnArgs& a, int b, int& befo
   const int tree = (a.T + GEO::TILE - 1) / GEO::TILE + GEO::EXTRA;
   int x = 0, y = 0;
   for (int i = lane_id(); i < a.B; i += 64) {
-    const int n = lane_tiles<GEO>(a, i) + tree;
+    const int n = cache_tiles<GEO>(a, a.lens[i]) + tree;
     y += n;
     if (i < b) x += n;
   }
@@ -228,29 +224,31 @@ __device__ __forceinline__ long long share_start(long long U, int N, int w) {
 
 // A worker's place: its share [u0, u1), and of tile u0 the sequence, key head
 // and tile in them, with the tiles of that sequence (drafted nodes and the
-// extra ones, behind which nothing lies, included).
+// extra ones, behind which nothing lies, included) and its length as given.
 struct Place {
   long long u0, u1;
-  int b, h, at, nt;
+  int b, h, at, nt, given;
 };
 template <class GEO>
 __device__ __forceinline__ Place find_place(const AttnArgs& a, int w) {
   const int tree = (a.T + GEO::TILE - 1) / GEO::TILE + GEO::EXTRA, lane = lane_id();
-  const int mine = lane < a.B ? lane_tiles<GEO>(a, lane) + tree : 0;  // (of the first 64 sequences)
-  int y = mine;
-  for (int i = lane + 64; i < a.B; i += 64) y += lane_tiles<GEO>(a, i) + tree;
+  const int mine = lane < a.B ? a.lens[lane] : 0;  // (of the first 64 sequences)
+  int y = lane < a.B ? cache_tiles<GEO>(a, mine) + tree : 0;
+  for (int i = lane + 64; i < a.B; i += 64) y += cache_tiles<GEO>(a, a.lens[i]) + tree;
   const long long U = (long long)uniform(wave_sum(y)) * a.Hkv;
-  Place p{share_start(U, a.nwg, w), share_start(U, a.nwg, w + 1), 0, 0, 0, 0};
+  Place p{share_start(U, a.nwg, w), share_start(U, a.nwg, w + 1), 0, 0, 0, 0, 0};
   if (p.u0 == p.u1) return p;
   long long before = 0;
   for (int b0 = 0;; b0 += 64) {
-    const int n = b0 == 0 ? mine : b0 + lane < a.B ? lane_tiles<GEO>(a, b0 + lane) + tree : 0;
+    const int given = b0 == 0 || b0 + lane >= a.B ? mine : a.lens[b0 + lane];
+    const int n = b0 + lane < a.B ? cache_tiles<GEO>(a, given) + tree : 0;
     const int incl = wave_incl_scan(n);
     const u64 ends = __ballot(b0 + lane < a.B && before + (long long)incl * a.Hkv > p.u0);
     if (ends) {
       const int at = __ffsll((long long)ends) - 1;
       p.b = b0 + at;
       p.nt = (int)readlane_u32((uint32_t)n, at);
+      p.given = (int)readlane_u32((uint32_t)given, at);
       before += (long long)((int)readlane_u32((uint32_t)incl, at) - p.nt) * a.Hkv;
       const long long in = p.u0 - before;
       p.h = in >> 31 ? (int)(in / p.nt) : (int)((unsigned)in / (unsigned)p.nt);
@@ -452,6 +450,17 @@ __device__ __forceinline__ void join_one(const AttnArgs& a, JoinShared& s, int b
   const int r = i % a.QB, part = a.QB * a.D;
   const int lane = lane_id(), wave = uniform((int)threadIdx.x >> 6);
   const int j0 = n * wave / 4, j1 = n * (wave + 1) / 4;
+  float x[8][4];
+  auto load = [&](int from) {  // the sums of eight parts (past the wave's last: that one's, not used)
+#pragma unroll
+    for (int y = 0; y < 8; y++) {
+      const long long at = (long long)s.part[from + y < j1 ? from + y : j1 - 1] * part;
+#pragma unroll
+      for (int z = 0; z < 4; z++)
+        x[y][z] = z * 64 + lane < a.D ? a.part_o[at + part_at<GEO>(a.D, r, z * 64 + lane)] : 0.0f;
+    }
+  };
+  if (j0 < j1) load(j0);  // (on their way beside the maxima)
   float m = NEG;
   for (int j = j0 + lane; j < j1; j += 64) m = fmaxf(m, a.part_ml[2ll * (s.part[j] * a.QB + r)]);
   m = wave_maxf(m);
@@ -466,14 +475,7 @@ __device__ __forceinline__ void join_one(const AttnArgs& a, JoinShared& s, int b
     }
     const int cn = j1 - c < 64 ? j1 - c : 64;
     for (int j = 0; j < cn; j += 8) {
-      float x[8][4];
-#pragma unroll
-      for (int y = 0; y < 8; y++) {  // (past the last part: the last one's, not used)
-        const long long at = (long long)s.part[j + y < cn ? c + j + y : c + cn - 1] * part;
-#pragma unroll
-        for (int z = 0; z < 4; z++)
-          x[y][z] = z * 64 + lane < a.D ? a.part_o[at + part_at<GEO>(a.D, r, z * 64 + lane)] : 0.0f;
-      }
+      if (c + j > j0) load(c + j);
 #pragma unroll
       for (int y = 0; y < 8; y++) {
         if (j + y >= cn) break;
@@ -513,10 +515,13 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
   const int g = blockIdx.x % groups, bh = blockIdx.x / groups, h = bh % a.Hkv, b = bh / a.Hkv;
   int before, all;
   tiles_before<GEO>(a, b, before, all);
-  const int nt = cache_tiles<GEO>(a, b) + (a.T + GEO::TILE - 1) / GEO::TILE;
+  const int nt = cache_tiles<GEO>(a, uniform(a.lens[b])) + (a.T + GEO::TILE - 1) / GEO::TILE;
   const long long U = (long long)all * a.Hkv, s0 = (long long)before * a.Hkv + (long long)h * (nt + GEO::EXTRA), s1 = s0 + nt;
   const int N = a.nwg;
-  const int w0 = (int)(((s0 + 1) * N - 1) / U), w1 = (int)((s1 * N - 1) / U);
+  // (in 32 bits where the numbers allow: a division of 64 takes several times as long)
+  const bool narrow = (s1 * N) >> 32 == 0;
+  const int w0 = narrow ? (int)((unsigned)((s0 + 1) * N - 1) / (unsigned)U) : (int)(((s0 + 1) * N - 1) / U);
+  const int w1 = narrow ? (int)((unsigned)(s1 * N - 1) / (unsigned)U) : (int)((s1 * N - 1) / U);
   if (w0 == w1) return;
   const int i0 = g * R;  // (R divides QB: the rows lie in one row group)
   const int qb = i0 / a.QB, r0 = i0 - qb * a.QB;
@@ -546,29 +551,57 @@ __global__ __launch_bounds__(JOIN_NT) void join_kernel(AttnArgs a, int groups) {
   // A lane takes one row and, of the row's D / 4 fours, every sixteenth.
   const int i = i0 + (lane & 15), r = r0 + (lane & 15), sub = wave * 4 + (lane >> 4);
   const long long part = (long long)a.QB * a.D;
-  float m = NEG;
-  for (int j = 0; j < n; j++) m = fmaxf(m, a.part_ml[2ll * (s.part[j] * a.QB + r)]);
-  float l = 0.0f;
+  float m = NEG, l = 0.0f;
   f32x4 o[4] = {};
-  for (int j = 0; j < n; j += 2) {
-    f32x4 x[2][4];
-    float f[2];
+  f32x4 x[4][4];
+  float pm[4], pl[4];
+  // Of parts j .. j + 3, the first N of them (past the last part: that one's, not used).
+  auto load_ml = [&](int j) {
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-      const int p = s.part[j + k < n ? j + k : j];  // (past the last part: not used)
-      const float pm = a.part_ml[2ll * (p * a.QB + r)], pl = a.part_ml[2ll * (p * a.QB + r) + 1];
+    for (int k = 0; k < 4; k++) {
+      const long long at = 2ll * (s.part[j + k < n ? j + k : n - 1] * a.QB + r);
+      pm[k] = a.part_ml[at], pl[k] = a.part_ml[at + 1];
+    }
+  };
+  auto load_o = [&](int j) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int p = s.part[j + k < n ? j + k : n - 1];
 #pragma unroll
       for (int z = 0; z < 4; z++)
         if ((sub + 16 * z) * 4 < a.D) x[k][z] = *(const f32x4*)(a.part_o + p * part + part_at<GEO>(a.D, r, (sub + 16 * z) * 4));
-      f[k] = j + k >= n || pm == NEG ? 0.0f : exp2_hw(pm - m);
-      if (j + k < n) l += pm == NEG ? pl : f[k] * pl;  // (a part without weights has the sum 0, or NaN)
     }
+  };
+  auto top = [&](int j) {
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
+    for (int k = 0; k < 4; k++)
+      if (j + k < n) m = fmaxf(m, pm[k]);
+  };
+  auto add = [&](int j) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
       if (j + k >= n) break;
+      const float f = pm[k] == NEG ? 0.0f : exp2_hw(pm[k] - m);
+      l += pm[k] == NEG ? pl[k] : f * pl[k];  // (a part without weights has the sum 0, or NaN)
 #pragma unroll
       for (int z = 0; z < 4; z++)
-        if ((sub + 16 * z) * 4 < a.D) o[z] += x[k][z] * f[k];
+        if ((sub + 16 * z) * 4 < a.D) o[z] += x[k][z] * f;
+    }
+  };
+  if (n <= 4) {  // (as a rule: everything is asked for at once)
+    load_ml(0);
+    load_o(0);
+    top(0);
+    add(0);
+  } else {
+    for (int j = 0; j < n; j += 4) {
+      load_ml(j);
+      top(j);
+    }
+    for (int j = 0; j < n; j += 4) {
+      load_ml(j);
+      load_o(j);
+      add(j);
     }
   }
   if (i >= a.M) return;

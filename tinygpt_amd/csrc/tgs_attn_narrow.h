@@ -290,9 +290,9 @@ struct Narrow {
     for (int d = 0; d < DT16; d++) v.v[d] ^= odd_of<DT>(v.v[d]);
   }
 
-  // Tiles [t0, t1) of (b, h); full: they are all of it.  part: the workspace's rows otherwise.
-  __device__ __forceinline__ void segment(Shared& s, int t0, int t1, bool full, long long part) {
-    const int given = uniform(a.lens[b]);
+  // Tiles [t0, t1) of (b, h), a sequence of the length `given`; full: they are all of
+  // it.  part: the workspace's rows otherwise.
+  __device__ __forceinline__ void segment(Shared& s, int given, int t0, int t1, bool full, long long part) {
     len = clamp_len(a, given);
     nc = (len + GEO::TILE - 1) / GEO::TILE;
     table = a.tables + (long long)b * a.P;
@@ -462,25 +462,27 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void narrow_kernel(AttnA
   if (a.nwg == 0) {
     n.b = blockIdx.x / a.Hkv;
     n.h = blockIdx.x % a.Hkv;
-    n.segment(s, 0, cache_tiles<GEO>(a, n.b) + tree, true, 0);
+    const int given = uniform(a.lens[n.b]);
+    n.segment(s, given, 0, cache_tiles<GEO>(a, given) + tree, true, 0);
     return;
   }
-  const Place at0 = find_place<GEO>(a, blockIdx.x);
-  const long long u0 = at0.u0, u1 = at0.u1;
-  int b = at0.b, h = at0.h, at = at0.at, nt = at0.nt;
-  for (long long u = u0; u < u1;) {
-    const int end = nt - at < u1 - u ? nt : at + (int)(u1 - u);
-    const int real = nt - GEO::EXTRA;
-    if (at < real) {
-      n.b = b;
-      n.h = h;
-      n.segment(s, at, end < real ? end : real, at == 0 && end >= real, ((long long)blockIdx.x * 2 + (u != u0)) * a.QB);
+  Place p = find_place<GEO>(a, blockIdx.x);
+  for (long long u = p.u0; u < p.u1;) {
+    const int end = p.nt - p.at < p.u1 - u ? p.nt : p.at + (int)(p.u1 - u);
+    const int real = p.nt - GEO::EXTRA;
+    if (p.at < real) {
+      n.b = p.b;
+      n.h = p.h;
+      n.segment(s, p.given, p.at, end < real ? end : real, p.at == 0 && end >= real, ((long long)blockIdx.x * 2 + (u != p.u0)) * a.QB);
     }
-    u += end - at;
-    at = 0;
-    if (++h == a.Hkv) {
-      h = 0;
-      if (++b < a.B) nt = cache_tiles<GEO>(a, b) + tree + GEO::EXTRA;
+    u += end - p.at;
+    p.at = 0;
+    if (++p.h == a.Hkv) {
+      p.h = 0;
+      if (++p.b < a.B) {
+        p.given = uniform(a.lens[p.b]);
+        p.nt = cache_tiles<GEO>(a, p.given) + tree + GEO::EXTRA;
+      }
     }
   }
 }

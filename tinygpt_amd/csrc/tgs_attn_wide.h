@@ -300,8 +300,7 @@ struct Wide {
     sched_fence();
   }
 
-  __device__ __forceinline__ void segment(Shared& s, int t0, int t1, bool full, long long part) {
-    const int given = uniform(a.lens[b]);
+  __device__ __forceinline__ void segment(Shared& s, int given, int t0, int t1, bool full, long long part) {
     len = clamp_len(a, given);
     nc = (len + WTILE - 1) / WTILE;
     table = a.tables + (long long)b * a.P;
@@ -482,7 +481,8 @@ __global__ __launch_bounds__(QW * 64, D == 256 ? 1 : 2) void wide_kernel(AttnArg
     n.qb = blockIdx.x % a.nqb;
     n.b = seg / a.Hkv;
     n.h = seg % a.Hkv;
-    n.segment(s, 0, cache_tiles<WideGeo>(a, n.b) + tree, true, 0);
+    const int given = uniform(a.lens[n.b]);
+    n.segment(s, given, 0, cache_tiles<WideGeo>(a, given) + tree, true, 0);
     if (n.odd) n.put_odd(true, 0);
     return;
   }
@@ -494,27 +494,30 @@ __global__ __launch_bounds__(QW * 64, D == 256 ? 1 : 2) void wide_kernel(AttnArg
   const Place at0 = find_place<WideGeo>(a, w);
   const long long u0 = at0.u0, u1 = at0.u1;
   auto walk = [&](auto f) {
-    int b = at0.b, h = at0.h, at = at0.at, nt = at0.nt;
+    int b = at0.b, h = at0.h, at = at0.at, nt = at0.nt, given = at0.given;
     for (long long u = u0; u < u1;) {
       const int end = nt - at < u1 - u ? nt : at + (int)(u1 - u);
       const int real = nt - WideGeo::EXTRA;
       if (at < real) {
         n.b = b;
         n.h = h;
-        f(at, end < real ? end : real, real, at == 0 && end >= real, ((long long)(n.qb * a.nwg + w) * 2 + (u != u0)) * a.QB);
+        f(given, at, end < real ? end : real, real, at == 0 && end >= real, ((long long)(n.qb * a.nwg + w) * 2 + (u != u0)) * a.QB);
       }
       u += end - at;
       at = 0;
       if (++h == a.Hkv) {
         h = 0;
-        if (++b < a.B) nt = cache_tiles<WideGeo>(a, b) + tree + WideGeo::EXTRA;
+        if (++b < a.B) {
+          given = uniform(a.lens[b]);
+          nt = cache_tiles<WideGeo>(a, given) + tree + WideGeo::EXTRA;
+        }
       }
     }
   };
-  walk([&](int t0, int t1, int, bool full, long long part) { n.segment(s, t0, t1, full, part); });
+  walk([&](int given, int t0, int t1, int, bool full, long long part) { n.segment(s, given, t0, t1, full, part); });
   // (Behind everything: code to jump over in a segment costs 1 us of 33, for 16
   // sequences of 1000 to 3000 tokens and 48 rows of 128.)
-  if (n.odd) walk([&](int, int t1, int real, bool full, long long part) {
+  if (n.odd) walk([&](int, int, int t1, int real, bool full, long long part) {
     if (t1 == real) n.put_odd(full, part);
   });
 }

@@ -306,28 +306,25 @@ __device__ __forceinline__ void plan(const KvForkArgs& a, PlanShared& s, unsigne
 // The blocks of row r's page that are in use lie contiguous per head: copies
 // those of layer y / 2, keys or values (and with them their scales).  A block's
 // vectors of 16 bytes are as many as a head has dimensions, of 8 tokens in 16
-// bits or of 16 in 8.
+// bits or of 16 in 8 (E8).
+template <bool E8>
 __device__ __forceinline__ void copy_page(const KvForkArgs& a, const int4& c, int y) {
   if (c.z == 0) return;
   const int l = y >> 1, D = a.c.head_dim, H = a.c.kv_heads;
   const bool val = y & 1;
-  const int bytes = a.scales ? 1 : 2, per = a.scales ? e8::BLOCK : 8;
-  unsigned char* pool = (unsigned char*)(val ? a.c.v : a.c.k) + l * (val ? a.c.v_layer : a.c.k_layer) * bytes;
-  const long long ps = (val ? a.c.v_page : a.c.k_page) * bytes;
+  constexpr int BYTES = E8 ? 1 : 2, PER = E8 ? e8::BLOCK : 8;
+  unsigned char* pool = (unsigned char*)(val ? a.c.v : a.c.k) + l * (val ? a.c.v_layer : a.c.k_layer) * BYTES;
+  const long long ps = (val ? a.c.v_page : a.c.k_page) * BYTES;
   const uint4* from = (const uint4*)(pool + c.x * ps);
   uint4* to = (uint4*)(pool + c.y * ps);
   const int n = c.z * D;  // vectors of a head's blocks
-  const int blocks = (1 << a.page_shift) / per;
+  const int hs = (D << a.page_shift) / PER;  // and of its page
   // a wave a head, so that every thread has work where a head's blocks are few
   for (int h = threadIdx.x >> 6; h < H; h += blockDim.x >> 6) {
-    for (int i = lane_id(); i < n; i += 64) to[((long long)h * blocks) * D + i] = from[((long long)h * blocks) * D + i];
-    if (a.scales) {
-      const uint8_t* sc = a.scales + l * a.s_layer;
-      uint8_t* st = a.scales + l * a.s_layer;
-      for (int i = lane_id(); i < c.z; i += 64) {
-        const long long at = ((long long)h * blocks + i) * 2 + val;
-        st[c.y * a.s_page + at] = sc[c.x * a.s_page + at];
-      }
+    for (int i = lane_id(); i < n; i += 64) to[(long long)h * hs + i] = from[(long long)h * hs + i];
+    if constexpr (E8) {
+      uint8_t* scales = a.scales + l * a.s_layer + ((h << a.page_shift) / PER) * 2 + val;
+      for (int i = lane_id(); i < c.z; i += 64) scales[c.y * a.s_page + 2 * i] = scales[c.x * a.s_page + 2 * i];
     }
   }
 }
@@ -340,17 +337,21 @@ __global__ __launch_bounds__(KV_PLAN_NT) void plan_kernel(KvForkArgs a) {
 }
 
 // Workgroup (row, layer and pool).
-__global__ __launch_bounds__(KV_NT) void copy_kernel(KvForkArgs a) { copy_page(a, a.copies[blockIdx.x], blockIdx.y); }
+template <bool E8>
+__global__ __launch_bounds__(KV_NT) void copy_kernel(KvForkArgs a) {
+  copy_page<E8>(a, a.copies[blockIdx.x], blockIdx.y);
+}
 
 // Both in one launch, every workgroup planning for itself: where no more than
 // a workgroup a CU copies, planning 256 times at once costs less than a second
 // launch (4 beams of 530 tokens, 16 layers: kernels of 12 us in two, 5.8 in one).
+template <bool E8>
 __global__ __launch_bounds__(KV_PLAN_NT) void fork_kernel(KvForkArgs a) {
   TGS_STATIC_SMEM(PlanShared, s);
   TGS_DYN_SMEM(dyn);
   plan<true>(a, s, dyn, blockIdx.x == 0 && blockIdx.y == 0, blockIdx.x);
   __syncthreads();
-  copy_page(a, s.copy, blockIdx.y);
+  copy_page<E8>(a, s.copy, blockIdx.y);
 }
 
 }  // namespace kv
@@ -383,7 +384,11 @@ size_t kv_fork_lds(int n_pages, int rows) {
 hipError_t launch_kv_fork(const KvForkArgs& a, int num_cu, hipStream_t st) {
   const size_t lds = kv_fork_lds(a.c.n_pages, a.R);
   if (lds && (long long)a.R * 2 * a.c.layers <= num_cu) {
-    hipLaunchKernelGGL(kv::fork_kernel, dim3(a.R, 2 * a.c.layers), dim3(KV_PLAN_NT), lds, st, a);
+    const dim3 grid(a.R, 2 * a.c.layers);
+    if (a.scales)
+      hipLaunchKernelGGL(kv::fork_kernel<true>, grid, dim3(KV_PLAN_NT), lds, st, a);
+    else
+      hipLaunchKernelGGL(kv::fork_kernel<false>, grid, dim3(KV_PLAN_NT), lds, st, a);
     return hipGetLastError();
   }
   if (lds)
@@ -392,15 +397,20 @@ hipError_t launch_kv_fork(const KvForkArgs& a, int num_cu, hipStream_t st) {
     hipLaunchKernelGGL(kv::plan_kernel<false>, dim3(1), dim3(KV_PLAN_NT), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kv::copy_kernel, dim3(a.R, 2 * a.c.layers), dim3(KV_NT), 0, st, a);
+  if (a.scales)
+    hipLaunchKernelGGL(kv::copy_kernel<true>, dim3(a.R, 2 * a.c.layers), dim3(KV_NT), 0, st, a);
+  else
+    hipLaunchKernelGGL(kv::copy_kernel<false>, dim3(a.R, 2 * a.c.layers), dim3(KV_NT), 0, st, a);
   return hipGetLastError();
 }
 
 hipError_t set_kv_fork_lds_limit(size_t bytes) {
   const int n = (int)(bytes < FORK_LDS ? bytes : FORK_LDS);
-  const hipError_t e = hipFuncSetAttribute((const void*)kv::plan_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, n);
-  const hipError_t f = hipFuncSetAttribute((const void*)kv::fork_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, n);
-  return e != hipSuccess ? e : f;
+  for (const void* f : {(const void*)kv::plan_kernel<true>, (const void*)kv::fork_kernel<false>, (const void*)kv::fork_kernel<true>}) {
+    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, n);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace tgs
