@@ -274,6 +274,17 @@ __device__ __forceinline__ uint4 tg_load_nt(const void* p) {
 #endif
 }
 
+// A 16-byte store of what this launch does not read again (copied and new cache
+// rows): marked non-temporal.
+__device__ __forceinline__ void tg_store_nt(void* p, const uint4& x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef unsigned v4u __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store(v4u{x.x, x.y, x.z, x.w}, (v4u*)p);
+#else
+  *(uint4*)p = x;
+#endif
+}
+
 // Per-half signed 16-bit maxima of two words (one packed max).
 __device__ __forceinline__ uint32_t pk_max_i16(uint32_t a, uint32_t b) {
 #if defined(__HIP_DEVICE_COMPILE__)

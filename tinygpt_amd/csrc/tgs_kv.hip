@@ -4,9 +4,10 @@
 // [page][kv_head][token / 8][D][8]: the eight tokens of a block lie next to
 // each other for each d, which is the operand order of the attention's second
 // product.  No arithmetic: every kernel here moves 16-bit values and is bound
-// by bytes, or by latency for single tokens.  Measured: prompts of 300 to 2048
-// tokens, 16 layers, 176 us (923 MB, 5.2 TB/s read and written); pages of 128
-// forked beams 94 us (403 MB, 4.3 TB/s).
+// by bytes, or by latency for single tokens; appended keys may turn by their
+// positions on the way, in floats.  Measured: prompts of 300 to 2048 tokens, 16
+// layers, 175 us (923 MB, 5.3 TB/s read and written); pages of 128 forked beams 83 us
+// (403 MB, 4.9 TB/s), of an 8-bit cache 51 us (220 MB, 4.3 TB/s).
 #include "tgs_device.h"
 #include "tgs_e8.h"
 #include "tgs_kv.h"
@@ -319,9 +320,20 @@ __device__ __forceinline__ void copy_page(const KvForkArgs& a, const int4& c, in
   uint4* to = (uint4*)(pool + c.y * ps);
   const int n = c.z * D;  // vectors of a head's blocks
   const int hs = (D << a.page_shift) / PER;  // and of its page
-  // a wave a head, so that every thread has work where a head's blocks are few
+  // A wave a head, so that every thread has work where a head's blocks are few.
+  // (Non-temporal stores: 83 us where plain ones take 100, an 8-bit cache's 51 : 60;
+  // one vector at a time 66, loads that are non-temporal too 65.)
   for (int h = threadIdx.x >> 6; h < H; h += blockDim.x >> 6) {
-    for (int i = lane_id(); i < n; i += 64) to[(long long)h * hs + i] = from[(long long)h * hs + i];
+    for (int i0 = 0; i0 < n; i0 += 256) {  // (four on their way)
+      const int i = i0 + lane_id();
+      uint4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (i + 64 * j < n) x[j] = from[(long long)h * hs + i + 64 * j];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (i + 64 * j < n) tg_store_nt(to + (long long)h * hs + i + 64 * j, x[j]);
+    }
     if constexpr (E8) {
       uint8_t* scales = a.scales + l * a.s_layer + ((h << a.page_shift) / PER) * 2 + val;
       for (int i = lane_id(); i < c.z; i += 64) scales[c.y * a.s_page + 2 * i] = scales[c.x * a.s_page + 2 * i];
