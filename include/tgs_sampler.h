@@ -71,7 +71,7 @@ typedef enum {
   TGS_ETOOBIG = -5     /* size beyond what the handle was created for     */
 } tgs_status;
 
-typedef enum { TGS_F32 = 0, TGS_BF16 = 1, TGS_F16 = 2 /* key/value caches only */ } tgs_dtype;
+typedef enum { TGS_F32 = 0, TGS_BF16 = 1, TGS_F16 = 2 /* key/value caches, their rows, rotation */ } tgs_dtype;
 
 #define TGS_FLAG_GREEDY 1 /* decode this row by argmax regardless of T */
 

@@ -157,7 +157,9 @@ struct Narrow16 {
   static constexpr int TILE = 32, EXTRA = 8;
   static constexpr bool ROWS = true;
 };
-struct Narrow8 {  // (of an 8-bit cache: as many bytes a tile)
+// (Of an 8-bit cache: as many bytes a tile.  EXTRA for 32 sequences of 100 to 4096
+// tokens, 32 rows of 128, us: 2 55, 4 49.2, 6 48.4, 8 47.2.)
+struct Narrow8 {
   static constexpr int TILE = 64, EXTRA = 8;
   static constexpr bool ROWS = true;
 };

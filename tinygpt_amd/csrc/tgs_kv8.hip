@@ -10,6 +10,12 @@
 // largest magnitude is one reduction over the wave.  Numbers stay in 16 bits, two to
 // an instruction, from the load to the conversion (magnitudes compare as integers);
 // only keys that turn become floats.
+//
+// 16 layers, 8 key heads of 128: prompts of 300 to 2048 tokens, keys turned, 147 to 155
+// us (692 MB, 4.6 TB/s; with floats from the load on and a thread to a number's unit
+// 359); single tokens of 8 sequences 5.1 (latency); 32 layers, 64 trees of 63 nodes, up
+// to 8 taken, 44 us (first 101).  There the bytes that have to move are 57 MB, but the
+// values of a few tokens lie in whole sectors of other tokens', read and written.
 #include <type_traits>
 
 #include "tgs_device.h"
@@ -558,7 +564,9 @@ __global__ __launch_bounds__(STEP_NT) void step_kernel(KvWriteArgs a, int round)
 template <typename DT, bool COMMIT, bool ROT>
 hipError_t run(const KvWriteArgs& a, int num_cu, hipStream_t st) {
   // Layers to a workgroup: as many as leave eight workgroups a CU (half of them for
-  // blocks that are not there, as a rule).
+  // blocks that are not there, as a rule).  One always, this rule, eight always (us):
+  // 64 trees of 32 layers 71, 45, 53; prompts of 16 layers 217, 153, 157; one tree of
+  // 16 layers 5.9, 5.9, 15.5.
   const long long all = 2ll * a.nblk * a.B * a.c.layers;
   int per = (int)(all / (8ll * num_cu));
   per = per < 1 ? 1 : per > 8 ? 8 : per;

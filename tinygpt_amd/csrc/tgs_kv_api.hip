@@ -462,6 +462,9 @@ int tgs_rotate(tgs_handle h, tgs_dtype dt, const tgs_rotate_rows* q, const tgs_r
   a.T = T;
   a.D = head_dim;
   a.dtype = dt;
+  // Several tokens a workgroup where all CUs have work then.  Four against one (us): 4,032
+  // tokens of 10 heads of 64 5.4 : 6.9, of 40 heads of 128 16.3 : 16.2; 1,008 of those
+  // 10.5 : 7.5; 8 tokens 6.0 : 4.1.
   a.tokens = (int64_t)B * T >= 4 * h->num_cu && heads * units * tgs::ROTATE_TOKENS <= 65535 ? tgs::ROTATE_TOKENS : 1;
   a.units = tgs::fast_div(units);
   a.heads = tgs::fast_div((unsigned)heads);
