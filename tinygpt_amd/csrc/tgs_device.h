@@ -274,7 +274,7 @@ __device__ __forceinline__ uint4 tg_load_nt(const void* p) {
 #endif
 }
 
-// A 16-byte store of what this launch does not read again (copied and new cache
+// A store of 16 bytes of what this launch does not read again (copied and new cache
 // rows): marked non-temporal.
 __device__ __forceinline__ void tg_store_nt(void* p, const uint4& x) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -282,6 +282,15 @@ __device__ __forceinline__ void tg_store_nt(void* p, const uint4& x) {
   __builtin_nontemporal_store(v4u{x.x, x.y, x.z, x.w}, (v4u*)p);
 #else
   *(uint4*)p = x;
+#endif
+}
+// The same of 8 bytes.
+__device__ __forceinline__ void tg_store_nt(void* p, const uint2& x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef unsigned v2u __attribute__((ext_vector_type(2)));
+  __builtin_nontemporal_store(v2u{x.x, x.y}, (v2u*)p);
+#else
+  *(uint2*)p = x;
 #endif
 }
 

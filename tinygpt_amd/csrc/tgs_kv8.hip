@@ -11,10 +11,10 @@
 // an instruction, from the load to the conversion (magnitudes compare as integers);
 // only keys that turn become floats.
 //
-// 16 layers, 8 key heads of 128: prompts of 300 to 2048 tokens, keys turned, 147 to 155
-// us (692 MB, 4.6 TB/s; with floats from the load on and a thread to a number's unit
+// 16 layers, 8 key heads of 128: prompts of 300 to 2048 tokens, keys turned, 145 to 147
+// us (692 MB, 4.7 TB/s; with floats from the load on and a thread to a number's unit
 // 359); single tokens of 8 sequences 5.1 (latency); 32 layers, 64 trees of 63 nodes, up
-// to 8 taken, 44 us (first 101).  There the bytes that have to move are 57 MB, but the
+// to 8 taken, 43 us (first 101).  There the bytes that have to move are 57 MB, but the
 // values of a few tokens lie in whole sectors of other tokens', read and written.
 #include <type_traits>
 
@@ -29,7 +29,7 @@ namespace kv8 {
 
 using kv::div_by;
 
-constexpr int NT = 512;
+constexpr int NT = 512;  // (64 trees 45 us, with 256 53, with 1024 58)
 
 template <bool ROT>
 struct Shared {
@@ -245,8 +245,8 @@ struct Part {
   __device__ __forceinline__ void put_key(const KeyUnit& x, uint8_t* to, uint2 lo, uint2 hi) const {
     if (!x.fresh) return;
     uint8_t* p = to + x.token * D;
-    *(uint2*)(p + x.u.a) = lo;
-    *(uint2*)(p + x.u.b) = hi;
+    tg_store_nt(p + x.u.a, lo);
+    tg_store_nt(p + x.u.b, hi);
   }
   // A scale of NaN, which another program has written, makes NaN of what is added too.
   static __device__ __forceinline__ uint32_t code(uint32_t c, int byte) { return !WHOLE && byte == 255 ? 0x7F7F7F7Fu : c; }
@@ -336,8 +336,8 @@ struct Part {
         uint8_t* p = to + x.d * e8::BLOCK + x.first;
 #pragma unroll
         for (int d = 0; d < 2; d++, p += e8::BLOCK) {
-          if constexpr (H == 2) *(uint4*)p = make_uint4(c[0][d].x, c[0][d].y, c[1][d].x, c[1][d].y);
-          else *(uint2*)p = c[0][d];
+          if constexpr (H == 2) tg_store_nt(p, make_uint4(c[0][d].x, c[0][d].y, c[1][d].x, c[1][d].y));
+          else tg_store_nt(p, c[0][d]);
         }
       }
       return;
@@ -366,14 +366,18 @@ struct Part {
 };
 
 // Workgroup (sequence b, x, layers from l0 on, keys or values) over the 16-token blocks
-// x, x + step, ... of the positions that b's new rows take.  The layers of a workgroup
+// x, x + step, ... of the positions that b's new rows take.  An append's values come
+// behind all keys, so that what runs together reads and writes the same pools (prompts
+// 152 us where they alternate 160; a commit, of few workgroups, alternates: one tree
+// 6.0 where keys first take 6.4).  The layers of a workgroup
 // share the look at the sequence and the cosines and sines of a block's positions.
 template <typename DT, int NU, bool COMMIT, bool ROT>
 __global__ __launch_bounds__(NT) void write_kernel(KvWriteArgs a, int per, int step, FastDiv heads) {
   TGS_STATIC_SMEM(Shared<ROT>, sh);
   kv::WriteHead& s = sh.head;
-  const bool values = blockIdx.y & 1;
-  const int b = blockIdx.x, y = blockIdx.y >> 1, g = y / step, x = y - g * step, l0 = g * per;
+  const int b = blockIdx.x, half = gridDim.y >> 1;
+  const bool values = COMMIT ? blockIdx.y & 1 : (int)blockIdx.y >= half;
+  const int y = COMMIT ? blockIdx.y >> 1 : blockIdx.y - (values ? half : 0), g = y / step, x = y - g * step, l0 = g * per;
   const int tid = threadIdx.x;
   const int len = a.lens[b], n = kv::rows_of<COMMIT>(a, s, b);
   const int* table = a.tables + (long long)b * a.P;
@@ -564,12 +568,14 @@ __global__ __launch_bounds__(STEP_NT) void step_kernel(KvWriteArgs a, int round)
 template <typename DT, bool COMMIT, bool ROT>
 hipError_t run(const KvWriteArgs& a, int num_cu, hipStream_t st) {
   // Layers to a workgroup: as many as leave eight workgroups a CU (half of them for
-  // blocks that are not there, as a rule).  One always, this rule, eight always (us):
-  // 64 trees of 32 layers 71, 45, 53; prompts of 16 layers 217, 153, 157; one tree of
-  // 16 layers 5.9, 5.9, 15.5.
+  // blocks that are not there, as a rule), and at most four (layer, head)s to a wave.  One
+  // always, this rule, eight always (us): 64 trees of 32 layers, 8 heads of 128, 71, 45,
+  // 53; prompts of 16 layers 217, 148, 157; one tree of 16 layers 5.9, 5.9, 15.5.
   const long long all = 2ll * a.nblk * a.B * a.c.layers;
   int per = (int)(all / (8ll * num_cu));
-  per = per < 1 ? 1 : per > 8 ? 8 : per;
+  const int most = 4 * NT / 64 / a.c.kv_heads;
+  per = per < most ? per : most;
+  per = per < 1 ? 1 : per;
   per = per < a.c.layers ? per : a.c.layers;
   const int groups = (a.c.layers + per - 1) / per, tasks = a.c.kv_heads * per;
   if (groups > 32767) return hipErrorInvalidValue;
