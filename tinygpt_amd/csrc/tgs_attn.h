@@ -38,6 +38,15 @@ namespace attn {
 typedef float f32x4 __attribute__((vector_size(16)));
 typedef float f32x16 __attribute__((vector_size(64)));
 typedef uint32_t Vec __attribute__((vector_size(16)));  // eight 16-bit values
+
+// 16 aligned bytes that are read once; NT: without a place in the caches.
+template <bool NT>
+__device__ __forceinline__ Vec load_once(const void* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (NT) return __builtin_nontemporal_load((const Vec*)p);
+#endif
+  return *(const Vec*)p;
+}
 __device__ __forceinline__ Vec vec16(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return Vec{a, b, c, d}; }
 // At any alignment of the values.
 __device__ __forceinline__ Vec load16(const uint16_t* p) {

@@ -13,12 +13,12 @@
 // scale along, when they are used: the lane's sixteen tokens are one block of
 // values, and the rows that it brings to the first product are one block of keys.
 //
-// 16-bit, D = 128, 8 key heads: one sequence of 131,000 tokens 96 us (537 MB,
-// 5.6 TB/s; a plain read reaches 6.2); 32 sequences of 100 to 4096 tokens 62 us
-// (280 MB, 4.5 TB/s), where a worker starts and ends about 1.5 of the
-// (sequence, key head) pairs.  8-bit: the one sequence 62 us (269 MB, 4.3 TB/s; a
-// longer one adds 1 us for 6.1 MB), the 32 46 us (143 MB, 3.1 TB/s).  What is not
-// reading is about 15 us a call, as with 16 bits: the first requests' chain
+// 16-bit, D = 128, 8 key heads, whole calls: one sequence of 131,000 tokens 94 us
+// (537 MB, 5.7 TB/s; a plain read reaches 6.2); 32 sequences of 100 to 4096 tokens 64 us
+// (280 MB, 4.4 TB/s), where a worker starts and ends about 1.5 of the (sequence, key
+// head) pairs.  8-bit: the one sequence 58 us (269 MB, 4.6 TB/s), the 32 46 us
+// (143 MB, 3.1 TB/s; 39 where three such caches take turns, whose keys stay in the
+// memory-side cache).  What is not reading is about 15 us a call, as with 16 bits: the first requests' chain
 // (length, entry, tile), the joining of waves, and 6 to 7 us of the parts' launch.
 // Requesting the drafted rows before the last tiles are done costs more registers
 // than there are (spills: 51 us for the 32), wave priorities change nothing.
@@ -40,6 +40,14 @@ struct Narrow {
   static constexpr int ROWS = 16 * QT;
   static constexpr int XB = GEO::TILE / 16;  // products of 16 tokens in a tile
   static constexpr int PER = GEO::TILE / 4;  // tokens of a lane in it, consecutive ones
+  // What is read once takes no place in the caches: values, and keys of rows of at least
+  // 256 bytes (a shorter row's lines are asked for again by the requests that follow).
+  // Caches of 10 and more calls in turn, all plain / values / both (us): 32 sequences of
+  // 100 to 4096 tokens, D = 128, 8 bits 46.8 / 45.7 / 47.6, 16 bits 70.7 / 66.2 / 63.8;
+  // 131,000 tokens 62.0 / 57.9 / 61.8, 103 / 93.4 / 94.1; 64 sequences of 3000 to 9000,
+  // 16 rows of 256, 89.5 / 82.5 / 81.2, 165 / 161 / 139; of 96 43.3 / 40.9 / 41.9,
+  // 75.9 / 72.0 / 75.5.
+  static constexpr bool ROWS_NT = D * (E8 ? 1 : 2) >= 256;
   struct Shared {
     f32x4 o[NW][DT16 * QT][64];
     float ml[NW][ROWS][2];
@@ -127,7 +135,7 @@ struct Narrow {
       if constexpr (E8) {
         const uint8_t* base = (const uint8_t*)a.k + at + p * D;
 #pragma unroll
-        for (int c = 0; c < D / 64; c++) k.k[x][c] = *(const Vec*)(base + c * 64 + grp * 16);
+        for (int c = 0; c < D / 64; c++) k.k[x][c] = load_once<ROWS_NT>(base + c * 64 + grp * 16);
         if constexpr (D % 64 != 0) {
           const uint2 w = *(const uint2*)(base + D / 64 * 64 + grp * 8);
           k.k[x][D / 64] = vec16(w.x, w.y, 0, 0);
@@ -135,7 +143,7 @@ struct Narrow {
       } else {
         const uint16_t* base = (const uint16_t*)a.k + at + grp * 8;
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) k.k[x][kk] = *(const Vec*)(base + p * D + kk * 32);
+        for (int kk = 0; kk < KK; kk++) k.k[x][kk] = load_once<ROWS_NT>(base + p * D + kk * 32);
       }
     }
   }
@@ -147,10 +155,10 @@ struct Narrow {
     if constexpr (E8) {
       v.scale = scale_at(page, p, 1);
 #pragma unroll
-      for (int d = 0; d < DT16; d++) v.v[d] = *(const Vec*)((const uint8_t*)a.v + at + d * 256);
+      for (int d = 0; d < DT16; d++) v.v[d] = load_once<true>((const uint8_t*)a.v + at + d * 256);
     } else {
 #pragma unroll
-      for (int d = 0; d < DT16; d++) v.v[d] = *(const Vec*)((const uint16_t*)a.v + at + d * 128);
+      for (int d = 0; d < DT16; d++) v.v[d] = load_once<true>((const uint16_t*)a.v + at + d * 128);
     }
   }
 

@@ -321,8 +321,10 @@ __device__ __forceinline__ void copy_page(const KvForkArgs& a, const int4& c, in
   const int n = c.z * D;  // vectors of a head's blocks
   const int hs = (D << a.page_shift) / PER;  // and of its page
   // A wave a head, so that every thread has work where a head's blocks are few.
-  // (Non-temporal stores: 83 us where plain ones take 100, an 8-bit cache's 51 : 60;
-  // one vector at a time 66, loads that are non-temporal too 65.)
+  // (Non-temporal stores leave the memory-side cache to the pages that are copied, where
+  // it still has them: 83 us where plain ones take 100, an 8-bit cache's 51 : 60, and
+  // where it does not 60 : 61.  One vector at a time 66, loads that are non-temporal too
+  // 65.)
   for (int h = threadIdx.x >> 6; h < H; h += blockDim.x >> 6) {
     for (int i0 = 0; i0 < n; i0 += 256) {  // (four on their way)
       const int i = i0 + lane_id();
