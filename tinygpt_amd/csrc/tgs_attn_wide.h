@@ -15,7 +15,7 @@
 // product's rate).  28 us of it are not in the tile loop.  In the loop a tile's
 // LDS reads, products and weights follow each other in both waves of a SIMD;
 // 64 rows a wave would halve the reads but need copies between the register
-// files and scratch (165 us).  Of an 8-bit cache the same 91 to 94 us: half the bytes
+// files and scratch (165 us).  Of an 8-bit cache the same 88 to 94 us: half the bytes
 // do not help, as reading does not bound it, and the conversions come on top (matrix
 // units are busy 43 % of the waves' time, vector ones 48 %, mostly in turn).
 #pragma once
