@@ -7,8 +7,8 @@ import gpu_harness as H
 import kv8_cases as K
 import kv_cases as C
 from test_gpu_kv import dev
-from test_gpu_kv8 import pools
-from test_kv8_edges import SHAPES, check_unseen, unseen_garbage
+from test_gpu_kv8 import pools, run_attn
+from test_kv8_edges import SHAPES, check_unseen, unseen_garbage, widened
 from test_kv8_sim import FREQ, attn_inputs, write_inputs
 from test_kv_sim import commit_ids, gen
 
@@ -24,9 +24,21 @@ def test_unseen_garbage(sampler, shape):
         H.log(f"8-bit attention, garbage in unseen nodes {shape} {dt} chain={chain}")
         lse = torch.empty(q.shape[:3], device=DEV)
         _, (k, v, s) = pools(p)
-        out = sampler.tree_attention(dev(q), dev(kn), dev(vn), k, v, dev(tabs), dev(lens), parents=dev(par), lse=lse, scales=s)
-        torch.cuda.synchronize()
-        check_unseen(out.cpu(), lse.cpu(), args)
+        for more in (0, 1700):
+            slots = dev(widened(args, more)[4])
+            out = sampler.tree_attention(dev(q), dev(kn), dev(vn), k, v, slots, dev(lens), parents=dev(par), lse=lse, scales=s)
+            torch.cuda.synchronize()
+            check_unseen(out.cpu(), lse.cpu(), args)
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D,lens,page,dt", [
+    (1, 4, 2, 64, [1500, 0, 77, 1535], 16, F16), (5, 8, 2, 128, [1200, 130, 1536], 64, BF16), (3, 2, 1, 96, [1000, 1], 32, BF16),
+    (20, 1, 1, 64, [933, 300], 16, F16), (2, 8, 1, 256, [460, 90], 64, BF16), (2, 20, 1, 96, [1500, 40], 16, F16)])
+def test_shares_of_few_rows(sampler, T, Hq, Hkv, D, lens, page, dt):
+    """Workers that share (sequence, key head)s, and the unshared form, of the same rows."""
+    args = attn_inputs(T + D, len(lens), T, Hq, Hkv, D, lens, page, dt)
+    for more in (0, 1700):
+        run_attn(sampler, widened(args, more))
 
 
 @pytest.mark.parametrize("dims,pairs", [(0, False), (16, True)])

@@ -7,7 +7,7 @@ import torch
 
 import kv8_cases as K
 import kv_edges as E
-from test_kv8_sim import attn_inputs
+from test_kv8_sim import attn_inputs, run_attn
 from test_kv_sim import check_attn, sim  # noqa: F401  (sim: a fixture)
 
 BF16, F16 = torch.bfloat16, torch.float16
@@ -35,10 +35,29 @@ def check_unseen(out, lse, args):
 def test_unseen_garbage(sim, shape, chain):  # noqa: F811
     args = unseen_garbage(*shape, chain=chain)
     q, kn, vn, p, tabs, lens, par = args
-    for kw in ({}, dict(max_len=1000)):
-        rc, out, lse = K.sim_attention(sim, q, kn, vn, p, tabs, lens, par, None, **kw)
+    for more in (0, 1700):
+        wide = widened(args, more)[4]
+        rc, out, lse = K.sim_attention(sim, q, kn, vn, p, wide, lens, par, None)
         assert rc == 0
         check_unseen(out, lse, args)
+
+
+def widened(args, tokens):
+    """The same sequences with slots for `tokens` tokens, the added ones without a page: work is shared by that bound."""
+    q, kn, vn, p, tabs, lens, par = args
+    page = p[0].shape[2]
+    more = torch.full((tabs.shape[0], max(0, -(-tokens // page) - tabs.shape[1])), -1, dtype=tabs.dtype)
+    return q, kn, vn, p, torch.cat([tabs, more], 1), lens, par
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D,lens,page,dt,cu", [
+    (1, 4, 2, 64, [300, 0, 77], 16, F16, 3), (5, 8, 2, 128, [200, 130], 64, BF16, 2), (3, 2, 1, 96, [500, 1], 32, BF16, 4),
+    (20, 1, 1, 64, [333], 16, F16, 2), (2, 8, 1, 256, [260, 90], 64, BF16, 5)])
+def test_shares_of_few_rows(sim, T, Hq, Hkv, D, lens, page, dt, cu):  # noqa: F811
+    """Workers that share (sequence, key head)s, and the unshared form, of the same rows."""
+    args = attn_inputs(T + D, len(lens), T, Hq, Hkv, D, lens, page, dt)
+    for more in (0, 1700):
+        run_attn(sim, widened(args, more), num_cu=cu)
 
 
 def test_finite_scores_far_apart(sim):  # noqa: F811

@@ -93,8 +93,8 @@ def test_attention_many_rows(sim, T, Hq, Hkv, D, lens, page, dt):  # noqa: F811
 
 
 @pytest.mark.parametrize("T,Hq,Hkv,lens,max_len,cu", [
-    (1, 2, 2, [1500, 3, 611], None, 3),   # shares that start and end inside sequences
-    (2, 4, 1, [1240], None, 7),
+    (1, 2, 2, [1700, 3, 611], None, 3),   # shares that start and end inside sequences
+    (2, 4, 1, [1640], None, 7),
     (40, 1, 1, [900], None, 2),           # the same with tiles in LDS
     (33, 8, 1, [700], None, 16),          # and two groups of rows, eight workers each
     (1, 2, 1, [1000], 20, 3),             # a bound of the lengths that is too low changes nothing

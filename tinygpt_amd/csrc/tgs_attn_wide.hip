@@ -25,6 +25,12 @@ AttnPlan attn_plan(int M, int D, bool e8) {
     p.QB = M <= 16 ? 16 : 32;
     p.per_cu = D == 256 ? 1 : 2;
     p.least = 4;  // one per wave
+    // 8-bit caches, one workgroup each against shares and a join (us): 1015 tokens, D =
+    // 128, 1 sequence 10.6 : 12.8, 8 11.6 : 16.3, 64 26.2 : 30.8; 1527 13.6 : 13.0, 14.6 :
+    // 15.9, 35.8 : 40.7; 100 to 1460 tokens, 17 sequences with 8 nodes 16.5 : 23.3, 128 54
+    // : 73; D = 256, where a CU has one workgroup, 1000 tokens 18.1 : 16.2.  (A 16-bit
+    // cache's sums keep the order that they have.)
+    p.whole = e8 && D <= 128 ? 25 : 8;
   } else {
     p.wide = 1;
     p.tile = attn::WideGeo::TILE;
@@ -33,6 +39,7 @@ AttnPlan attn_plan(int M, int D, bool e8) {
     p.QB = D == 256 || M <= 128 ? 128 : 256;
     p.per_cu = D == 256 || p.QB == 256 ? 1 : 2;
     p.least = 4;
+    p.whole = 8;
   }
   p.nqb = (M + p.QB - 1) / p.QB;
   return p;

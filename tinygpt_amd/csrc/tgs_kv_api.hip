@@ -217,7 +217,7 @@ int attention(tgs_ctx* h, const tgs_kv_cache& cache, const uint8_t* scales, int6
   const int64_t len = std::min<int64_t>(attn->max_len, (int64_t)a.P * cache.page);
   const int64_t per = (len + p.tile - 1) / p.tile + (T + p.tile - 1) / p.tile;
   int64_t n = 0;
-  if (per > 2 * p.least) {
+  if (per > p.whole) {
     n = std::min<int64_t>((int64_t)h->num_cu * p.per_cu / p.nqb, (per * B * a.Hkv + p.least - 1) / p.least);
     const int64_t part = (int64_t)2 * p.QB * (D + 2) * p.nqb;  // floats
     n = std::min(n, (int64_t)h->ws_words * 2 / part);
