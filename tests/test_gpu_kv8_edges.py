@@ -24,7 +24,7 @@ def test_unseen_garbage(sampler, shape):
         H.log(f"8-bit attention, garbage in unseen nodes {shape} {dt} chain={chain}")
         lse = torch.empty(q.shape[:3], device=DEV)
         _, (k, v, s) = pools(p)
-        for more in (0, 1700):
+        for more in (0, 6000):
             slots = dev(widened(args, more)[4])
             out = sampler.tree_attention(dev(q), dev(kn), dev(vn), k, v, slots, dev(lens), parents=dev(par), lse=lse, scales=s)
             torch.cuda.synchronize()
@@ -37,7 +37,7 @@ def test_unseen_garbage(sampler, shape):
 def test_shares_of_few_rows(sampler, T, Hq, Hkv, D, lens, page, dt):
     """Workers that share (sequence, key head)s, and the unshared form, of the same rows."""
     args = attn_inputs(T + D, len(lens), T, Hq, Hkv, D, lens, page, dt)
-    for more in (0, 1700):
+    for more in (0, 6000):
         run_attn(sampler, widened(args, more))
 
 

@@ -35,7 +35,7 @@ def check_unseen(out, lse, args):
 def test_unseen_garbage(sim, shape, chain):  # noqa: F811
     args = unseen_garbage(*shape, chain=chain)
     q, kn, vn, p, tabs, lens, par = args
-    for more in (0, 1700):
+    for more in (0, 6000):
         wide = widened(args, more)[4]
         rc, out, lse = K.sim_attention(sim, q, kn, vn, p, wide, lens, par, None)
         assert rc == 0
@@ -56,7 +56,7 @@ def widened(args, tokens):
 def test_shares_of_few_rows(sim, T, Hq, Hkv, D, lens, page, dt, cu):  # noqa: F811
     """Workers that share (sequence, key head)s, and the unshared form, of the same rows."""
     args = attn_inputs(T + D, len(lens), T, Hq, Hkv, D, lens, page, dt)
-    for more in (0, 1700):
+    for more in (0, 6000):
         run_attn(sim, widened(args, more), num_cu=cu)
 
 

@@ -93,7 +93,7 @@ def test_attention_many_rows(sim, T, Hq, Hkv, D, lens, page, dt):  # noqa: F811
 
 
 @pytest.mark.parametrize("T,Hq,Hkv,lens,max_len,cu", [
-    (1, 2, 2, [1700, 3, 611], None, 3),   # shares that start and end inside sequences
+    (1, 2, 2, [1700, 3, 611], None, 4),   # shares that start and end inside sequences
     (2, 4, 1, [1640], None, 7),
     (40, 1, 1, [900], None, 2),           # the same with tiles in LDS
     (33, 8, 1, [700], None, 16),          # and two groups of rows, eight workers each

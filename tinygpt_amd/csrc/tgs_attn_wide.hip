@@ -28,9 +28,13 @@ AttnPlan attn_plan(int M, int D, bool e8) {
     // 8-bit caches, one workgroup each against shares and a join (us): 1015 tokens, D =
     // 128, 1 sequence 10.6 : 12.8, 8 11.6 : 16.3, 64 26.2 : 30.8; 1527 13.6 : 13.0, 14.6 :
     // 15.9, 35.8 : 40.7; 100 to 1460 tokens, 17 sequences with 8 nodes 16.5 : 23.3, 128 54
-    // : 73; D = 256, where a CU has one workgroup, 1000 tokens 18.1 : 16.2.  (A 16-bit
-    // cache's sums keep the order that they have.)
+    // : 73; D = 256, where a CU has one workgroup, 1000 tokens 18.1 : 16.2.  Where there
+    // are several for each worker, a long one among short ones is hidden by the others:
+    // 128 sequences of 100 to 4096 tokens, 8 nodes, 119 : 133, of 400 and one of 4096 49 :
+    // 53, of 2500 with one node 103 : 110.  (A 16-bit cache's sums keep the order that
+    // they have.)
     p.whole = e8 && D <= 128 ? 25 : 8;
+    p.round = e8 && D <= 128 ? 33 : 0;
   } else {
     p.wide = 1;
     p.tile = attn::WideGeo::TILE;
@@ -40,6 +44,7 @@ AttnPlan attn_plan(int M, int D, bool e8) {
     p.per_cu = D == 256 || p.QB == 256 ? 1 : 2;
     p.least = 4;
     p.whole = 8;
+    p.round = 0;
   }
   p.nqb = (M + p.QB - 1) / p.QB;
   return p;

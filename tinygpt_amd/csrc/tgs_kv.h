@@ -140,6 +140,7 @@ struct AttnPlan {
   int per_cu;  // workgroups that a CU holds
   int least;   // tiles worth a worker of their own
   int whole;   // tiles of a (sequence, key head) up to which it is one workgroup's
+  int round;   // the same for each of them that a worker would have
 };
 AttnPlan attn_plan(int M, int D, bool e8);
 hipError_t launch_attn(const AttnArgs& a, const AttnPlan& p, int dtype, hipStream_t st);

@@ -216,9 +216,10 @@ int attention(tgs_ctx* h, const tgs_kv_cache& cache, const uint8_t* scales, int6
   // key head) is short, one workgroup each and no join.
   const int64_t len = std::min<int64_t>(attn->max_len, (int64_t)a.P * cache.page);
   const int64_t per = (len + p.tile - 1) / p.tile + (T + p.tile - 1) / p.tile;
+  const int64_t most = (int64_t)h->num_cu * p.per_cu / p.nqb;
   int64_t n = 0;
-  if (per > p.whole) {
-    n = std::min<int64_t>((int64_t)h->num_cu * p.per_cu / p.nqb, (per * B * a.Hkv + p.least - 1) / p.least);
+  if (per > std::max<int64_t>(p.whole, p.round * ((int64_t)B * a.Hkv / std::max<int64_t>(most, 1)))) {
+    n = std::min<int64_t>(most, (per * B * a.Hkv + p.least - 1) / p.least);
     const int64_t part = (int64_t)2 * p.QB * (D + 2) * p.nqb;  // floats
     n = std::min(n, (int64_t)h->ws_words * 2 / part);
     if (p.nqb > 1 && n >= 8) n = n / 8 * 8;  // (row groups of a worker on one XCD)
